@@ -320,6 +320,109 @@ int t5e_tcgen05_sparse_cases(int32_t kind, uint32_t idesc, int32_t meta_layout, 
                              const uint32_t* c, const uint32_t* meta, const uint32_t* scales, uint32_t* d,
                              int32_t* disagree, uint32_t* dump, uint64_t cases, int32_t* error, void* stream);
 
+/* ---- block-scaled E2M1 tensors (no counterpart in the reference, which takes
+ * raw words only): real tensors to the operands of the MXF4, MXF4NVF4 and
+ * NVFP4 instructions, back, and their matrix product. ---- */
+
+/* types of real tensors */
+enum { T5E_REAL_F32 = 0, T5E_REAL_BF16 = 1, T5E_REAL_F16 = 2 };
+
+/* rounding of UE8M0 scales; UE4M3 scales take T5E_SCALE_ROUND_NEAREST */
+enum { T5E_SCALE_ROUND_NEAREST = 0, T5E_SCALE_ROUND_FLOOR = 1, T5E_SCALE_ROUND_CEIL = 2 };
+
+/*
+ * Rows of E2M1 codes with a scale per block of scale_block elements (16 or
+ * 32, the last block of a row may be short): what the packed rows of t5e_batch
+ * are for one format, with tiled scales.
+ *   data: rows of `stride` bytes, element i of a row in bits [4i, 4i+4); stride
+ *     a multiple of 16, data 16-byte aligned; codes from k up to the next
+ *     multiple of 32 are zero.
+ *   scales: bytes in tiles of 128 rows by 4 blocks, 512 bytes a tile, tiles
+ *     of a row of tiles consecutive (groups = ceil(ceil(k/scale_block)/4) of
+ *     them): the scale of block b of row r is byte
+ *     ((r/128)*groups + b/4)*512 + (r%32)*16 + (r%128)/32*4 + b%4;
+ *     16-byte aligned; blocks behind the last one are zero in every row r <
+ *     rows, rows behind the last one hold anything.
+ * k is 1..T5E_MAX_BLOCK_K and rows 0..T5E_MAX_BLOCK_ROWS.
+ * scale_format/scale_block: T5E_SCALE_UE4M3 with 16, T5E_SCALE_UE8M0 with 16
+ * or 32 (make_model's scaling and scale_vec 4 or 2).
+ */
+#define T5E_MAX_BLOCK_K (1ll << 28)
+#define T5E_MAX_BLOCK_ROWS (1ull << 30)
+typedef struct t5e_blocks {
+    void* data;
+    int64_t stride;
+    void* scales;
+    uint64_t rows;
+    int64_t k;
+    int32_t scale_format;
+    int32_t scale_block;
+} t5e_blocks;
+
+/* Partial maxima of |x| (F32 bits) over a [rows, cols] tensor with row stride
+ * `stride` (elements): `count` words, 1..T5E_MAX_PARTIALS, all written. */
+#define T5E_MAX_PARTIALS 1024
+int t5e_block_partials(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
+                       int32_t count, void* stream);
+
+/* multiplier[0] = the largest power of two m, 2^-126..2^126, with
+ * m * max|x| <= 6 * 448, from those partial maxima; 1 where max|x| is zero or
+ * not finite. */
+int t5e_block_multiplier(const uint32_t* partials, int32_t count, float* multiplier, void* stream);
+
+/* Rounds x [rows, cols] (row stride in elements) to blocks along its rows
+ * (by_rows: rows = rows, k = cols), along its columns (by_cols: rows = cols,
+ * k = rows), or both; the pointer of the one not wanted is NULL.
+ *   u = F32(x * m), m = *multiplier or 1 (NULL); a = max|u| of a block;
+ *   UE4M3: scale = RNE(min(a / 6, 448)); UE8M0: 2^(floor(log2 a) - 2) or
+ *   (CEIL) the smallest power of two >= a / 6, held to 2^+-127;
+ *   code = RNE(u / scale) of the real quotient, magnitudes above 6 become 6.
+ * A block with a NaN or an infinity gets the NaN scale and codes 0; a zero
+ * scale gets codes that are zeros.  With partials != NULL the multiplier is
+ * taken from those partial maxima (t5e_block_partials of the same x) and
+ * stored to *multiplier. */
+int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, int32_t rounding,
+                        float* multiplier, const uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
+                        const t5e_blocks* by_cols, void* stream);
+
+/* out[r][i] = code * scale * F32(1 / m) rounded to `type`; out_stride in
+ * elements. */
+int t5e_dequantize_blocks(const t5e_blocks* blocks, const float* multiplier, int32_t type, void* out,
+                          int64_t out_stride, void* stream);
+
+/*
+ * The matrix product of block-scaled rows on the tensor cores:
+ *   D[i][j] = alpha * F32(1/ma) * F32(1/mb) * sum_k a[i][k] b[j][k] + C[i][j]
+ * a has m rows, b n rows (the columns of B), with equal k, scale format and
+ * scale block.  The sum is the instruction's: F32 accumulators, K in
+ * ascending steps of 64 (in parts that are joined in F32 where the call
+ * splits K).  c (NULL: none) is of type c_type with strides in elements (0
+ * broadcasts); d is of type d_type with row stride d_stride and unit column
+ * stride; c may be d.  split: 0 lets the library choose, 1, 2, 4 or 8 parts.
+ * If a bounded wait inside the kernel runs out, the tile becomes NaN and
+ * t5e_block_scaled_mm_expired reports it.
+ */
+typedef struct t5e_block_mm {
+    const t5e_blocks* a;
+    const t5e_blocks* b;
+    const float* multiplier_a;   /* device scalars or NULL (1) */
+    const float* multiplier_b;
+    float alpha;
+    int32_t split;
+    const void* c;
+    int32_t c_type;
+    int32_t d_type;
+    int64_t c_row_stride;
+    int64_t c_col_stride;
+    void* d;
+    int64_t d_stride;
+} t5e_block_mm;
+int t5e_block_scaled_mm(const t5e_block_mm* mm, void* stream);
+
+/* *expired = 1 if a wait of t5e_block_scaled_mm ran out on the current device
+ * since the library was loaded; synchronizes the device. */
+int t5e_block_scaled_mm_expired(int32_t* expired);
+
 #ifdef __cplusplus
 }
 #endif

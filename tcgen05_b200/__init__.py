@@ -7,8 +7,22 @@ keep the reference's signatures and errors; ``mma_dot_batch`` and
 ``mma_batch`` evaluate millions of independent dot products or tiles per
 kernel launch.  Every result word is computed by hand-written integer CUDA
 kernels in ``tcgen05_b200/_lib/libt5e.so``; there is no CPU fallback.
+
+Real tensors meet that arithmetic in ``quantize_blocks`` (tensors to
+block-scaled E2M1 rows: the operands of the MXF4, MXF4NVF4 and NVFP4
+instructions), ``dequantize_blocks``, ``block_scaled_mm`` (their matrix product
+on the tensor cores) and ``block_scaled_linear`` (a linear layer with its
+gradients).
 """
 
+from .blocks import (
+    BlockScaledRows,
+    block_multiplier,
+    block_scaled_linear,
+    block_scaled_mm,
+    dequantize_blocks,
+    quantize_blocks,
+)
 from .formats import bits_to_f32, f32_to_bits
 from .model import (
     DotProduct,
@@ -23,6 +37,7 @@ from .model import (
 from .simulator import PackedRows, PendingBatch, mma, mma_batch, mma_dot, mma_dot_batch, sparse_active_indices
 
 __all__ = [
+    "BlockScaledRows",
     "DotProduct",
     "PackedRows",
     "PendingBatch",
@@ -32,6 +47,10 @@ __all__ = [
     "Tcgen05MixedRawWindowMmaModel",
     "Tcgen05RawWindowNvfp4MmaModel",
     "bits_to_f32",
+    "block_multiplier",
+    "block_scaled_linear",
+    "block_scaled_mm",
+    "dequantize_blocks",
     "f32_to_bits",
     "make_model",
     "mma",
@@ -39,5 +58,6 @@ __all__ = [
     "mma_dot",
     "mma_dot_batch",
     "normalize_format",
+    "quantize_blocks",
     "sparse_active_indices",
 ]

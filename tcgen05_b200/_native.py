@@ -53,6 +53,13 @@ MAX_K = 65536
 # bytes of the static device array t5e_mma_dot_batch_noalloc stages batches in
 NOALLOC_STAGE_BYTES = 32 * 1024 * 1024
 
+# block-scaled tensors
+REAL_F32, REAL_BF16, REAL_F16 = 0, 1, 2
+SCALE_ROUND_NEAREST, SCALE_ROUND_FLOOR, SCALE_ROUND_CEIL = 0, 1, 2
+MAX_PARTIALS = 1024
+MAX_BLOCK_K = 1 << 28
+MAX_BLOCK_ROWS = 1 << 30
+
 CASE_OK, CASE_BAD_SELECTOR, CASE_EMPTY, CASE_SCALE_COVER, CASE_META_WORDS, CASE_TIMEOUT = 0, 1, 2, 3, 4, 5
 
 
@@ -106,6 +113,40 @@ class Batch(ctypes.Structure):
     ]
 
 
+class Blocks(ctypes.Structure):
+    """t5e_blocks: rows of E2M1 codes with tiled block scales."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("stride", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("k", ctypes.c_int64),
+        ("scale_format", ctypes.c_int32),
+        ("scale_block", ctypes.c_int32),
+    ]
+
+
+class BlockMm(ctypes.Structure):
+    """t5e_block_mm: one product of block-scaled rows."""
+
+    _fields_ = [
+        ("a", ctypes.POINTER(Blocks)),
+        ("b", ctypes.POINTER(Blocks)),
+        ("multiplier_a", ctypes.c_void_p),
+        ("multiplier_b", ctypes.c_void_p),
+        ("alpha", ctypes.c_float),
+        ("split", ctypes.c_int32),
+        ("c", ctypes.c_void_p),
+        ("c_type", ctypes.c_int32),
+        ("d_type", ctypes.c_int32),
+        ("c_row_stride", ctypes.c_int64),
+        ("c_col_stride", ctypes.c_int64),
+        ("d", ctypes.c_void_p),
+        ("d_stride", ctypes.c_int64),
+    ]
+
+
 # every symbol include/t5e.h declares
 EXPORTED = (
     "t5e_abi_version",
@@ -121,6 +162,12 @@ EXPORTED = (
     "t5e_tcgen05_tiles",
     "t5e_tcgen05_block_scaled_tiles",
     "t5e_tcgen05_sparse_cases",
+    "t5e_block_partials",
+    "t5e_block_multiplier",
+    "t5e_quantize_blocks",
+    "t5e_dequantize_blocks",
+    "t5e_block_scaled_mm",
+    "t5e_block_scaled_mm_expired",
 )
 
 _lib = None
@@ -177,6 +224,23 @@ def load() -> ctypes.CDLL:
     lib.t5e_tcgen05_sparse_cases.restype = ctypes.c_int
     lib.t5e_tcgen05_sparse_cases.argtypes = [ctypes.c_int32, ctypes.c_uint32, ctypes.c_int32] + [ctypes.c_void_p] * 8 \
         + [ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p]
+    lib.t5e_block_partials.restype = ctypes.c_int
+    lib.t5e_block_partials.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
+                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
+    lib.t5e_block_multiplier.restype = ctypes.c_int
+    lib.t5e_block_multiplier.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+    lib.t5e_quantize_blocks.restype = ctypes.c_int
+    lib.t5e_quantize_blocks.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
+                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+                                        ctypes.c_int32, ctypes.POINTER(Blocks), ctypes.POINTER(Blocks),
+                                        ctypes.c_void_p]
+    lib.t5e_dequantize_blocks.restype = ctypes.c_int
+    lib.t5e_dequantize_blocks.argtypes = [ctypes.POINTER(Blocks), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+                                          ctypes.c_int64, ctypes.c_void_p]
+    lib.t5e_block_scaled_mm.restype = ctypes.c_int
+    lib.t5e_block_scaled_mm.argtypes = [ctypes.POINTER(BlockMm), ctypes.c_void_p]
+    lib.t5e_block_scaled_mm_expired.restype = ctypes.c_int
+    lib.t5e_block_scaled_mm_expired.argtypes = [ctypes.POINTER(ctypes.c_int32)]
     version = lib.t5e_abi_version()
     if version != ABI_VERSION:
         raise NativeLibraryError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")

@@ -1,0 +1,493 @@
+"""Block-scaled E2M1 tensors: the operands of the MXF4, MXF4NVF4 and NVFP4
+instructions made from real tensors, turned back, and multiplied.
+
+``quantize_blocks`` rounds a CUDA tensor to E2M1 codes with one 8-bit scale per
+block of 16 or 32 consecutive elements; the result, ``BlockScaledRows``, feeds
+the emulator (``packed()`` and ``scale_words()`` are what ``mma_dot_batch``
+takes) as well as ``block_scaled_mm``, which multiplies two of them on the
+tensor cores.  ``dequantize_blocks`` gives the real values back and
+``block_scaled_linear`` is a linear layer whose three products (output, input
+gradient, weight gradient) all run in this arithmetic.
+
+``scaling`` and ``scale_vec`` are make_model's: "ue4m3" with 4 (blocks of 16,
+NVFP4), "ue8m0" with 2 (blocks of 32, MXF4) or 4 (blocks of 16).  Everything
+runs on the current stream of the tensors' device, allocates its results and
+workspaces there per call and keeps nothing between calls, so calls may run
+side by side on several streams and be captured into CUDA graphs.  There is no
+CPU fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as nat
+from . import packing
+from .simulator import PackedRows
+
+_REAL = {torch.float32: nat.REAL_F32, torch.bfloat16: nat.REAL_BF16, torch.float16: nat.REAL_F16}
+# (scaling, scale_vec) -> (scale format, elements per block)
+_FORMS = {
+    ("ue4m3", 4): (nat.SCALE_UE4M3, 16),
+    ("ue8m0", 2): (nat.SCALE_UE8M0, 32),
+    ("ue8m0", 4): (nat.SCALE_UE8M0, 16),
+}
+_ROUNDINGS = {"nearest": nat.SCALE_ROUND_NEAREST, "floor": nat.SCALE_ROUND_FLOOR, "ceil": nat.SCALE_ROUND_CEIL}
+
+
+def _form(scaling, scale_vec) -> tuple[str, int]:
+    scaling = str(scaling).lower()
+    if scale_vec is None:
+        scale_vec = 4 if scaling == "ue4m3" else 2
+    if (scaling, scale_vec) not in _FORMS:
+        raise ValueError(f"block-scaled E2M1 takes scaling 'ue4m3' with scale_vec 4 or 'ue8m0' with 2 or 4, "
+                         f"not {scaling!r} with {scale_vec!r}")
+    return scaling, scale_vec
+
+
+def _rounding(scaling: str, scale_rounding) -> int:
+    if scale_rounding is None:
+        scale_rounding = "nearest" if scaling == "ue4m3" else "floor"
+    if scale_rounding not in _ROUNDINGS or (scale_rounding == "nearest") != (scaling == "ue4m3"):
+        raise ValueError(f"scale_rounding is 'floor' or 'ceil' for ue8m0 and 'nearest' for ue4m3, "
+                         f"not {scale_rounding!r} for {scaling}")
+    return _ROUNDINGS[scale_rounding]
+
+
+def tile_scales(words: torch.Tensor) -> torch.Tensor:
+    """[rows, blocks] scale bytes -> the tiles of t5e_blocks (include/t5e.h):
+    [ceil(rows / 128), ceil(blocks / 4), 512] bytes, zeros where no block is."""
+    if words.dim() != 2 or words.dtype != torch.uint8:
+        raise ValueError("scale words are a [rows, blocks] uint8 tensor")
+    rows, blocks = words.shape
+    full = torch.zeros((rows + 127) // 128 * 128, (blocks + 3) // 4 * 4, dtype=torch.uint8, device=words.device)
+    full[:rows, :blocks] = words
+    tiles = full.view(full.shape[0] // 128, 4, 32, full.shape[1] // 4, 4).permute(0, 3, 2, 1, 4)
+    return tiles.reshape(full.shape[0] // 128, full.shape[1] // 4, 512)
+
+
+def untile_scales(tiles: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
+    """Inverse of tile_scales."""
+    t = tiles.reshape(tiles.shape[0], tiles.shape[1], 32, 4, 4).permute(0, 3, 2, 1, 4)
+    return t.reshape(tiles.shape[0] * 128, tiles.shape[1] * 4)[:rows, :blocks].contiguous()
+
+
+class BlockScaledRows:
+    """Rows of E2M1 codes with a scale per block: what PackedRows are for one
+    format, with scales.
+
+    ``data`` is a [rows, stride] uint8 tensor of packed rows (stride a multiple
+    of 16, at least ``row_stride(k)``; codes behind k, up to the next multiple
+    of 32, zero), ``scales`` the tiled scale bytes (``tile_scales``),
+    ``multiplier`` a one-element float32 tensor that the values were
+    multiplied by before rounding, or None: element i of row r stands for
+    code * scale / multiplier."""
+
+    __slots__ = ("data", "scales", "k", "scaling", "scale_vec", "multiplier")
+
+    def __init__(self, data, scales, k: int, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
+        scaling, scale_vec = _form(scaling, scale_vec)
+        k = int(k)
+        if not 1 <= k <= nat.MAX_BLOCK_K:
+            raise ValueError(f"K={k} outside 1..{nat.MAX_BLOCK_K}")
+        if data.dim() != 2 or data.dtype != torch.uint8 or (data.shape[0] and not data.is_contiguous()):
+            raise ValueError("data must be a contiguous [rows, stride] uint8 tensor")
+        if data.shape[0] > nat.MAX_BLOCK_ROWS:
+            raise ValueError(f"more than {nat.MAX_BLOCK_ROWS} rows")
+        if data.shape[1] % 16 or data.shape[1] < self.row_stride(k):
+            raise ValueError(f"row stride {data.shape[1]} is not a multiple of 16 of at least {self.row_stride(k)}")
+        tiles = (data.shape[0] + 127) // 128
+        groups = -(-k // (4 * _FORMS[scaling, scale_vec][1]))
+        if scales.dtype != torch.uint8 or tuple(scales.shape) != (tiles, groups, 512) or not scales.is_contiguous():
+            raise ValueError(f"scales must be a contiguous [{tiles}, {groups}, 512] uint8 tensor (tile_scales)")
+        if scales.device != data.device:
+            raise ValueError("data and scales are on different devices")
+        if multiplier is not None:
+            if multiplier.dtype != torch.float32 or multiplier.numel() != 1 or multiplier.device != data.device:
+                raise ValueError("multiplier must be a one-element float32 tensor on the data's device")
+        if data.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("data and scales must start on 16-byte boundaries")
+        self.data, self.scales, self.k = data, scales, k
+        self.scaling, self.scale_vec, self.multiplier = scaling, scale_vec, multiplier
+
+    @classmethod
+    def _made(cls, data, scales, k, scaling, scale_vec, multiplier):
+        """An instance whose parts are known to fit."""
+        self = cls.__new__(cls)
+        self.data, self.scales, self.k = data, scales, k
+        self.scaling, self.scale_vec, self.multiplier = scaling, scale_vec, multiplier
+        return self
+
+    @classmethod
+    def from_words(cls, words, scales, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
+        """From a [rows, K] CUDA tensor of raw E2M1 container words and
+        [rows, blocks] scale bytes, as ``mma_dot_batch`` takes them."""
+        scaling, scale_vec = _form(scaling, scale_vec)
+        if words.dim() != 2:
+            raise ValueError("words must be a [rows, K] tensor of words")
+        rows, k = words.shape
+        blocks = -(-k // _FORMS[scaling, scale_vec][1])
+        if tuple(scales.shape) != (rows, blocks):
+            raise ValueError(f"scales must be [{rows}, {blocks}] bytes")
+        data = packing.pack_rows_device(words, nat.FMT_E2M1, cls.row_stride(k))
+        return cls(data, tile_scales(scales), k, scaling=scaling, scale_vec=scale_vec, multiplier=multiplier)
+
+    @staticmethod
+    def row_stride(k: int) -> int:
+        """Smallest row stride in bytes: whole groups of 32 elements."""
+        return (k + 31) // 32 * 16
+
+    @property
+    def rows(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def block(self) -> int:
+        """Elements per scale."""
+        return _FORMS[self.scaling, self.scale_vec][1]
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def packed(self) -> PackedRows:
+        """The codes as the emulator's operand rows."""
+        return PackedRows(self.data, self.k)
+
+    def scale_words(self) -> torch.Tensor:
+        """[rows, blocks] scale bytes, as the emulator takes them."""
+        return untile_scales(self.scales, self.rows, -(-self.k // self.block))
+
+    def _struct(self) -> nat.Blocks:
+        fmt, block = _FORMS[self.scaling, self.scale_vec]
+        return nat.Blocks(self.data.data_ptr(), self.data.shape[1], self.scales.data_ptr(), self.data.shape[0], self.k,
+                          fmt, block)
+
+    def __repr__(self):
+        return (f"BlockScaledRows({self.rows} x {self.k}, {self.scaling}, scale_vec={self.scale_vec}, "
+                f"device={self.device})")
+
+
+class _On:
+    """Makes `device` current for a library call, and gives its current stream."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _real_tensor(x, name: str):
+    if not isinstance(x, torch.Tensor):
+        raise ValueError(f"{name} must be a torch tensor")
+    if x.dtype not in _REAL:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device (there is no CPU fallback)")
+
+
+def _matrix_of(x):
+    """(matrix, turned): x as rows of its last dimension with unit column
+    stride, or `turned`, the matrix whose columns those rows are (no copy of a
+    transposed matrix); other layouts are copied."""
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    rows, cols = m.shape
+    if (m.stride(1) == 1 or cols == 1) and (rows == 1 or m.stride(0) >= cols):
+        return m, False
+    if m.stride(0) == 1 and m.stride(1) >= rows:
+        return m.t(), True
+    return m.contiguous(), False
+
+
+def _partials(m, handle, lib):
+    count = max(1, min(592, -(-m.numel() // 8192)))
+    partials = torch.empty(count, dtype=torch.int32, device=m.device)
+    nat.check(lib.t5e_block_partials(_REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0),
+                                     partials.data_ptr(), count, handle), "t5e_block_partials")
+    return partials, count
+
+
+def block_multiplier(x) -> torch.Tensor:
+    """The power of two that ``quantize_blocks(x, multiplier="auto")``
+    multiplies by: the largest m, within 2^-126..2^126, for which every
+    |x| * m <= 6 * 448, so that UE4M3 scales use their whole range; 1 where the
+    largest |x| is zero or not finite.  A one-element float32 tensor, computed
+    without a synchronization."""
+    _real_tensor(x, "x")
+    if x.dim() == 0:
+        x = x.reshape(1)
+    out = torch.empty(1, dtype=torch.float32, device=x.device)
+    lib = nat.load()
+    if x.numel() == 0:
+        return out.fill_(1.0)
+    with _On(x.device) as handle:
+        m, _ = _matrix_of(x.detach())
+        partials, count = _partials(m, handle, lib)
+        nat.check(lib.t5e_block_multiplier(partials.data_ptr(), count, out.data_ptr(), handle), "t5e_block_multiplier")
+    return out
+
+
+def _empty_blocks(rows, k, scaling, scale_vec, multiplier, device):
+    data = torch.empty((rows, BlockScaledRows.row_stride(k)), dtype=torch.uint8, device=device)
+    groups = -(-k // (4 * _FORMS[scaling, scale_vec][1]))
+    scales = torch.empty(((rows + 127) // 128, groups, 512), dtype=torch.uint8, device=device)
+    return BlockScaledRows._made(data, scales, k, scaling, scale_vec, multiplier)
+
+
+def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None = None,
+                    scale_rounding: str | None = None, multiplier=None):
+    """Round a CUDA tensor (float32, bfloat16 or float16, any strides, at least
+    one dimension) to block-scaled E2M1 rows.
+
+    ``x`` is taken as a matrix of its last dimension [R, K].  ``axis=-1``
+    rounds blocks along its rows (a BlockScaledRows of R rows and K elements),
+    ``axis=0`` along its columns (K rows of R elements: the transposed
+    operand), ``axis="both"`` returns the pair from one call.
+
+    With u = x * multiplier rounded to float32 and a = max |u| of a block: a
+    UE4M3 scale is a / 6 rounded to nearest (at most 448); a UE8M0 scale is
+    2^(floor(log2 a) - 2) ("floor", the default) or the smallest power of two
+    not below a / 6 ("ceil", nothing exceeds the E2M1 range).  Codes are u /
+    scale rounded to nearest even, magnitudes above 6 become 6; both roundings
+    are those of the real quotients.  A block that holds a NaN or an infinity
+    gets the NaN scale, and everything computed from it is NaN.
+
+    ``multiplier``: None (1), a positive float, a one-element float32 tensor, or
+    "auto", ``block_multiplier(x)`` found in the same call.  The result carries
+    no gradient (see ``block_scaled_linear``)."""
+    scaling, scale_vec = _form(scaling, scale_vec)
+    rounding = _rounding(scaling, scale_rounding)
+    if axis not in (-1, 0, "both"):
+        raise ValueError(f"axis is -1, 0 or 'both', not {axis!r}")
+    if isinstance(multiplier, str) and multiplier != "auto":
+        raise ValueError(f"multiplier is a number, a tensor, 'auto' or None, not {multiplier!r}")
+    if isinstance(multiplier, (int, float)) and not 0 < multiplier < float("inf"):
+        raise ValueError(f"multiplier must be positive and finite, not {multiplier!r}")
+    _real_tensor(x, "x")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("x must have at least one dimension and a non-empty last one")
+    if isinstance(multiplier, torch.Tensor) and (multiplier.dtype != torch.float32 or multiplier.numel() != 1
+                                                 or multiplier.device != x.device):
+        raise ValueError("multiplier must be a one-element float32 tensor on x's device")
+    k = x.shape[-1]
+    r = x.numel() // k
+    by_rows, by_cols = axis in (-1, "both"), axis in (0, "both")
+    if by_cols and r == 0:
+        raise ValueError("blocks along an empty axis")
+    if (by_rows and k > nat.MAX_BLOCK_K) or (by_cols and r > nat.MAX_BLOCK_K) or max(r, k) > nat.MAX_BLOCK_ROWS:
+        raise ValueError(f"x is larger than {nat.MAX_BLOCK_K} elements along a block axis or {nat.MAX_BLOCK_ROWS} rows")
+    lib = nat.load()
+    with _On(x.device) as handle:
+        m, turned = _matrix_of(x.detach())
+        partials, count = None, 0
+        if isinstance(multiplier, str):
+            if m.numel():
+                partials, count = _partials(m, handle, lib)
+            multiplier = torch.empty(1, dtype=torch.float32, device=x.device) if m.numel() else None
+        elif isinstance(multiplier, (int, float)):
+            multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=x.device)
+        rows = _empty_blocks(r, k, scaling, scale_vec, multiplier, x.device) if by_rows else None
+        cols = _empty_blocks(k, r, scaling, scale_vec, multiplier, x.device) if by_cols else None
+        along, across = (cols, rows) if turned else (rows, cols)
+        nat.check(lib.t5e_quantize_blocks(
+            _REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0), rounding,
+            None if multiplier is None else multiplier.data_ptr(),
+            None if partials is None else partials.data_ptr(), count,
+            None if along is None else ctypes.byref(along._struct()),
+            None if across is None else ctypes.byref(across._struct()), handle), "t5e_quantize_blocks")
+    if axis == "both":
+        return rows, cols
+    return rows if by_rows else cols
+
+
+def _check_blocks(q, name: str):
+    if not isinstance(q, BlockScaledRows):
+        raise ValueError(f"{name} must be BlockScaledRows")
+    if not q.data.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device (there is no CPU fallback)")
+
+
+def _result(out, shape, dtype, device):
+    """The result tensor: `out` checked, or a new one."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor on {device}")
+    if out.numel() and ((out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1])):
+        raise ValueError("out must have unit column stride and rows that do not overlap")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out must not require a gradient")
+    return out
+
+
+def dequantize_blocks(blocks: BlockScaledRows, *, dtype=torch.float32, out=None) -> torch.Tensor:
+    """The [rows, K] values code * scale / multiplier (times the reciprocal of
+    the multiplier, rounded to float32) rounded to ``dtype``; into ``out`` (unit
+    column stride) if given."""
+    _check_blocks(blocks, "blocks")
+    if dtype not in _REAL:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    out = _result(out, (blocks.rows, blocks.k), dtype, blocks.device)
+    lib = nat.load()
+    with _On(blocks.device) as handle:
+        m = blocks.multiplier
+        nat.check(lib.t5e_dequantize_blocks(ctypes.byref(blocks._struct()), None if m is None else m.data_ptr(),
+                                            _REAL[dtype], out.data_ptr(), out.stride(0) if blocks.rows > 1 else blocks.k,
+                                            handle), "t5e_dequantize_blocks")
+    return out
+
+
+def _span(t):
+    """[first, behind the last) byte of a tensor's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def block_scaled_mm(a: BlockScaledRows, b: BlockScaledRows, c=None, *, alpha: float = 1.0, dtype=torch.bfloat16,
+                    out=None) -> torch.Tensor:
+    """``D = alpha * A @ B.T + C`` on the tensor cores, in one kernel launch:
+    ``a`` [M, K] and ``b`` [N, K] block-scaled rows of the same form (b's rows
+    are the columns of B, as in the packed rows of ``mma_batch``); their
+    multipliers are divided out.  ``c``: a real tensor that broadcasts to
+    [M, N] (a bias, an accumulator), or None.  Returns [M, N] of ``dtype``, or
+    ``out`` (unit column stride), which may be ``c`` itself.
+
+    Sums are the instruction's own: float32 accumulators that take K in
+    ascending steps of 64, each step truncated as ``mma_dot_batch`` models it
+    word for word; where few tiles would leave the GPU idle, K is split into
+    parts that are joined in float32.  The result carries no gradient (see
+    ``block_scaled_linear``)."""
+    _check_blocks(a, "a")
+    _check_blocks(b, "b")
+    return _mm(a, b, c, alpha, dtype, out, 0)
+
+
+def _mm(a, b, c, alpha, dtype, out, split):
+    if (a.scaling, a.scale_vec) != (b.scaling, b.scale_vec):
+        raise ValueError(f"a and b have different forms: {a!r}, {b!r}")
+    if a.k != b.k:
+        raise ValueError(f"a has K={a.k} but b has K={b.k}")
+    if a.device != b.device:
+        raise ValueError("a and b are on different devices")
+    if dtype not in _REAL:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    shape = (a.rows, b.rows)
+    if c is not None:
+        _real_tensor(c, "c")
+        if c.device != a.device:
+            raise ValueError("c is on another device")
+        if c.requires_grad and torch.is_grad_enabled():
+            raise ValueError("block_scaled_mm gives c no gradient; detach it or use block_scaled_linear")
+        try:
+            c = c.detach().expand(shape)
+        except RuntimeError:
+            raise ValueError(f"c of shape {tuple(c.shape)} does not broadcast to {shape}") from None
+    given = out is not None
+    out = _result(out, shape, dtype, a.device)
+    if given and c is not None and out.numel():
+        (c0, c1), (d0, d1) = _span(c), _span(out)
+        same = c0 == d0 and c.dtype == out.dtype and all(n == 1 or s == t for n, s, t in
+                                                         zip(shape, c.stride(), out.stride()))
+        if c0 < d1 and d0 < c1 and not same:
+            raise ValueError("c overlaps out without being out")
+    lib = nat.load()
+    sa, sb = a._struct(), b._struct()
+    mm = nat.BlockMm()
+    mm.a, mm.b = ctypes.pointer(sa), ctypes.pointer(sb)
+    mm.multiplier_a = None if a.multiplier is None else a.multiplier.data_ptr()
+    mm.multiplier_b = None if b.multiplier is None else b.multiplier.data_ptr()
+    mm.alpha, mm.split = alpha, split
+    if c is not None:
+        mm.c, mm.c_type = c.data_ptr(), _REAL[c.dtype]
+        mm.c_row_stride, mm.c_col_stride = c.stride()
+    mm.d, mm.d_type = out.data_ptr(), _REAL[dtype]
+    mm.d_stride = out.stride(0) if shape[0] > 1 else shape[1]
+    with _On(a.device) as handle:
+        nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
+    return out
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, scaling, scale_vec, scale_rounding, need_x, need_w):
+        form = dict(scaling=scaling, scale_vec=scale_vec, scale_rounding=scale_rounding,
+                    multiplier="auto" if scaling == "ue4m3" else None)
+        flat = x.reshape(-1, x.shape[-1])
+        tokens = flat.shape[0]
+        # blocks run along the contraction: K here, the tokens and N in the
+        # gradients, so what a gradient needs is rounded along the other axis
+        qx, xt = quantize_blocks(flat, axis="both", **form) if need_w and tokens else (quantize_blocks(flat, **form), None)
+        qw, wt = quantize_blocks(w, axis="both", **form) if need_x and tokens else (quantize_blocks(w, **form), None)
+        y = _mm(qx, qw, None, 1.0, x.dtype, None, 0)
+        ctx.form, ctx.shapes, ctx.need = form, (x.shape, w.shape), (need_x, need_w)
+        saved = []
+        for q in (xt, wt):
+            saved += [None, None, None] if q is None else [q.data, q.scales, q.multiplier]
+        ctx.save_for_backward(*saved)
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (x_shape, w_shape), (need_x, need_w) = ctx.shapes, ctx.need
+        n, k = w_shape
+        flat = g.reshape(-1, n)
+        tokens = flat.shape[0]
+        dx = dw = None
+        if tokens == 0:
+            return (g.new_zeros(x_shape) if need_x else None, g.new_zeros(w_shape) if need_w else None,
+                    None, None, None, None, None)
+        form = ctx.form
+        kept = ctx.saved_tensors
+
+        def held(i, length):
+            return BlockScaledRows._made(kept[i], kept[i + 1], length, form["scaling"], form["scale_vec"], kept[i + 2])
+
+        axis = "both" if need_x and need_w else (-1 if need_x else 0)
+        q = quantize_blocks(flat, axis=axis, **form)
+        rows, cols = q if axis == "both" else ((q, None) if need_x else (None, q))
+        if need_x:
+            dx = _mm(rows, held(3, n), None, 1.0, g.dtype, None, 0).view(x_shape)
+        if need_w:
+            dw = _mm(cols, held(0, tokens), None, 1.0, g.dtype, None, 0)
+        return dx, dw, None, None, None, None, None
+
+
+def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None = None,
+                        scale_rounding: str | None = None) -> torch.Tensor:
+    """``x @ w.T`` with both rounded to block-scaled E2M1 rows, and its
+    gradients in the same arithmetic:
+
+        y  = Q(x) Q(w)^T           blocks along K
+        dx = Q(g) Q(w^T)^T         blocks along N
+        dw = Q(g^T) Q(x^T)^T       blocks along the tokens
+
+    (the rounding itself passes gradients straight through).  ``x`` [..., K]
+    and ``w`` [N, K] are CUDA tensors of one type; y, dx and dw have that type.
+    UE4M3 forms take the "auto" multiplier for x, w and g.  x and w are read
+    once each; a training step keeps their 4-bit transposes for the backward
+    pass, not the tensors.  Differentiable once."""
+    scaling, scale_vec = _form(scaling, scale_vec)
+    _rounding(scaling, scale_rounding)
+    _real_tensor(x, "x")
+    _real_tensor(w, "w")
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x [..., K] and w [N, K] do not fit: {tuple(x.shape)}, {tuple(w.shape)}")
+    if w.shape[0] == 0 or w.shape[1] == 0:
+        raise ValueError("w must not be empty")
+    if x.dtype != w.dtype or x.device != w.device:
+        raise ValueError("x and w must have one type and device")
+    grad = torch.is_grad_enabled()
+    return _Linear.apply(x, w, scaling, scale_vec, scale_rounding, grad and x.requires_grad, grad and w.requires_grad)

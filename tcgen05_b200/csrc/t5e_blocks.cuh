@@ -1,0 +1,202 @@
+// t5e_blocks.cuh -- device pieces shared by the block-scaled E2M1 kernels:
+// real types, the block scale rules, the E2M1 conversions and the scale
+// layout.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "t5e.h"
+
+namespace t5e {
+namespace blocks {
+
+// Real element types (T5E_REAL_*): bits, conversion to F32.
+template <int TYPE>
+struct Real;
+template <>
+struct Real<T5E_REAL_F32> {
+  using type = float;
+  static constexpr int kBytes = 4;
+};
+template <>
+struct Real<T5E_REAL_BF16> {
+  using type = __nv_bfloat16;
+  static constexpr int kBytes = 2;
+};
+template <>
+struct Real<T5E_REAL_F16> {
+  using type = __half;
+  static constexpr int kBytes = 2;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <int TYPE>
+__device__ __forceinline__ typename Real<TYPE>::type from_f32(float v) {
+  if constexpr (TYPE == T5E_REAL_F32) return v;
+  else if constexpr (TYPE == T5E_REAL_BF16) return __float2bfloat16_rn(v);
+  else return __float2half_rn(v);
+}
+
+// Two elements of a packed 32-bit word (low element first).
+template <int TYPE>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (TYPE == T5E_REAL_BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (TYPE == T5E_REAL_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// Byte offset of scale b of row r in the scale tiles: 128 rows by 4 scales
+// are 512 consecutive bytes, ordered so that one 16-byte line holds the four
+// scales of rows r, r + 32, r + 64 and r + 96 (the order in which the tensor
+// cores take them from tensor memory).  `groups` = ceil(scales per row / 4).
+__device__ __forceinline__ uint64_t scale_offset(uint64_t r, uint32_t b, uint32_t groups) {
+  return ((r >> 7) * groups + (b >> 2)) * 512u + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
+}
+
+// Scale of a block from the largest magnitude `a` of its (multiplied)
+// elements; returns the scale byte and the step that elements are divided by,
+// as its reciprocal-or-power in `inv` and its value in `step`.
+//   UE4M3: RNE of min(a / 6, 448).  a / 6 correctly rounded to F32 is a tie
+//          of the 4-bit rounding only where the real quotient is (6 t has at
+//          most 7 significand bits), so the second rounding is exact.
+//   UE8M0: 2^(floor(log2 a) - 2), or with `ceil` the smallest 2^e >= a / 6.
+// A block with a NaN or an infinity gets the NaN scale and a zero step.
+template <bool E8M0>
+__device__ __forceinline__ uint32_t block_scale(float a, bool ceil, float& step, float& inv) {
+  const uint32_t bits = __float_as_uint(a);
+  if constexpr (E8M0) {
+    // word = floor(log2 a) - 2 + 127: the F32 exponent field less 2; F32
+    // subnormals have field 0 and clamp to word 0 (2^-127), as zero does
+    const int field = (int)(bits >> 23);
+    int w = field - 2;
+    if (ceil && (bits & 0x7FFFFFu) > 0x400000u) w += 1;  // a > 1.5 * 2^floor(log2 a) = 6 * 2^(floor(log2 a) - 2)
+    w = w < 0 ? 0 : w;
+    if (bits >= 0x7F800000u) {
+      step = inv = 0.f;
+      return 0xFFu;
+    }
+    // 2^(127 - w) without leaving F32: w = 0 gives 2^127, w = 254 the
+    // subnormal 2^-127, both exact
+    inv = w == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - w) << 23);
+    step = 0.f;  // unused: products with inv are exact wherever they reach the E2M1 range
+    return (uint32_t)w;
+  } else {
+    if (bits >= 0x7F800000u) {
+      step = inv = 0.f;
+      return 0x7Fu;
+    }
+    const float want = __fdiv_rn(a, 6.f);
+    uint16_t two;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(want));
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(two));
+    step = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
+    inv = step > 0.f ? __frcp_rn(step) : 0.f;
+    return two & 0x7Fu;
+  }
+}
+
+// u / step correctly rounded to F32 (Markstein's correction of the product
+// with the correctly rounded reciprocal), for UE4M3 steps.  A quotient so
+// rounded is an E2M1 tie only where the real one is: step has 4 significand
+// bits and a tie 3, so a neighbour of a tie stays one after rounding.
+template <bool E8M0>
+__device__ __forceinline__ float divide(float u, float step, float inv) {
+  const float y = __fmul_rn(u, inv);
+  if constexpr (E8M0) return y;
+  else return __fmaf_rn(-__fmaf_rn(y, step, -u), inv, y);  // this order of signs keeps a negative zero
+}
+
+// Two values to two E2M1 codes (RNE, magnitudes above 6 become 6): `lo` in
+// the low nibble.
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}\n"
+      : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}\n"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Eight E2M1 codes to their values.
+__device__ __forceinline__ void from_e2m1x8(uint32_t w, float* v) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// Value of a scale byte (NaN for the NaN codes; the sign bit of a UE4M3 byte
+// is ignored, as by the tensor cores).
+template <bool E8M0>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  if constexpr (E8M0) {
+    if (byte == 0xFFu) return __uint_as_float(0x7FC00000u);
+    return byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+  } else {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(byte & 0x7Fu)));
+    return __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
+  }
+}
+
+// The tensor multiplier of a largest magnitude: the largest power of two m
+// with a * m <= 6 * 448, held to 2^+-126; 1 where a is 0 or not finite.
+// 2688 = 1.3125 * 2^11.
+__device__ __forceinline__ float multiplier_of(uint32_t abs_bits) {
+  if (abs_bits == 0u || abs_bits >= 0x7F800000u) return 1.f;
+  int e;
+  const float f = frexpf(__uint_as_float(abs_bits), &e);  // a = 2f * 2^(e - 1)
+  int p = 11 - (e - 1) - (2.f * f > 1.3125f ? 1 : 0);
+  p = p > 126 ? 126 : (p < -126 ? -126 : p);
+  return __uint_as_float((uint32_t)(p + 127) << 23);
+}
+
+__device__ __forceinline__ void wait_for_previous_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+}  // namespace blocks
+}  // namespace t5e

@@ -39,16 +39,24 @@ int grid_for(uint64_t n, int block);
 // would return), made without any CUDA call.
 int validate(const t5e_model* M, const t5e_batch* B);
 
+// Multiprocessors of the current device.
+int sm_count();
+
+// Block-scaled rows (t5e_blocks): groups of four scales per row, and the
+// checks every entry point makes.
+uint32_t scale_groups(const t5e_blocks& b);
+bool blocks_ok(const t5e_blocks* b);
+
 // Launches `kernel` on `stream` as a programmatic dependent of the previous
 // kernel there (programmatic stream serialisation): its blocks may start
 // while that kernel's last blocks run, so the kernel must execute
 // griddepcontrol.wait before it reads or writes global memory that earlier
 // work on the stream may touch.
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
-                             cudaStream_t stream, Args... args) {
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+                             Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

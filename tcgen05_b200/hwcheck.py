@@ -16,6 +16,10 @@ where the B200 writes F16 words; that pairing is counted separately.
 ``cross_check_sparse`` for the sparse ones (tcgen05.mma.sp): the cases of a
 sparse validation path, one uniform tile per case.
 
+``cross_check_product`` compares whole products: ``block_scaled_mm`` of matrices
+of any K against the emulator's words carried from one K=64 instruction to the
+next.
+
     python -m tcgen05_b200.hwcheck [--tiles 64] [--seed 0]
 """
 
@@ -541,6 +545,54 @@ def cross_check_sparse(spec, n: int = 1024, *, layout: int | None = None, device
             "nonuniform_tiles": int((hw["disagree"] != 0).sum()), "hardware": hw["d"], "emulator": emu}
 
 
+def emulated_product(a, b):
+    """The F32 words [M, N] of A @ B.T of two BlockScaledRows as a chain of
+    emulated K=64 instructions, each accumulating onto the words of the one
+    before (int32 tensor on their device)."""
+    import torch
+
+    from .simulator import mma_batch
+
+    per = 64 // a.block
+    args = dict(scaling="ue4m3", scale_vec=4) if a.scaling == "ue4m3" else \
+        dict(scaling="ue8m0", kind="mxf4", scale_vec=2) if a.scale_vec == 2 else \
+        dict(scaling="ue8m0", kind="mxf4nvf4", scale_vec=4)
+
+    def steps(q):
+        n = -(-q.k // 64)
+        words = torch.stack((q.data & 15, q.data >> 4), dim=2).reshape(q.rows, -1)[:, :q.k].int()
+        scales = q.scale_words()
+        words = torch.nn.functional.pad(words, (0, 64 * n - q.k)).reshape(q.rows, n, 64)
+        return words, torch.nn.functional.pad(scales, (0, per * n - scales.shape[1])).reshape(q.rows, n, per)
+
+    (aw, sa), (bw, sb) = steps(a), steps(b)
+    c = torch.zeros(1, a.rows, b.rows, dtype=torch.int32, device=a.device)
+    for i in range(aw.shape[1]):
+        c = mma_batch(aw[None, :, i], bw[:, i].t()[None], c, a_format="e2m1", scale_a=sa[None, :, i].contiguous(),
+                      scale_b=sb[None, :, i].contiguous(), **args).view(torch.int32)
+    return c[0]
+
+
+def cross_check_product(a, b, split: int = 1) -> dict:
+    """Words of ``block_scaled_mm`` in F32 (K in one part unless `split` says
+    otherwise) and of the emulated chain, multipliers left out."""
+    import torch
+
+    from .blocks import BlockScaledRows, _mm
+
+    a, b = (BlockScaledRows(q.data, q.scales, q.k, scaling=q.scaling, scale_vec=q.scale_vec) for q in (a, b))
+    hw = _mm(a, b, None, 1.0, torch.float32, None, split)
+    emu = emulated_product(a, b)
+    diff = (hw.view(torch.int32) != emu) & ~(torch.isnan(hw) & torch.isnan(emu.view(torch.float32)))
+    return {"product": [a.rows, b.rows, a.k], "scaling": a.scaling, "scale_vec": a.scale_vec, "cases": hw.numel(),
+            "mismatches": int(diff.sum()), "hardware": hw, "emulator": emu.view(torch.float32)}
+
+
+# (M, N, K, scaling, scale_vec) of the products the command cross-checks
+PRODUCTS = [(128, 128, 1024, "ue4m3", 4), (300, 200, 700, "ue4m3", 4), (5, 260, 2048, "ue8m0", 2),
+            (300, 520, 333, "ue8m0", 4)]
+
+
 def sparse_paths():
     """The sparse validation paths, in workload order."""
     from . import workloads
@@ -572,10 +624,22 @@ def main(argv=None) -> int:
         r = cross_check_sparse(spec, args.sparse_cases)
         sp_failed += r["mismatches"] != 0 or r["nonuniform_tiles"] != 0
         print(json.dumps({k: v for k, v in r.items() if k not in ("hardware", "emulator")}), flush=True)
-    print(json.dumps({"pairs": len(PAIRS), "pairs_with_mismatches": failed, "block_scaled_pairs": len(BS_PAIRS),
+    import torch
+
+    from .blocks import quantize_blocks
+
+    mm_failed = 0
+    for i, (m, n, k, scaling, vec) in enumerate(PRODUCTS):
+        g = torch.Generator(device="cuda").manual_seed(args.seed + 2000 + i)
+        a, b = (quantize_blocks(torch.randn(r, k, generator=g, device="cuda"), scaling=scaling, scale_vec=vec)
+                for r in (m, n))
+        r = cross_check_product(a, b)
+        mm_failed += r["mismatches"] != 0
+        print(json.dumps({k: v for k, v in r.items() if k not in ("hardware", "emulator")}), flush=True)
+    print(json.dumps({"products": len(PRODUCTS), "products_with_mismatches": mm_failed, "pairs": len(PAIRS), "pairs_with_mismatches": failed, "block_scaled_pairs": len(BS_PAIRS),
                       "block_scaled_pairs_with_mismatches": bs_failed, "sparse_paths": len(sparse_paths()),
                       "sparse_paths_with_mismatches": sp_failed}), flush=True)
-    return 1 if failed or bs_failed or sp_failed else 0
+    return 1 if failed or bs_failed or sp_failed or mm_failed else 0
 
 
 if __name__ == "__main__":
