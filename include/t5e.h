@@ -359,16 +359,13 @@ typedef struct t5e_blocks {
     int32_t scale_block;
 } t5e_blocks;
 
-/* Partial maxima of |x| (F32 bits) over a [rows, cols] tensor with row stride
- * `stride` (elements): `count` words, 1..T5E_MAX_PARTIALS, all written. */
-#define T5E_MAX_PARTIALS 1024
-int t5e_block_partials(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
-                       int32_t count, void* stream);
-
 /* multiplier[0] = the largest power of two m, 2^-126..2^126, with
- * m * max|x| <= 6 * 448, from those partial maxima; 1 where max|x| is zero or
- * not finite. */
-int t5e_block_multiplier(const uint32_t* partials, int32_t count, float* multiplier, void* stream);
+ * m * max|x| <= 6 * 448 over a [rows, cols] tensor with row stride `stride`
+ * (elements); 1 where max|x| is zero or not finite.  partials: workspace of
+ * `count` words, 1..T5E_MAX_PARTIALS, one per block of the first launch. */
+#define T5E_MAX_PARTIALS 1024
+int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
+                         int32_t count, float* multiplier, void* stream);
 
 /* Rounds x [rows, cols] (row stride in elements) to blocks along its rows
  * (by_rows: rows = rows, k = cols), along its columns (by_cols: rows = cols,
@@ -378,11 +375,11 @@ int t5e_block_multiplier(const uint32_t* partials, int32_t count, float* multipl
  *   (CEIL) the smallest power of two >= a / 6, held to 2^+-127;
  *   code = RNE(u / scale) of the real quotient, magnitudes above 6 become 6.
  * A block with a NaN or an infinity gets the NaN scale and codes 0; a zero
- * scale gets codes that are zeros.  With partials != NULL the multiplier is
- * taken from those partial maxima (t5e_block_partials of the same x) and
- * stored to *multiplier. */
+ * scale gets codes that are zeros.  With partials != NULL (a workspace of
+ * `count` words) the multiplier is first computed as by t5e_block_multiplier
+ * and stored to *multiplier. */
 int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, int32_t rounding,
-                        float* multiplier, const uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
+                        float* multiplier, uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
                         const t5e_blocks* by_cols, void* stream);
 
 /* out[r][i] = code * scale * F32(1 / m) rounded to `type`; out_stride in
@@ -398,7 +395,10 @@ int t5e_dequantize_blocks(const t5e_blocks* blocks, const float* multiplier, int
  * ascending steps of 64 (in parts that are joined in F32 where the call
  * splits K).  c (NULL: none) is of type c_type with strides in elements (0
  * broadcasts); d is of type d_type with row stride d_stride and unit column
- * stride; c may be d.  split: 0 lets the library choose, 1, 2, 4 or 8 parts.
+ * stride; c may be d.  form: 0 lets the library choose the kernel; 1, 2, 4
+ * or 8: tiles of 128 rows by up to 128, K in that many parts (at most
+ * ceil(k/256)); 128 or 256: tiles of 256 rows of a by that many of b (not
+ * where a has fewer rows than b and at most 128).
  * If a bounded wait inside the kernel runs out, the tile becomes NaN and
  * t5e_block_scaled_mm_expired reports it.
  */
@@ -408,7 +408,7 @@ typedef struct t5e_block_mm {
     const float* multiplier_a;   /* device scalars or NULL (1) */
     const float* multiplier_b;
     float alpha;
-    int32_t split;
+    int32_t form;
     const void* c;
     int32_t c_type;
     int32_t d_type;

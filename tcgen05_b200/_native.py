@@ -136,7 +136,7 @@ class BlockMm(ctypes.Structure):
         ("multiplier_a", ctypes.c_void_p),
         ("multiplier_b", ctypes.c_void_p),
         ("alpha", ctypes.c_float),
-        ("split", ctypes.c_int32),
+        ("form", ctypes.c_int32),
         ("c", ctypes.c_void_p),
         ("c_type", ctypes.c_int32),
         ("d_type", ctypes.c_int32),
@@ -162,7 +162,6 @@ EXPORTED = (
     "t5e_tcgen05_tiles",
     "t5e_tcgen05_block_scaled_tiles",
     "t5e_tcgen05_sparse_cases",
-    "t5e_block_partials",
     "t5e_block_multiplier",
     "t5e_quantize_blocks",
     "t5e_dequantize_blocks",
@@ -224,11 +223,10 @@ def load() -> ctypes.CDLL:
     lib.t5e_tcgen05_sparse_cases.restype = ctypes.c_int
     lib.t5e_tcgen05_sparse_cases.argtypes = [ctypes.c_int32, ctypes.c_uint32, ctypes.c_int32] + [ctypes.c_void_p] * 8 \
         + [ctypes.c_uint64, ctypes.c_void_p, ctypes.c_void_p]
-    lib.t5e_block_partials.restype = ctypes.c_int
-    lib.t5e_block_partials.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
-                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
     lib.t5e_block_multiplier.restype = ctypes.c_int
-    lib.t5e_block_multiplier.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+    lib.t5e_block_multiplier.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
+                                         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+                                         ctypes.c_void_p]
     lib.t5e_quantize_blocks.restype = ctypes.c_int
     lib.t5e_quantize_blocks.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
                                         ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,

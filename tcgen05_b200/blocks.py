@@ -85,39 +85,53 @@ class BlockScaledRows:
     multiplied by before rounding, or None: element i of row r stands for
     code * scale / multiplier."""
 
-    __slots__ = ("data", "scales", "k", "scaling", "scale_vec", "multiplier")
+    __slots__ = ("rows", "k", "scaling", "scale_vec", "device", "multiplier", "_data", "_scales", "_buffer", "_struct")
 
     def __init__(self, data, scales, k: int, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
         scaling, scale_vec = _form(scaling, scale_vec)
+        fmt, block = _FORMS[scaling, scale_vec]
         k = int(k)
         if not 1 <= k <= nat.MAX_BLOCK_K:
             raise ValueError(f"K={k} outside 1..{nat.MAX_BLOCK_K}")
         if data.dim() != 2 or data.dtype != torch.uint8 or (data.shape[0] and not data.is_contiguous()):
             raise ValueError("data must be a contiguous [rows, stride] uint8 tensor")
-        if data.shape[0] > nat.MAX_BLOCK_ROWS:
+        rows, stride = data.shape
+        if rows > nat.MAX_BLOCK_ROWS:
             raise ValueError(f"more than {nat.MAX_BLOCK_ROWS} rows")
-        if data.shape[1] % 16 or data.shape[1] < self.row_stride(k):
-            raise ValueError(f"row stride {data.shape[1]} is not a multiple of 16 of at least {self.row_stride(k)}")
-        tiles = (data.shape[0] + 127) // 128
-        groups = -(-k // (4 * _FORMS[scaling, scale_vec][1]))
-        if scales.dtype != torch.uint8 or tuple(scales.shape) != (tiles, groups, 512) or not scales.is_contiguous():
+        if stride % 16 or stride < self.row_stride(k):
+            raise ValueError(f"row stride {stride} is not a multiple of 16 of at least {self.row_stride(k)}")
+        tiles, groups = (rows + 127) // 128, -(-k // (4 * block))
+        if scales.dtype != torch.uint8 or scales.shape != (tiles, groups, 512) or not scales.is_contiguous():
             raise ValueError(f"scales must be a contiguous [{tiles}, {groups}, 512] uint8 tensor (tile_scales)")
         if scales.device != data.device:
             raise ValueError("data and scales are on different devices")
         if multiplier is not None:
             if multiplier.dtype != torch.float32 or multiplier.numel() != 1 or multiplier.device != data.device:
                 raise ValueError("multiplier must be a one-element float32 tensor on the data's device")
-        if data.data_ptr() % 16 or scales.data_ptr() % 16:
+        at, scales_at = data.data_ptr(), scales.data_ptr()
+        if at % 16 or scales_at % 16:
             raise ValueError("data and scales must start on 16-byte boundaries")
-        self.data, self.scales, self.k = data, scales, k
-        self.scaling, self.scale_vec, self.multiplier = scaling, scale_vec, multiplier
+        self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
+        self.device, self.multiplier = data.device, multiplier
+        self._data, self._scales, self._buffer = data, scales, None
+        self._struct = nat.Blocks(at, stride, scales_at, rows, k, fmt, block)
 
     @classmethod
-    def _made(cls, data, scales, k, scaling, scale_vec, multiplier):
-        """An instance whose parts are known to fit."""
+    def _within(cls, buffer, rows, k, scaling, scale_vec, multiplier):
+        """An instance over one uint8 buffer (a new one if None): the rows, then
+        the scale tiles.  The views are made when they are asked for."""
         self = cls.__new__(cls)
-        self.data, self.scales, self.k = data, scales, k
-        self.scaling, self.scale_vec, self.multiplier = scaling, scale_vec, multiplier
+        fmt, block = _FORMS[scaling, scale_vec]
+        stride = (k + 31) // 32 * 16
+        if not isinstance(buffer, torch.Tensor):
+            buffer = torch.empty(rows * stride + (rows + 127) // 128 * (-(-k // (4 * block)) * 512), dtype=torch.uint8,
+                                 device=buffer)
+        self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
+        self.device, self.multiplier = buffer.device, multiplier
+        self._data = self._scales = None
+        self._buffer = buffer
+        at = buffer.data_ptr()
+        self._struct = nat.Blocks(at, stride, at + rows * stride, rows, k, fmt, block)
         return self
 
     @classmethod
@@ -140,17 +154,23 @@ class BlockScaledRows:
         return (k + 31) // 32 * 16
 
     @property
-    def rows(self) -> int:
-        return self.data.shape[0]
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            stride = self._struct.stride
+            self._data = self._buffer[:self.rows * stride].view(self.rows, stride)
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buffer[self.rows * self._struct.stride:].view(
+                (self.rows + 127) // 128, -(-self.k // (4 * self.block)), 512)
+        return self._scales
 
     @property
     def block(self) -> int:
         """Elements per scale."""
-        return _FORMS[self.scaling, self.scale_vec][1]
-
-    @property
-    def device(self):
-        return self.data.device
+        return self._struct.scale_block
 
     def packed(self) -> PackedRows:
         """The codes as the emulator's operand rows."""
@@ -160,29 +180,25 @@ class BlockScaledRows:
         """[rows, blocks] scale bytes, as the emulator takes them."""
         return untile_scales(self.scales, self.rows, -(-self.k // self.block))
 
-    def _struct(self) -> nat.Blocks:
-        fmt, block = _FORMS[self.scaling, self.scale_vec]
-        return nat.Blocks(self.data.data_ptr(), self.data.shape[1], self.scales.data_ptr(), self.data.shape[0], self.k,
-                          fmt, block)
-
     def __repr__(self):
         return (f"BlockScaledRows({self.rows} x {self.k}, {self.scaling}, scale_vec={self.scale_vec}, "
                 f"device={self.device})")
 
 
 class _On:
-    """Makes `device` current for a library call, and gives its current stream."""
+    """Makes the device of index `index` current for a library call, and gives
+    its current stream."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, device):
-        self.index = device.index
+    def __init__(self, index):
+        self.index = index
 
     def __enter__(self):
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return torch.cuda.current_stream().cuda_stream
 
     def __exit__(self, *exc):
         if self.before != self.index:
@@ -211,12 +227,10 @@ def _matrix_of(x):
     return m.contiguous(), False
 
 
-def _partials(m, handle, lib):
-    count = max(1, min(592, -(-m.numel() // 8192)))
-    partials = torch.empty(count, dtype=torch.int32, device=m.device)
-    nat.check(lib.t5e_block_partials(_REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0),
-                                     partials.data_ptr(), count, handle), "t5e_block_partials")
-    return partials, count
+def _partial_count(n: int) -> int:
+    """Blocks that look for the largest of n elements: 8192 elements each, up
+    to four per multiprocessor."""
+    return min(592, -(-n // 8192)) or 1
 
 
 def block_multiplier(x) -> torch.Tensor:
@@ -228,22 +242,17 @@ def block_multiplier(x) -> torch.Tensor:
     _real_tensor(x, "x")
     if x.dim() == 0:
         x = x.reshape(1)
-    out = torch.empty(1, dtype=torch.float32, device=x.device)
     lib = nat.load()
     if x.numel() == 0:
-        return out.fill_(1.0)
-    with _On(x.device) as handle:
+        return torch.ones(1, dtype=torch.float32, device=x.device)
+    with _On(x.device.index) as handle:
         m, _ = _matrix_of(x.detach())
-        partials, count = _partials(m, handle, lib)
-        nat.check(lib.t5e_block_multiplier(partials.data_ptr(), count, out.data_ptr(), handle), "t5e_block_multiplier")
-    return out
-
-
-def _empty_blocks(rows, k, scaling, scale_vec, multiplier, device):
-    data = torch.empty((rows, BlockScaledRows.row_stride(k)), dtype=torch.uint8, device=device)
-    groups = -(-k // (4 * _FORMS[scaling, scale_vec][1]))
-    scales = torch.empty(((rows + 127) // 128, groups, 512), dtype=torch.uint8, device=device)
-    return BlockScaledRows._made(data, scales, k, scaling, scale_vec, multiplier)
+        count = _partial_count(m.numel())
+        work = torch.empty(1 + count, dtype=torch.float32, device=m.device)
+        at = work.data_ptr()
+        nat.check(lib.t5e_block_multiplier(_REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0), at + 4,
+                                           count, at, handle), "t5e_block_multiplier")
+    return work[:1]
 
 
 def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None = None,
@@ -288,26 +297,36 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
         raise ValueError("blocks along an empty axis")
     if (by_rows and k > nat.MAX_BLOCK_K) or (by_cols and r > nat.MAX_BLOCK_K) or max(r, k) > nat.MAX_BLOCK_ROWS:
         raise ValueError(f"x is larger than {nat.MAX_BLOCK_K} elements along a block axis or {nat.MAX_BLOCK_ROWS} rows")
+    return _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier)
+
+
+def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier):
+    """quantize_blocks of checked arguments, x as r rows of k: the rows, the
+    columns or the pair."""
     lib = nat.load()
-    with _On(x.device) as handle:
+    device = x.device
+    with _On(device.index) as handle:
         m, turned = _matrix_of(x.detach())
-        partials, count = None, 0
-        if isinstance(multiplier, str):
-            if m.numel():
-                partials, count = _partials(m, handle, lib)
-            multiplier = torch.empty(1, dtype=torch.float32, device=x.device) if m.numel() else None
-        elif isinstance(multiplier, (int, float)):
-            multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=x.device)
-        rows = _empty_blocks(r, k, scaling, scale_vec, multiplier, x.device) if by_rows else None
-        cols = _empty_blocks(k, r, scaling, scale_vec, multiplier, x.device) if by_cols else None
+        partials, count, at = None, 0, None
+        if multiplier is not None:
+            if isinstance(multiplier, str):
+                multiplier = None
+                if r:
+                    count = _partial_count(r * k)
+                    work = torch.empty(1 + count, dtype=torch.float32, device=device)
+                    partials, multiplier = work.data_ptr() + 4, work[:1]
+            elif not isinstance(multiplier, torch.Tensor):
+                multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
+            at = None if multiplier is None else multiplier.data_ptr()
+        rows = BlockScaledRows._within(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
+        cols = BlockScaledRows._within(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
         along, across = (cols, rows) if turned else (rows, cols)
+        shape = m.shape
         nat.check(lib.t5e_quantize_blocks(
-            _REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0), rounding,
-            None if multiplier is None else multiplier.data_ptr(),
-            None if partials is None else partials.data_ptr(), count,
-            None if along is None else ctypes.byref(along._struct()),
-            None if across is None else ctypes.byref(across._struct()), handle), "t5e_quantize_blocks")
-    if axis == "both":
+            _REAL[m.dtype], m.data_ptr(), shape[0], shape[1], m.stride(0), rounding, at, partials, count,
+            None if along is None else ctypes.byref(along._struct),
+            None if across is None else ctypes.byref(across._struct), handle), "t5e_quantize_blocks")
+    if by_rows and by_cols:
         return rows, cols
     return rows if by_rows else cols
 
@@ -315,14 +334,14 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
 def _check_blocks(q, name: str):
     if not isinstance(q, BlockScaledRows):
         raise ValueError(f"{name} must be BlockScaledRows")
-    if not q.data.is_cuda:
+    if q.device.type != "cuda":
         raise ValueError(f"{name} must be on a CUDA device (there is no CPU fallback)")
 
 
 def _result(out, shape, dtype, device):
     """The result tensor: `out` checked, or a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
         raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor on {device}")
     if out.numel() and ((out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1])):
@@ -341,9 +360,9 @@ def dequantize_blocks(blocks: BlockScaledRows, *, dtype=torch.float32, out=None)
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     out = _result(out, (blocks.rows, blocks.k), dtype, blocks.device)
     lib = nat.load()
-    with _On(blocks.device) as handle:
+    with _On(blocks.device.index) as handle:
         m = blocks.multiplier
-        nat.check(lib.t5e_dequantize_blocks(ctypes.byref(blocks._struct()), None if m is None else m.data_ptr(),
+        nat.check(lib.t5e_dequantize_blocks(ctypes.byref(blocks._struct), None if m is None else m.data_ptr(),
                                             _REAL[dtype], out.data_ptr(), out.stride(0) if blocks.rows > 1 else blocks.k,
                                             handle), "t5e_dequantize_blocks")
     return out
@@ -374,7 +393,7 @@ def block_scaled_mm(a: BlockScaledRows, b: BlockScaledRows, c=None, *, alpha: fl
     return _mm(a, b, c, alpha, dtype, out, 0)
 
 
-def _mm(a, b, c, alpha, dtype, out, split):
+def _mm(a, b, c, alpha, dtype, out, form):
     if (a.scaling, a.scale_vec) != (b.scaling, b.scale_vec):
         raise ValueError(f"a and b have different forms: {a!r}, {b!r}")
     if a.k != b.k:
@@ -403,65 +422,63 @@ def _mm(a, b, c, alpha, dtype, out, split):
         if c0 < d1 and d0 < c1 and not same:
             raise ValueError("c overlaps out without being out")
     lib = nat.load()
-    sa, sb = a._struct(), b._struct()
-    mm = nat.BlockMm()
-    mm.a, mm.b = ctypes.pointer(sa), ctypes.pointer(sb)
-    mm.multiplier_a = None if a.multiplier is None else a.multiplier.data_ptr()
-    mm.multiplier_b = None if b.multiplier is None else b.multiplier.data_ptr()
-    mm.alpha, mm.split = alpha, split
+    mm = nat.BlockMm(
+        ctypes.pointer(a._struct), ctypes.pointer(b._struct), None if a.multiplier is None else a.multiplier.data_ptr(),
+        None if b.multiplier is None else b.multiplier.data_ptr(), alpha, form, None, 0, _REAL[dtype], 0, 0,
+        out.data_ptr(), out.stride(0) if given and shape[0] > 1 else shape[1])
     if c is not None:
         mm.c, mm.c_type = c.data_ptr(), _REAL[c.dtype]
         mm.c_row_stride, mm.c_col_stride = c.stride()
-    mm.d, mm.d_type = out.data_ptr(), _REAL[dtype]
-    mm.d_stride = out.stride(0) if shape[0] > 1 else shape[1]
-    with _On(a.device) as handle:
+    with _On(a.device.index) as handle:
         nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
     return out
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, scaling, scale_vec, scale_rounding, need_x, need_w):
-        form = dict(scaling=scaling, scale_vec=scale_vec, scale_rounding=scale_rounding,
-                    multiplier="auto" if scaling == "ue4m3" else None)
-        flat = x.reshape(-1, x.shape[-1])
-        tokens = flat.shape[0]
+    def forward(ctx, x, w, scaling, scale_vec, rounding, need_x, need_w):
+        (n, k), tokens = w.shape, x.numel() // w.shape[1]
+        form = (scaling, scale_vec, rounding, "auto" if scaling == "ue4m3" else None)
         # blocks run along the contraction: K here, the tokens and N in the
         # gradients, so what a gradient needs is rounded along the other axis
-        qx, xt = quantize_blocks(flat, axis="both", **form) if need_w and tokens else (quantize_blocks(flat, **form), None)
-        qw, wt = quantize_blocks(w, axis="both", **form) if need_x and tokens else (quantize_blocks(w, **form), None)
+        need_x, need_w = need_x and tokens > 0, need_w and tokens > 0
+        qx = _quantize(x, tokens, k, True, need_w, *form)
+        qw = _quantize(w, n, k, True, need_x, *form)
+        ctx.form, ctx.need = form, (need_x, need_w)
+        kept = []
+        if need_w:
+            qx, xt = qx
+            kept += [xt._buffer, xt.multiplier]
+        if need_x:
+            qw, wt = qw
+            kept += [wt._buffer, wt.multiplier]
+        ctx.save_for_backward(*kept)
+        ctx.shapes = x.shape, w.shape
         y = _mm(qx, qw, None, 1.0, x.dtype, None, 0)
-        ctx.form, ctx.shapes, ctx.need = form, (x.shape, w.shape), (need_x, need_w)
-        saved = []
-        for q in (xt, wt):
-            saved += [None, None, None] if q is None else [q.data, q.scales, q.multiplier]
-        ctx.save_for_backward(*saved)
-        return y.view(*x.shape[:-1], w.shape[0])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        (x_shape, w_shape), (need_x, need_w) = ctx.shapes, ctx.need
-        n, k = w_shape
-        flat = g.reshape(-1, n)
-        tokens = flat.shape[0]
-        dx = dw = None
-        if tokens == 0:
-            return (g.new_zeros(x_shape) if need_x else None, g.new_zeros(w_shape) if need_w else None,
-                    None, None, None, None, None)
-        form = ctx.form
-        kept = ctx.saved_tensors
-
-        def held(i, length):
-            return BlockScaledRows._made(kept[i], kept[i + 1], length, form["scaling"], form["scale_vec"], kept[i + 2])
-
-        axis = "both" if need_x and need_w else (-1 if need_x else 0)
-        q = quantize_blocks(flat, axis=axis, **form)
-        rows, cols = q if axis == "both" else ((q, None) if need_x else (None, q))
-        if need_x:
-            dx = _mm(rows, held(3, n), None, 1.0, g.dtype, None, 0).view(x_shape)
-        if need_w:
-            dw = _mm(cols, held(0, tokens), None, 1.0, g.dtype, None, 0)
+        (need_x, need_w), form = ctx.need, ctx.form
+        x_shape, (n, k) = ctx.shapes
+        tokens = g.numel() // n
+        asked_x, asked_w = ctx.needs_input_grad[:2]
+        dx = g.new_zeros(x_shape) if asked_x and not tokens else None
+        dw = g.new_zeros(n, k) if asked_w and not tokens else None
+        need_x, need_w = need_x and asked_x, need_w and asked_w
+        if need_x or need_w:
+            kept = ctx.saved_tensors
+            q = _quantize(g, tokens, n, need_x, need_w, *form)
+            rows, cols = q if need_x and need_w else (q, q)
+            if need_x:
+                wt = BlockScaledRows._within(kept[-2], k, n, *form[:2], kept[-1])
+                dx = _mm(rows, wt, None, 1.0, g.dtype, None, 0)
+                if len(x_shape) != 2:
+                    dx = dx.view(x_shape)
+            if need_w:
+                xt = BlockScaledRows._within(kept[0], k, tokens, *form[:2], kept[1])
+                dw = _mm(cols, xt, None, 1.0, g.dtype, None, 0)
         return dx, dw, None, None, None, None, None
 
 
@@ -480,7 +497,7 @@ def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None =
     once each; a training step keeps their 4-bit transposes for the backward
     pass, not the tensors.  Differentiable once."""
     scaling, scale_vec = _form(scaling, scale_vec)
-    _rounding(scaling, scale_rounding)
+    rounding = _rounding(scaling, scale_rounding)
     _real_tensor(x, "x")
     _real_tensor(w, "w")
     if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
@@ -490,4 +507,4 @@ def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None =
     if x.dtype != w.dtype or x.device != w.device:
         raise ValueError("x and w must have one type and device")
     grad = torch.is_grad_enabled()
-    return _Linear.apply(x, w, scaling, scale_vec, scale_rounding, grad and x.requires_grad, grad and w.requires_grad)
+    return _Linear.apply(x, w, scaling, scale_vec, rounding, grad and x.requires_grad, grad and w.requires_grad)

@@ -19,24 +19,20 @@ using blocks::to_f32;
 constexpr int kStageK = 256;      // elements of K per pipeline stage: 128 bytes, one swizzle atom wide
 constexpr int kInstrK = 64;       // elements of K per tcgen05.mma
 constexpr int kRowBytes = 128;    // bytes of a row in a stage
-// Bounded waits: a wait polls at most this often (each poll itself suspends
-// for up to some microseconds), then the tile is given up.
-constexpr uint32_t kWaitPolls = 1u << 22;
+// Bounded waits: after this long (2 s) the tile is given up.
+constexpr uint64_t kWaitNs = 2000000000ull;
 
 __device__ int g_expired;  // 1 once a wait ran out on this device
 
 struct Params {
-  CUtensorMap p_map, q_map;      // the operand with 128 rows a tile, the other one
-  const uint8_t* p_scales;
-  const uint8_t* q_scales;
   const float* multiplier_a;
   const float* multiplier_b;
   const void* c;
   void* d;
   int64_t c_p_stride, c_q_stride;  // elements
   int64_t d_stride;                // elements, along the axis that is not contiguous
-  uint32_t p_rows, q_rows;
-  uint32_t k, stages, groups;      // elements, pipeline stages, groups of four scales per row
+  uint32_t p_rows, q_rows;         // P: the operand with 128 rows a tile, Q: the other one
+  uint32_t k, stages;              // elements, pipeline stages
   uint32_t idesc;
   float alpha;
   int32_t c_type, d_type;
@@ -62,28 +58,83 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   return done != 0u;
 }
 
-// Waits for the phase; gives up after kWaitPolls polls or once another thread
-// of the block gave up (*failed).
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Waits for the phase; gives up after kWaitNs, or once another thread of the
+// block gave up (*failed; NULL: do not look).
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-  for (uint32_t poll = 0; poll < kWaitPolls; ++poll) {
+  if (barrier_try(bar, parity)) return true;
+  const uint64_t start = now_ns();
+  do {
     if (barrier_try(bar, parity)) return true;
-    if (*failed) return false;
-  }
-  *failed = 1;
+    if (failed != nullptr && *failed) return false;
+  } while (now_ns() - start < kWaitNs);
+  if (failed != nullptr) *failed = 1;
   return false;
 }
 
-// ---- copies -----------------------------------------------------------------
+// One thread of a converged warp.  elect.sync (rather than lane == 0) and a
+// broadcast warp index let the compiler see that what follows is uniform,
+// which the operands of tcgen05 and TMA instructions have to be.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, P;\n\t}\n" : "=r"(p));
+  return p != 0u;
+}
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0); }
 
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-               "[%4];"
-               :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
 
-__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+// The address of a variable of this block in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void arrive_in(uint32_t bar_in_cluster) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar_in_cluster) : "memory");
+}
+
+// ---- copies -----------------------------------------------------------------
+//
+// In a pair the barrier may be the other block's (cta_group::2).
+
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                 "[%1, {%2, %3}], [%4];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+                 "[%4];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                        uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                 "[%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                 "[%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
 // ---- tensor memory and products -----------------------------------------------
@@ -101,27 +152,48 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
 }
 
-// 512 bytes of scales to four columns, the same in each 32-lane quarter.
+// 512 bytes of scales to four columns, the same in each 32-lane quarter (in a
+// pair each block's bytes to its own tensor memory).
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(scale_desc(smem)) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(scale_desc(smem)) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(scale_desc(smem)) : "memory");
 }
 
-template <int BLOCK>
+#define T5E_BLOCK_MMA(group, form)                                                                       \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                         \
+               "tcgen05.mma.cta_group::" group ".kind::" form " [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n" \
+               :: "r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(accumulate), "r"(tsp), "r"(tsq))
+
+template <bool PAIR, int BLOCK>
 __device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t dp, uint64_t dq, uint32_t idesc, uint32_t tsp, uint32_t tsq,
                                     uint32_t accumulate) {
-  if constexpr (BLOCK == 32) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n"
-                 :: "r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(accumulate), "r"(tsp), "r"(tsq));
-  } else {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.block16 [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n"
-                 :: "r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(accumulate), "r"(tsp), "r"(tsq));
-  }
+  if constexpr (PAIR && BLOCK == 32) T5E_BLOCK_MMA("2", "mxf4.block_scale.block32");
+  else if constexpr (PAIR) T5E_BLOCK_MMA("2", "mxf4nvf4.block_scale.block16");
+  else if constexpr (BLOCK == 32) T5E_BLOCK_MMA("1", "mxf4.block_scale.block32");
+  else T5E_BLOCK_MMA("1", "mxf4nvf4.block_scale.block16");
 }
 
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+#undef T5E_BLOCK_MMA
+
+// Arrives on this block's barrier when what this thread issued so far is
+// complete; commit_all arrives on it in both blocks of a pair.
+template <bool PAIR>
+__device__ __forceinline__ void commit_here(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit_all(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    commit_here<false>(bar);
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -140,6 +212,18 @@ __device__ __forceinline__ void load_acc16(uint32_t addr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void load_acc32(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+               "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void acc_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
 // ---- results ---------------------------------------------------------------------
 
 __device__ __forceinline__ float read_real(const void* p, int64_t i, int32_t type) {
@@ -154,10 +238,43 @@ __device__ __forceinline__ void write_real(void* p, int64_t i, int32_t type, flo
   else static_cast<__half*>(p)[i] = from_f32<T5E_REAL_F16>(v);
 }
 
+// N neighbouring finished results of row p, columns q .. q + N - 1: vectors where
+// the row is aligned.
+template <int N>
+__device__ __forceinline__ void store_plain(const Params& P, uint32_t p, uint32_t q, float (&v)[N], int count = N) {
+  if (p >= P.p_rows) return;
+  if (q + count > P.q_rows) count = q >= P.q_rows ? 0 : (int)(P.q_rows - q);
+  const int64_t at = (int64_t)p * P.d_stride + q;
+  if (P.d_type == T5E_REAL_F32) {
+    float* dst = static_cast<float*>(P.d) + at;
+    if (N % 4 == 0 && count == N && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i)
+        reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      return;
+    }
+  } else {
+    uint16_t* dst = static_cast<uint16_t*>(P.d) + at;
+    if (N % 8 == 0 && count == N && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+      uint32_t w[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        w[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(v[2 * i], v[2 * i + 1])
+                                         : pack2<T5E_REAL_F16>(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i)
+        reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < count) write_real(P.d, at + i, P.d_type, v[i]);
+}
+
 // N neighbouring results of row p of the tile grid, columns q .. q + count - 1:
 // scales them, adds C and stores them.  SWAP: D is contiguous along p (lanes
-// store neighbouring elements), otherwise along q (a lane stores vectors where
-// the row is aligned).
+// store neighbouring elements), otherwise along q (a lane stores vectors).
 template <bool SWAP, int N>
 __device__ __forceinline__ void store_results(const Params& P, float alpha, uint32_t p, uint32_t q, int count,
                                               float (&v)[N]) {
@@ -175,81 +292,316 @@ __device__ __forceinline__ void store_results(const Params& P, float alpha, uint
     for (int i = 0; i < N; ++i)
       if (i < count) write_real(P.d, (int64_t)(q + i) * P.d_stride + p, P.d_type, v[i]);
   } else {
-    const int64_t at = (int64_t)p * P.d_stride + q;
-    if (P.d_type == T5E_REAL_F32) {
-      float* dst = static_cast<float*>(P.d) + at;
-      if (N % 4 == 0 && count == N && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i)
-          reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        return;
-      }
-    } else {
-      uint16_t* dst = static_cast<uint16_t*>(P.d) + at;
-      if (N % 8 == 0 && count == N && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
-        uint32_t w[N / 2];
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-          w[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(v[2 * i], v[2 * i + 1])
-                                           : pack2<T5E_REAL_F16>(v[2 * i], v[2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < N / 8; ++i)
-          reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        return;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < count) write_real(P.d, at + i, P.d_type, v[i]);
+    store_plain<N>(P, p, q, v, count);
   }
+}
+
+// A warp's 32 x 32 results by way of shared memory (a 32 x 33 buffer of its
+// own): lane r brings row p + r, columns q .. q + 31; the stores, and the loads
+// of C, then run along the rows, 32 neighbouring elements at a time, whatever
+// the alignment.
+__device__ __forceinline__ void store_turned(const Params& P, float alpha, uint32_t p, uint32_t q, const float* v,
+                                             float* buffer) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) buffer[lane * 33 + j] = v[j];
+  __syncwarp();
+  const uint32_t col = q + lane;
+  if (col >= P.q_rows || p >= P.p_rows) return;
+  const int rows = P.p_rows - p < 32u ? (int)(P.p_rows - p) : 32;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    float x = buffer[r * 33 + lane];
+    x = P.c != nullptr ? __fmaf_rn(x, alpha, read_real(P.c, (int64_t)(p + r) * P.c_p_stride + (int64_t)col * P.c_q_stride,
+                                                       P.c_type))
+                       : x * alpha;
+    write_real(P.d, (int64_t)(p + r) * P.d_stride + col, P.d_type, x);
+  }
+}
+
+// The same results, without C, through a box of 32 rows that TMA writes: rows
+// of 64 bytes (16-bit results) or 128, swizzled as the map says, so that the
+// lanes' 16-byte stores meet no bank twice.  `box` is the box to fill; the
+// caller alternates between two.
+__device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* map, float alpha, uint32_t p, uint32_t q,
+                                          const float* v, uint8_t* box) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the box before the last has been read
+  __syncwarp();
+  if (P.d_type == T5E_REAL_F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+          make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = v[8 * j + 2 * i] * alpha, hi = v[8 * j + 2 * i + 1] * alpha;
+        w[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(lo, hi) : pack2<T5E_REAL_F16>(lo, hi);
+      }
+      *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    if (q < P.q_rows && p < P.p_rows)
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                   :: "l"(map), "r"((int32_t)q), "r"((int32_t)p), "r"(smem_u32(box)) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+
+// ---- the pipeline both kernels share ----------------------------------------------
+//
+// Four roles, one thread each, and two rings of shared-memory stages of 256 K:
+//
+//   operands   TMA loads the codes of P and Q into the operand ring
+//   scales     TMA loads the scale tiles into the scale ring
+//   spread     tcgen05.cp copies a unit's scales (128 K) from the scale ring
+//              to one of four unit buffers in tensor memory
+//   products   waits for a stage's codes and a unit's scales and issues the
+//              unit's two tcgen05.mma
+//
+// The scales have a ring and a thread of their own because a tcgen05.cp of 512
+// bytes takes about 32 cycles, and in one thread with the products it runs
+// between them: a 256 x 256 pair stage (512 cycles of products) spent 384 more on
+// its 12 copies.  From another thread they run beside the products, and run
+// ahead of the codes, so that a stage of codes is held no longer than its
+// load and its products take; what bounds the rate is the number of bytes in
+// flight (8192^3 in blocks of 16: 384 us with the copies between the
+// products, 328 with their own thread, measured before the separate ring).
+//
+// In a pair (PAIR) both blocks load their own parts, and the first block
+// spreads and issues for both; its barriers count the bytes of both, and its
+// commits arrive in both.
+template <bool PAIR_, int BN_, int BLOCK_, int STAGES_, int SCALE_STAGES_, int TMEM_>
+struct Pipe {
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int BN = BN_, BLOCK = BLOCK_, STAGES = STAGES_, SCALE_STAGES = SCALE_STAGES_;
+  static constexpr int kTmem = TMEM_;                            // columns allocated
+  static constexpr int kGroups = kStageK / (4 * BLOCK);          // 512-byte scale tiles of a stage per 128 rows
+  static constexpr int kUnitGroups = kGroups / 2;
+  static constexpr int kQTiles = (BN + 127) / 128;               // scale tiles of Q's rows
+  static constexpr int kQRows = PAIR ? BN / 2 : BN;              // rows of Q a block loads
+  static constexpr int kPBytes = 128 * kRowBytes, kQBytes = kQRows * kRowBytes;
+  static constexpr int kStageBytes = kPBytes + kQBytes;
+  static constexpr int kScaleBytes = kGroups * 512 * (1 + kQTiles);
+  static constexpr int kUnitCols = kUnitGroups * 4 * (1 + kQTiles);
+  static constexpr int kUnits = 4;
+  static constexpr int kScaleCol = kTmem - kUnits * kUnitCols;   // first column of the unit buffers
+  static constexpr int kBytes = STAGES * kStageBytes + SCALE_STAGES * kScaleBytes;
+  static constexpr int kBlocks = PAIR ? 2 : 1;
+};
+
+template <typename S>
+struct Barriers {
+  uint64_t full[S::STAGES], empty[S::STAGES];
+  uint64_t scale_full[S::SCALE_STAGES], scale_empty[S::SCALE_STAGES];
+  uint64_t unit_full[S::kUnits], unit_empty[S::kUnits];
+};
+
+struct Maps {
+  CUtensorMap p, q, ps, qs;
+};
+
+template <typename S>
+__device__ __forceinline__ void init_barriers(Barriers<S>& b) {
+  for (int i = 0; i < S::STAGES; ++i) {
+    barrier_init(smem_u32(&b.full[i]), 1);
+    barrier_init(smem_u32(&b.empty[i]), 1);
+  }
+  for (int i = 0; i < S::SCALE_STAGES; ++i) {
+    barrier_init(smem_u32(&b.scale_full[i]), 1);
+    barrier_init(smem_u32(&b.scale_empty[i]), 1);
+  }
+  for (int i = 0; i < S::kUnits; ++i) {
+    barrier_init(smem_u32(&b.unit_full[i]), 1);
+    barrier_init(smem_u32(&b.unit_empty[i]), 1);
+  }
+}
+
+__device__ __forceinline__ void prefetch_maps(const Maps& m) {
+  asm volatile("prefetch.tensormap [%0];" :: "l"(&m.p));
+  asm volatile("prefetch.tensormap [%0];" :: "l"(&m.q));
+  asm volatile("prefetch.tensormap [%0];" :: "l"(&m.ps));
+  asm volatile("prefetch.tensormap [%0];" :: "l"(&m.qs));
+}
+
+// Waits until the slot of use `n` of a ring of `size` stages has been released
+// by its use before (at once the first time round).
+__device__ __forceinline__ bool wait_slot(uint64_t* empty, uint32_t n, uint32_t size, int* failed) {
+  return barrier_wait(smem_u32(empty + n % size), ((n / size) & 1u) ^ 1u, failed);
+}
+__device__ __forceinline__ bool wait_use(uint64_t* full, uint32_t n, uint32_t size, int* failed) {
+  return barrier_wait(smem_u32(full + n % size), (n / size) & 1u, failed);
+}
+
+// Announces `bytes` per block and returns the barrier that the copies arrive
+// on: the first block's in a pair.
+template <typename S>
+__device__ __forceinline__ uint32_t announce(uint64_t* full, uint32_t rank, uint32_t bytes) {
+  const uint32_t bar = smem_u32(full);
+  if (!S::PAIR || rank == 0) barrier_expect(bar, S::kBlocks * bytes);
+  return S::PAIR ? in_block(bar, 0) : bar;
+}
+
+// Stages first .. last - 1 of a tile; `n` counts the uses of the ring.
+template <typename S>
+__device__ __forceinline__ bool load_operands(const Maps& m, Barriers<S>& b, uint8_t* ring, uint32_t rank, uint32_t first,
+                                              uint32_t last, int32_t p0, int32_t q0, uint32_t& n, int* failed) {
+  for (uint32_t st = first; st < last; ++st, ++n) {
+    if (!wait_slot(b.empty, n, S::STAGES, failed)) return false;
+    const uint32_t slot = n % S::STAGES, at = smem_u32(ring) + slot * S::kStageBytes;
+    const uint32_t bar = announce<S>(&b.full[slot], rank, S::kStageBytes);
+    load_2d<S::PAIR>(at, &m.p, (int32_t)(st * kRowBytes), p0, bar);
+    load_2d<S::PAIR>(at + S::kPBytes, &m.q, (int32_t)(st * kRowBytes), q0, bar);
+  }
+  return true;
+}
+
+template <typename S>
+__device__ __forceinline__ bool load_scales(const Maps& m, Barriers<S>& b, uint8_t* ring, uint32_t rank, uint32_t first,
+                                            uint32_t last, int32_t p_tile, int32_t q_tile, uint32_t& n, int* failed) {
+  for (uint32_t st = first; st < last; ++st, ++n) {
+    if (!wait_slot(b.scale_empty, n, S::SCALE_STAGES, failed)) return false;
+    const uint32_t slot = n % S::SCALE_STAGES, at = smem_u32(ring) + slot * S::kScaleBytes;
+    const uint32_t bar = announce<S>(&b.scale_full[slot], rank, S::kScaleBytes);
+    load_3d<S::PAIR>(at, &m.ps, 0, (int32_t)(st * S::kGroups), p_tile, bar);
+    load_3d<S::PAIR>(at + S::kGroups * 512, &m.qs, 0, (int32_t)(st * S::kGroups), q_tile, bar);
+  }
+  return true;
+}
+
+// Products of K = 64 in a stage.
+__device__ __forceinline__ uint32_t steps_in(uint32_t k, uint32_t st) {
+  const uint32_t left = (k - st * kStageK + kInstrK - 1) / kInstrK;
+  return left < (uint32_t)(kStageK / kInstrK) ? left : kStageK / kInstrK;
+}
+
+template <typename S>
+__device__ __forceinline__ bool spread_scales(Barriers<S>& b, uint8_t* ring, uint32_t tmem, uint32_t k, uint32_t first,
+                                              uint32_t last, uint32_t& n, uint32_t& unit, int* failed) {
+  for (uint32_t st = first; st < last; ++st, ++n) {
+    if (!wait_use(b.scale_full, n, S::SCALE_STAGES, failed)) return false;
+    const uint32_t slot = n % S::SCALE_STAGES, at = smem_u32(ring) + slot * S::kScaleBytes;
+    const uint32_t steps = steps_in(k, st);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u * 2 >= (int)steps) break;
+      if (!wait_slot(b.unit_empty, unit, S::kUnits, failed)) return false;
+      fence_after();
+      const uint32_t to = tmem + S::kScaleCol + unit % S::kUnits * S::kUnitCols;
+#pragma unroll
+      for (int g = 0; g < S::kUnitGroups; ++g) {
+        const int from = u * S::kUnitGroups + g;
+        copy_scales<S::PAIR>(to + g * 4, at + from * 512);
+        // Q's scales of one group side by side: 4 columns per 128 rows
+#pragma unroll
+        for (int h = 0; h < S::kQTiles; ++h)
+          copy_scales<S::PAIR>(to + (S::kUnitGroups + g * S::kQTiles + h) * 4, at + (S::kGroups * (1 + h) + from) * 512);
+      }
+      commit_here<S::PAIR>(smem_u32(&b.unit_full[unit % S::kUnits]));
+      ++unit;
+    }
+    commit_all<S::PAIR>(smem_u32(&b.scale_empty[slot]));
+  }
+  return true;
+}
+
+template <typename S>
+__device__ __forceinline__ bool issue_products(Barriers<S>& b, uint8_t* ring, uint32_t acc, uint32_t tmem, uint32_t k,
+                                               uint32_t idesc, uint32_t first, uint32_t last, uint32_t& n, uint32_t& unit,
+                                               int* failed) {
+  for (uint32_t st = first; st < last; ++st, ++n) {
+    if (!wait_use(b.full, n, S::STAGES, failed)) return false;
+    const uint32_t slot = n % S::STAGES, at = smem_u32(ring) + slot * S::kStageBytes;
+    const uint64_t dp = operand_desc(at), dq = operand_desc(at + S::kPBytes);
+    const uint32_t steps = steps_in(k, st);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u * 2 >= (int)steps) break;
+      if (!wait_use(b.unit_full, unit, S::kUnits, failed)) return false;
+      fence_after();
+      const uint32_t tsp = tmem + S::kScaleCol + unit % S::kUnits * S::kUnitCols, tsq = tsp + S::kUnitGroups * 4;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (u * 2 + j < (int)steps) {
+          // a column of scales holds four bytes per row: one product's with
+          // blocks of 16, two products' (bytes 0-1, 2-3) with blocks of 32
+          const int g = S::BLOCK == 16 ? j : 0;
+          const uint32_t id = S::BLOCK == 16 ? 0u : (uint32_t)j * 2u;
+          mma<S::PAIR, S::BLOCK>(acc, dp + (u * 2 + j) * 2, dq + (u * 2 + j) * 2, idesc | (id << 4) | (id << 29),
+                                 tsp + g * 4, tsq + g * S::kQTiles * 4, st != first || u + j != 0);
+        }
+      }
+      commit_here<S::PAIR>(smem_u32(&b.unit_empty[unit % S::kUnits]));
+      ++unit;
+    }
+    commit_all<S::PAIR>(smem_u32(&b.empty[slot]));
+  }
+  return true;
+}
+
+// Waits until the last uses of a ring (`n` so far) have been released: no copy
+// into it is in flight then.
+__device__ __forceinline__ bool drain_ring(uint64_t* empty, uint32_t n, uint32_t size) {
+  bool ok = true;
+  for (uint32_t i = n > size ? n - size : 0u; i < n; ++i) ok &= wait_use(empty, i, size, nullptr);
+  return ok;
 }
 
 // ---- one tile per block ------------------------------------------------------------
 //
 // A block of 128 threads computes a tile of 128 rows of one operand (P) by BN
-// rows of the other (Q).  One thread keeps `kStages` stages of 256 K in flight
-// with TMA, one issues the products; then all four warps take the
-// accumulators from tensor memory.  A cluster of `split` blocks shares one
-// tile, each with its part of K; the partial sums meet in shared memory and
-// each block finishes BN / split columns, adding the parts in rank order.
+// rows of the other (Q): its warps are the four roles first, and all take the
+// accumulators from tensor memory afterwards.  A cluster of `split` blocks
+// shares one tile, each with its part of K; the partial sums meet in shared
+// memory and each block finishes BN / split columns, adding the parts in rank
+// order.
 template <int BN, int BLOCK>
 struct TileShape {
-  static constexpr int kGroups = kStageK / (4 * BLOCK);  // 512-byte scale tiles per stage
-  static constexpr int kScaleBytes = kGroups * 512;
-  static constexpr int kPBytes = 128 * kRowBytes, kQBytes = BN * kRowBytes;
-  static constexpr int kStageBytes = kPBytes + kQBytes + 2 * kScaleBytes;
-  static constexpr int kStages = 110 * 1024 / kStageBytes;  // two blocks on an SM
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
-  static constexpr int kScaleCol = BN < 32 ? 32 : BN;  // tensor memory column of the scales
-  static constexpr int kTmemCols = BN > 64 ? 256 : 128;
-  static_assert(kStages * kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
-  static_assert(kScaleCol + 2 * 2 * kGroups * 4 <= kTmemCols, "accumulators and two stages of scales");
+  static constexpr int kScaleStages = 3;
+  static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * 2;
+  static constexpr int kStages = (110 * 1024 - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN * kRowBytes);
+  using Pipe = blockmm::Pipe<false, BN, BLOCK, kStages, kScaleStages, BN <= 64 ? 128 : 256>;
+  static constexpr int kSmem = Pipe::kBytes + 1024;  // two blocks fit an SM
+  static_assert(kStages * Pipe::kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
+  static_assert(Pipe::kScaleCol >= BN, "accumulators and scales share tensor memory");
+};
+
+struct TileParams {
+  Maps maps;
+  Params r;
 };
 
 template <int BN, int BLOCK, bool SWAP>
-__global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ Params P, uint32_t split) {
-  using S = TileShape<BN, BLOCK>;
+__global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileParams T, uint32_t split) {
+  using S = typename TileShape<BN, BLOCK>::Pipe;
+  const Params& P = T.r;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], finished;
+  __shared__ Barriers<S> bars;
+  __shared__ uint64_t finished;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int t = threadIdx.x, warp = warp_index();
   uint8_t* stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* scale_stages = stages + S::STAGES * S::kStageBytes;
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmemCols));
+                 :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (t == 0) {
-    for (int i = 0; i < S::kStages; ++i) {
-      barrier_init(smem_u32(&full[i]), 1);
-      barrier_init(smem_u32(&empty[i]), 1);
-    }
+    init_barriers(bars);
     barrier_init(smem_u32(&finished), 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" :: "l"(&P.p_map));
-    asm volatile("prefetch.tensormap [%0];" :: "l"(&P.q_map));
+    prefetch_maps(T.maps);
   }
   fence_before();
   __syncthreads();
@@ -262,76 +614,47 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ Param
   const uint32_t p0 = tile % p_tiles * 128u, q0 = tile / p_tiles * (uint32_t)BN;
   const uint32_t first = (uint32_t)((uint64_t)P.stages * rank / split);
   const uint32_t last = (uint32_t)((uint64_t)P.stages * (rank + 1) / split);
-  if (warp == 0 && lane == 0) {
-    const uint8_t* ps = P.p_scales + (uint64_t)(p0 >> 7) * P.groups * 512u;
-    const uint8_t* qs = P.q_scales + (uint64_t)(q0 >> 7) * P.groups * 512u;
-    uint32_t issued = 0;
-    bool ok = true;
-    for (uint32_t st = first; st < last; ++st, ++issued) {
-      const uint32_t slot = issued % S::kStages, round = issued / S::kStages;
-      ok = barrier_wait(smem_u32(&empty[slot]), (round & 1u) ^ 1u, &failed);
-      if (!ok) break;
-      const uint32_t base = smem_u32(stages) + slot * S::kStageBytes, bar = smem_u32(&full[slot]);
-      const uint32_t g0 = st * S::kGroups;
-      const uint32_t gn = P.groups - g0 < (uint32_t)S::kGroups ? P.groups - g0 : (uint32_t)S::kGroups;
-      barrier_expect(bar, S::kPBytes + S::kQBytes + 2u * gn * 512u);
-      load_tile(base, &P.p_map, (int32_t)(st * kRowBytes), (int32_t)p0, bar);
-      load_tile(base + S::kPBytes, &P.q_map, (int32_t)(st * kRowBytes), (int32_t)q0, bar);
-      load_bytes(base + S::kPBytes + S::kQBytes, ps + (uint64_t)g0 * 512u, gn * 512u, bar);
-      load_bytes(base + S::kPBytes + S::kQBytes + S::kScaleBytes, qs + (uint64_t)g0 * 512u, gn * 512u, bar);
+  bool ok = true;
+  if (elected()) {
+    uint32_t n = 0, unit = 0;
+    if (warp == 0) {
+      ok = load_operands<S>(T.maps, bars, stages, 0, first, last, (int32_t)p0, (int32_t)q0, n, &failed);
+      ok &= drain_ring(bars.empty, n, S::STAGES);
+    } else if (warp == 1) {
+      ok = issue_products<S>(bars, stages, tmem, tmem, P.k, P.idesc, first, last, n, unit, &failed);
+      commit_here<false>(smem_u32(&finished));  // after a wait that ran out too: what was issued completes
+    } else if (warp == 2) {
+      ok = load_scales<S>(T.maps, bars, scale_stages, 0, first, last, (int32_t)(p0 >> 7), (int32_t)(q0 >> 7), n, &failed);
+      ok &= drain_ring(bars.scale_empty, n, S::SCALE_STAGES);
+    } else {
+      ok = spread_scales<S>(bars, scale_stages, tmem, P.k, first, last, n, unit, &failed);
     }
-    if (!ok) {  // given up: no copy may still be in flight when the block ends
-      for (uint32_t i = issued > (uint32_t)S::kStages ? issued - S::kStages : 0u; i < issued; ++i)
-        for (uint32_t poll = 0; poll < kWaitPolls && !barrier_try(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1u);
-             ++poll) {
-        }
-    }
-  } else if (warp == 1 && lane == 0) {
-    bool ok = true;
-    uint32_t used = 0;
-    for (uint32_t st = first; st < last; ++st, ++used) {
-      const uint32_t slot = used % S::kStages;
-      ok = barrier_wait(smem_u32(&full[slot]), (used / S::kStages) & 1u, &failed);
-      if (!ok) break;
-      fence_after();
-      const uint32_t base = smem_u32(stages) + slot * S::kStageBytes;
-      const uint32_t left = P.k - st * kStageK;
-      const uint32_t steps = left >= (uint32_t)kStageK ? kStageK / kInstrK : (left + kInstrK - 1) / kInstrK;
-      const uint32_t tsp = tmem + S::kScaleCol + (used & 1u) * (2 * S::kGroups * 4), tsq = tsp + S::kGroups * 4;
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
-        if (g * (BLOCK / 16) < (int)steps) {
-          copy_scales(tsp + g * 4, base + S::kPBytes + S::kQBytes + g * 512);
-          copy_scales(tsq + g * 4, base + S::kPBytes + S::kQBytes + S::kScaleBytes + g * 512);
-        }
-      }
-      const uint64_t dp = operand_desc(base), dq = operand_desc(base + S::kPBytes);
-#pragma unroll
-      for (int j = 0; j < kStageK / kInstrK; ++j) {
-        if (j < (int)steps) {
-          // a column of scales holds four bytes per row: one product's with
-          // blocks of 16, two products' with blocks of 32 (bytes 0-1, 2-3)
-          const int col = BLOCK == 16 ? j * 4 : j / 2 * 4;
-          const uint32_t id = BLOCK == 16 ? 0u : (uint32_t)(j & 1) * 2u;
-          mma<BLOCK>(tmem, dp + j * 2, dq + j * 2, P.idesc | (id << 4) | (id << 29), tsp + col, tsq + col,
-                     used != 0u || j != 0);
-        }
-      }
-      commit(smem_u32(&empty[slot]));
-    }
-    commit(smem_u32(&finished));  // after a wait that ran out too: the products issued before it complete
   }
   __syncwarp();
-  bool arrived = false;
-  for (uint32_t poll = 0; poll < kWaitPolls && !arrived; ++poll) arrived = barrier_try(smem_u32(&finished), 0);
+  ok &= barrier_wait(smem_u32(&finished), 0, nullptr);
   fence_after();
-  const bool bad = __syncthreads_or(!arrived || *static_cast<volatile int*>(&failed));
+  const bool bad = __syncthreads_or(!ok);
   if (bad && t == 0) atomicExch(&g_expired, 1);
   const float nan = __uint_as_float(0x7FC00000u);
   const float alpha = P.alpha * (P.multiplier_a != nullptr ? 1.f / *P.multiplier_a : 1.f) *
                       (P.multiplier_b != nullptr ? 1.f / *P.multiplier_b : 1.f);
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-  if (split == 1u) {
+  if (split == 1u && !SWAP && BN >= 32) {
+    // the stages are free: 32 x 33 floats of them for each warp
+    float* buffer = reinterpret_cast<float*>(stages) + warp * (32 * 33);
+#pragma unroll 1
+    for (int q = 0; q < BN; q += 32) {
+      if (q0 + q >= P.q_rows) break;
+      float v[32];
+      load_acc32(lanes + q, v);
+      acc_loaded();
+      if (bad) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = nan;
+      }
+      store_turned(P, alpha, p0 + warp * 32u, q0 + q, v, buffer);
+    }
+  } else if (split == 1u) {
 #pragma unroll 1
     for (int q = 0; q < BN; q += 16) {
       if (q0 + q >= P.q_rows) break;
@@ -352,7 +675,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ Param
 #pragma unroll
       for (int i = 0; i < 16; ++i) part[(q + i) * 128 + t] = bad ? nan : v[i];
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();
     const int width = BN / (int)split, w0 = width * (int)rank;
 #pragma unroll 1
     for (int q = w0; q < w0 + width; q += 8) {
@@ -362,8 +685,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ Param
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
       for (uint32_t r = 0; r < split; ++r) {
-        uint32_t there;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(part + q * 128 + t)), "r"(r));
+        const uint32_t there = in_block(smem_u32(part + q * 128 + t), r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (i < count) {
@@ -375,13 +697,170 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ Param
       }
       store_results<SWAP, 8>(P, alpha, p0 + t, q0 + q, count, v);
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();
   }
   fence_before();
   __syncthreads();
   if (warp == 2) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmem));
+  }
+}
+
+// ---- large products: pairs of blocks -------------------------------------------------
+//
+// A cluster of two blocks on one SM pair computes tiles of 256 rows (of A) by BN
+// rows (of B) with cta_group::2 instructions that the first block issues: each
+// block holds its 128 rows of A and half of B's rows, so B crosses shared
+// memory once for both, and accumulates its 128 x BN part in its own tensor
+// memory.  The blocks are persistent (tile = cluster, cluster + clusters, ...)
+// and specialised: four warps are the pipeline's roles, four take results out,
+// so that the results of a tile leave while the next one is computed.
+//
+// Tensor memory (512 columns): two accumulators of BN columns and the unit
+// buffers of the scales.  For BN = 256 the accumulators share columns: the
+// results' warps take those out first and then let the next tile start.
+template <int BN, int BLOCK>
+struct PairShape {
+  static constexpr int kScaleStages = 4;
+  static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * (1 + BN / 128);
+  static constexpr int kBoxBytes = 8192;  // a results warp's shared memory: two boxes, or the 32 x 33 buffer
+  static constexpr int kStages =
+      (226 * 1024 - 1024 - 4 * kBoxBytes - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN / 2 * kRowBytes);
+  using Pipe = blockmm::Pipe<true, BN, BLOCK, kStages, kScaleStages, 512>;
+  static constexpr int kSmem = Pipe::kBytes + 4 * kBoxBytes + 1024;
+  static constexpr int kSecond = BN <= 128 ? BN : (Pipe::kScaleCol - BN) / 32 * 32;  // column of the second accumulator
+  static constexpr int kShared = BN - kSecond;  // columns both use (0: none)
+  static_assert(kSecond + BN <= Pipe::kScaleCol && kShared % 32 == 0 && kShared >= 0, "tensor memory");
+};
+
+struct PairParams {
+  Maps maps;
+  CUtensorMap d_map;
+  Params r;
+  uint32_t p_tiles, q_tiles;
+  int32_t boxed;  // results leave through d_map: rows on 16-byte boundaries, no C
+};
+
+constexpr int kPairThreads = 256;  // warps 0-3 the roles, 4-7 the results
+
+template <int BN, int BLOCK>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams P) {
+  using L = PairShape<BN, BLOCK>;
+  using S = typename L::Pipe;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Barriers<S> bars;
+  __shared__ uint64_t acc_full[2], acc_free[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const int t = threadIdx.x, warp = warp_index(), lane = t & 31;
+  const uint32_t rank = cluster_rank();
+  uint8_t* boxes = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* stages = boxes + 4 * L::kBoxBytes;
+  uint8_t* scale_stages = stages + S::STAGES * S::kStageBytes;
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  if (t == 0) {
+    init_barriers(bars);
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(smem_u32(&acc_full[i]), 1);
+      barrier_init(smem_u32(&acc_free[i]), 8);  // four warps of each block
+    }
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_maps(P.maps);
+  }
+  fence_before();
+  cluster_sync();
+  fence_after();
+  blocks::let_next_grid_start();
+  blocks::wait_for_previous_grid();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t clusters = gridDim.x / 2, tiles = P.p_tiles * P.q_tiles, stage_count = P.r.stages;
+  bool ok = true;
+  if (warp < 4) {
+    if ((rank == 0 || warp == 0 || warp == 2) && elected()) {
+      uint32_t n = 0, unit = 0, count = 0;
+      for (uint32_t tile = blockIdx.x / 2; ok && tile < tiles; tile += clusters, ++count) {
+        const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
+        const int32_t p0 = (int32_t)(pt * 256u + rank * 128u), q0 = (int32_t)(qt * BN + rank * (BN / 2));
+        if (warp == 0) {
+          ok = load_operands<S>(P.maps, bars, stages, rank, 0, stage_count, p0, q0, n, &failed);
+        } else if (warp == 2) {
+          ok = load_scales<S>(P.maps, bars, scale_stages, rank, 0, stage_count, p0 >> 7, (int32_t)(qt * S::kQTiles), n,
+                              &failed);
+        } else if (warp == 3) {
+          ok = spread_scales<S>(bars, scale_stages, tmem, P.r.k, 0, stage_count, n, unit, &failed);
+        } else {
+          // the columns shared with the tile before are free (and all of the
+          // one before that, whose results were taken out first), or without
+          // shared columns those of the tile before the last
+          const uint32_t back = L::kShared ? 1u : 2u;
+          if (count >= back) {
+            const uint32_t before = count - back;
+            ok = barrier_wait(smem_u32(&acc_free[before & 1u]), (before >> 1) & 1u, &failed);
+            if (!ok) break;
+            fence_after();
+          }
+          ok = issue_products<S>(bars, stages, tmem + (count & 1u) * L::kSecond, tmem, P.r.k, P.r.idesc, 0, stage_count, n,
+                                 unit, &failed);
+          if (ok) commit_all<true>(smem_u32(&acc_full[count & 1u]));  // if not, the results' waits run out too
+        }
+      }
+      if (warp == 0) ok &= drain_ring(bars.empty, n, S::STAGES);
+      if (warp == 2) ok &= drain_ring(bars.scale_empty, n, S::SCALE_STAGES);
+    }
+  } else {
+    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    const float alpha = P.r.alpha * (P.r.multiplier_a != nullptr ? 1.f / *P.r.multiplier_a : 1.f) *
+                        (P.r.multiplier_b != nullptr ? 1.f / *P.r.multiplier_b : 1.f);
+    uint8_t* box = boxes + quarter * L::kBoxBytes;
+    uint32_t count = 0;
+    for (uint32_t tile = blockIdx.x / 2; ok && tile < tiles; tile += clusters, ++count) {
+      const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
+      const uint32_t p = pt * 256u + rank * 128u + quarter * 32u, q0 = qt * BN;
+      ok = barrier_wait(smem_u32(&acc_full[count & 1u]), (count >> 1) & 1u, &failed);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (count & 1u) * L::kSecond;
+      const uint32_t free_bar = in_block(smem_u32(&acc_free[count & 1u]), 0);
+      // chunks of 32 columns, the shared ones first: they are the last of the
+      // first accumulator and the first of the second
+      constexpr int kChunks = BN / 32, kFirst = L::kShared / 32;
+#pragma unroll 1
+      for (int i = 0; i < kChunks; ++i) {
+        int chunk = i;
+        if (L::kShared && (count & 1u) == 0u) chunk = i < kFirst ? kChunks - kFirst + i : i - kFirst;
+        float v[32];
+        load_acc32(acc + chunk * 32, v);
+        acc_loaded();
+        if (i == (L::kShared ? kFirst - 1 : kChunks - 1)) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_in(free_bar);
+        }
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
+        }
+        const uint32_t q = q0 + chunk * 32;
+        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box + (i & 1) * 4096);
+        else store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
+      }
+    }
+    if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  fence_before();
+  const bool bad = __syncthreads_or(!ok);
+  if (t == 0 && bad) atomicExch(&g_expired, 1);
+  cluster_sync();
+  if (warp == 4) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmem));
   }
 }
 
@@ -426,20 +905,80 @@ int encode(CUtensorMap* map, const t5e_blocks& b, uint32_t box_rows) {
   return T5E_OK;
 }
 
+// Map of scale tiles as 32-bit words: 128 words, the groups, the tiles of rows;
+// boxes of one pipeline stage's groups by `tiles` tiles.
+int encode_scales(CUtensorMap* map, const t5e_blocks& b, uint32_t box_groups, uint32_t box_tiles) {
+  const EncodeTiled f = encoder();
+  if (!f) return T5E_ERR_CUDA;
+  const cuuint64_t groups = scale_groups(b), tiles = (b.rows + 127) / 128;
+  const cuuint64_t dims[3] = {128, groups, tiles}, strides[2] = {512, groups * 512};
+  const cuuint32_t box[3] = {128, box_groups, box_tiles}, unit[3] = {1, 1, 1};
+  const CUresult r = f(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, b.scales, dims, strides, box, unit,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_cuda_error("cuTensorMapEncodeTiled", cudaErrorInvalidValue);
+    return T5E_ERR_CUDA;
+  }
+  return T5E_OK;
+}
+
+// Map of the results, boxes of 32 columns by 32 rows; *boxed = 0 where the rows
+// do not lie on 16-byte boundaries.
+int encode_results(CUtensorMap* map, const Params& P, int32_t* boxed) {
+  const int bytes = P.d_type == T5E_REAL_F32 ? 4 : 2;
+  *boxed = 0;
+  if ((reinterpret_cast<uintptr_t>(P.d) & 15u) || (P.d_stride * bytes) % 16 || P.d_stride * bytes >= (1ll << 40)) return T5E_OK;
+  const EncodeTiled f = encoder();
+  if (!f) return T5E_ERR_CUDA;
+  const cuuint64_t dims[2] = {P.q_rows, P.p_rows}, strides[1] = {(cuuint64_t)(P.d_stride * bytes)};
+  const cuuint32_t box[2] = {32, 32}, unit[2] = {1, 1};
+  const CUtensorMapDataType type = P.d_type == T5E_REAL_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : P.d_type == T5E_REAL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = f(map, type, 2, P.d, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                       CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_cuda_error("cuTensorMapEncodeTiled", cudaErrorInvalidValue);
+    return T5E_ERR_CUDA;
+  }
+  *boxed = 1;
+  return T5E_OK;
+}
+
+template <typename S>
+int encode_maps(Maps* m, const t5e_blocks& p, const t5e_blocks& q) {
+  int rc = encode(&m->p, p, 128);
+  if (rc == T5E_OK) rc = encode(&m->q, q, S::kQRows);
+  if (rc == T5E_OK) rc = encode_scales(&m->ps, p, S::kGroups, 1);
+  if (rc == T5E_OK) rc = encode_scales(&m->qs, q, S::kGroups, S::kQTiles);
+  return rc;
+}
+
 // Instruction descriptor: E2M1 x E2M1, M = 128, `n` columns.
 uint32_t instruction(const t5e_blocks& b, uint32_t n, uint32_t m = 128) {
   return (1u << 7) | (1u << 10) | ((n / 8u) << 17) | ((b.scale_format == T5E_SCALE_UE8M0 ? 1u : 0u) << 23) |
          ((m / 128u) << 27);
 }
 
+int blocks_launched(cudaError_t e) {
+  if (e != cudaSuccess) {
+    set_cuda_error("block product launch", e);
+    return T5E_ERR_CUDA;
+  }
+  return kernel_status("block product launch");
+}
+
 template <int BN, int BLOCK, bool SWAP>
-int launch_tile(Params& P, const t5e_blocks& p, const t5e_blocks& q, uint32_t split, cudaStream_t stream) {
+int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, uint32_t split, cudaStream_t stream) {
   using S = TileShape<BN, BLOCK>;
-  int rc = encode(&P.p_map, p, 128);
-  if (rc == T5E_OK) rc = encode(&P.q_map, q, BN);
+  TileParams P;
+  P.r = params;
+  int rc = encode_maps<typename S::Pipe>(&P.maps, p, q);
   if (rc == T5E_OK) rc = raise_smem_limit<tile_kernel<BN, BLOCK, SWAP>>(S::kSmem, "block product attribute");
   if (rc != T5E_OK) return rc;
-  P.idesc = instruction(p, BN);
+  P.r.idesc = instruction(p, BN);
   cudaLaunchConfig_t cfg = {};
   const uint64_t grid = ((p.rows + 127) / 128) * ((q.rows + BN - 1) / BN) * split;
   if (grid > 0x7FFFFFFFull) return T5E_ERR_INVALID;
@@ -454,16 +993,11 @@ int launch_tile(Params& P, const t5e_blocks& p, const t5e_blocks& q, uint32_t sp
   attr[1].val.clusterDim = {split, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tile_kernel<BN, BLOCK, SWAP>, P, split);
-  if (e != cudaSuccess) {
-    set_cuda_error("block product launch", e);
-    return T5E_ERR_CUDA;
-  }
-  return kernel_status("block product launch");
+  return blocks_launched(cudaLaunchKernelEx(&cfg, tile_kernel<BN, BLOCK, SWAP>, P, split));
 }
 
 template <int BLOCK>
-int launch_form(Params& P, const t5e_blocks& p, const t5e_blocks& q, bool swap, uint32_t split, cudaStream_t stream) {
+int launch_form(const Params& P, const t5e_blocks& p, const t5e_blocks& q, bool swap, uint32_t split, cudaStream_t stream) {
   if (q.rows <= 16)
     return swap ? launch_tile<16, BLOCK, true>(P, p, q, split, stream) : launch_tile<16, BLOCK, false>(P, p, q, split, stream);
   if (q.rows <= 32)
@@ -473,7 +1007,41 @@ int launch_form(Params& P, const t5e_blocks& p, const t5e_blocks& q, bool swap, 
   return swap ? launch_tile<128, BLOCK, true>(P, p, q, split, stream) : launch_tile<128, BLOCK, false>(P, p, q, split, stream);
 }
 
-uint64_t tiles_of(uint64_t p_rows, uint64_t q_rows) { return ((p_rows + 127) / 128) * ((q_rows + 127) / 128); }
+template <int BN, int BLOCK>
+int launch_pair(const Params& params, const t5e_blocks& a, const t5e_blocks& b, cudaStream_t stream) {
+  using S = PairShape<BN, BLOCK>;
+  PairParams P;
+  P.r = params;
+  int rc = encode_maps<typename S::Pipe>(&P.maps, a, b);
+  if (rc == T5E_OK) rc = raise_smem_limit<pair_kernel<BN, BLOCK>>(S::kSmem, "block product attribute");
+  if (rc != T5E_OK) return rc;
+  P.boxed = 0;
+  if (params.c == nullptr) {
+    rc = encode_results(&P.d_map, params, &P.boxed);
+    if (rc != T5E_OK) return rc;
+  }
+  if (!P.boxed) P.d_map = P.maps.p;  // not read
+  P.r.idesc = instruction(a, BN, 256);
+  P.p_tiles = (uint32_t)((a.rows + 255) / 256);
+  P.q_tiles = (uint32_t)((b.rows + BN - 1) / BN);
+  const uint64_t tiles = (uint64_t)P.p_tiles * P.q_tiles, room = (uint64_t)sm_count() / 2;
+  if (tiles > 0x7FFFFFFFull) return T5E_ERR_INVALID;
+  return blocks_launched(launch_dependent(pair_kernel<BN, BLOCK>, dim3((unsigned)(2 * (tiles < room ? tiles : room))),
+                                          kPairThreads, S::kSmem, stream, P));
+}
+
+uint32_t choose_form(uint64_t p_rows, uint64_t q_rows, uint32_t stages, bool swap) {
+  const uint64_t sms = (uint64_t)sm_count(), pairs = sms / 2;
+  auto tiles = [&](uint64_t rows, uint64_t cols) { return ((p_rows + rows - 1) / rows) * ((q_rows + cols - 1) / cols); };
+  uint32_t split = 1;
+  while (split < 8 && tiles(128, 128) * split * 2 <= sms && stages >= split * 4) split *= 2;
+  if (swap || q_rows <= 64 || split >= 4) return split;
+  // waves of tiles over the pairs, a 256-wide tile taking 1.6 times a 128-wide
+  // one (1536 x 1536 x 8192: 16.9 us in 36 tiles of 256, 15.7 in 72 of 128;
+  // 8192 x 4096 x 4096: 60 us in 7 waves, 82 in 14)
+  const uint64_t wide = (tiles(256, 256) + pairs - 1) / pairs * 16, narrow = (tiles(256, 128) + pairs - 1) / pairs * 10;
+  return wide < narrow ? 256 : 128;
+}
 
 }  // namespace blockmm
 }  // namespace t5e
@@ -489,7 +1057,8 @@ int t5e_block_scaled_mm(const t5e_block_mm* mm, void* stream) {
   if (a.k != b.k || a.scale_format != b.scale_format || a.scale_block != b.scale_block || !real(mm->d_type) ||
       (mm->c && !real(mm->c_type)))
     return T5E_ERR_INVALID;
-  if (mm->split != 0 && mm->split != 1 && mm->split != 2 && mm->split != 4 && mm->split != 8) return T5E_ERR_INVALID;
+  const int32_t form = mm->form;
+  if (form != 0 && form != 1 && form != 2 && form != 4 && form != 8 && form != 128 && form != 256) return T5E_ERR_INVALID;
   if (a.rows == 0 || b.rows == 0) return T5E_OK;
   const int bytes = mm->d_type == T5E_REAL_F32 ? 4 : 2;
   if (!mm->d || (reinterpret_cast<uintptr_t>(mm->d) & (bytes - 1)) ||
@@ -500,8 +1069,6 @@ int t5e_block_scaled_mm(const t5e_block_mm* mm, void* stream) {
   const bool swap = a.rows < b.rows && a.rows <= 128;
   const t5e_blocks &p = swap ? b : a, &q = swap ? a : b;
   Params P = {};
-  P.p_scales = static_cast<const uint8_t*>(p.scales);
-  P.q_scales = static_cast<const uint8_t*>(q.scales);
   P.multiplier_a = mm->multiplier_a;
   P.multiplier_b = mm->multiplier_b;
   P.c = mm->c;
@@ -513,19 +1080,19 @@ int t5e_block_scaled_mm(const t5e_block_mm* mm, void* stream) {
   P.q_rows = (uint32_t)q.rows;
   P.k = (uint32_t)a.k;
   P.stages = (uint32_t)((a.k + kStageK - 1) / kStageK);
-  P.groups = scale_groups(a);
   P.alpha = mm->alpha;
   P.c_type = mm->c_type;
   P.d_type = mm->d_type;
-  uint32_t split = (uint32_t)mm->split;
-  if (split == 0) {
-    split = 1;
-    const uint64_t tiles = tiles_of(p.rows, q.rows);
-    while (split < 8 && tiles * split * 2 <= (uint64_t)sm_count() && P.stages >= split * 4) split *= 2;
-  }
-  if (split > P.stages) return T5E_ERR_INVALID;  // every part has work
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a.scale_block == 32 ? launch_form<32>(P, p, q, swap, split, s) : launch_form<16>(P, p, q, swap, split, s);
+  const uint32_t chosen = form != 0 ? (uint32_t)form : choose_form(p.rows, q.rows, P.stages, swap);
+  if (chosen >= 128) {
+    if (swap) return T5E_ERR_INVALID;  // few rows: a tile of 256 would be empty
+    if (chosen == 256)
+      return a.scale_block == 32 ? launch_pair<256, 32>(P, p, q, s) : launch_pair<256, 16>(P, p, q, s);
+    return a.scale_block == 32 ? launch_pair<128, 32>(P, p, q, s) : launch_pair<128, 16>(P, p, q, s);
+  }
+  if (chosen > P.stages) return T5E_ERR_INVALID;  // every part has work
+  return a.scale_block == 32 ? launch_form<32>(P, p, q, swap, chosen, s) : launch_form<16>(P, p, q, swap, chosen, s);
 }
 
 int t5e_block_scaled_mm_expired(int32_t* expired) {

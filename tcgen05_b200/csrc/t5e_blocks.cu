@@ -424,12 +424,41 @@ int quantize_cols(int32_t type, const void* x, uint64_t rows, uint64_t cols, int
   });
 }
 
+bool matrix_ok(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride) {
+  if (rows == 0 || cols == 0) return true;
+  return x && (reinterpret_cast<uintptr_t>(x) & (type_bytes(type) - 1)) == 0 && (rows == 1 || stride >= (int64_t)cols);
+}
+
+int partial_maxima(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
+                   int32_t count, cudaStream_t stream) {
+  if (rows == 0 || cols == 0) rows = cols = 0;
+  if (rows > 1 && stride == (int64_t)cols) {
+    cols *= rows;
+    rows = 1;
+  }
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows <= 1 || (stride * type_bytes(type)) % 16 == 0);
+  auto go = [&](auto t, auto v) {
+    return launched(launch_dependent(partials_kernel<decltype(t)::value, decltype(v)::value>, dim3((unsigned)count),
+                                     kThreads, 0, stream, x, rows, cols, stride, partials),
+                    "partials_kernel launch");
+  };
+  auto by_vec = [&](auto t) { return vec ? go(t, std::true_type{}) : go(t, std::false_type{}); };
+  if (type == T5E_REAL_F32) return by_vec(std::integral_constant<int, T5E_REAL_F32>{});
+  if (type == T5E_REAL_BF16) return by_vec(std::integral_constant<int, T5E_REAL_BF16>{});
+  return by_vec(std::integral_constant<int, T5E_REAL_F16>{});
+}
+
 }  // namespace blocks
 
 int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  const bool cached = dev >= 0 && dev < 64;
+  int sms = cached ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return 148;
+  if (cached) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 
@@ -452,43 +481,22 @@ bool blocks_ok(const t5e_blocks* b) {
 
 extern "C" {
 
-int t5e_block_partials(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
-                       int32_t count, void* stream) {
+int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
+                         int32_t count, float* multiplier, void* stream) {
   using namespace t5e;
   using namespace t5e::blocks;
-  if (!type_ok(type) || !partials || count < 1 || count > T5E_MAX_PARTIALS) return T5E_ERR_INVALID;
-  if (rows && cols && (!x || (reinterpret_cast<uintptr_t>(x) & (type_bytes(type) - 1)) ||
-                       (rows > 1 && stride < (int64_t)cols)))
+  if (!type_ok(type) || !partials || !multiplier || count < 1 || count > T5E_MAX_PARTIALS ||
+      !matrix_ok(type, x, rows, cols, stride))
     return T5E_ERR_INVALID;
-  if (rows == 0 || cols == 0) rows = cols = 0;
-  if (rows > 1 && stride == (int64_t)cols) {
-    cols *= rows;
-    rows = 1;
-  }
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows <= 1 || (stride * type_bytes(type)) % 16 == 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto t, auto v) {
-    return launched(launch_dependent(partials_kernel<decltype(t)::value, decltype(v)::value>, dim3((unsigned)count),
-                                     kThreads, 0, s, x, rows, cols, stride, partials),
-                    "partials_kernel launch");
-  };
-  auto by_vec = [&](auto t) { return vec ? go(t, std::true_type{}) : go(t, std::false_type{}); };
-  if (type == T5E_REAL_F32) return by_vec(std::integral_constant<int, T5E_REAL_F32>{});
-  if (type == T5E_REAL_BF16) return by_vec(std::integral_constant<int, T5E_REAL_BF16>{});
-  return by_vec(std::integral_constant<int, T5E_REAL_F16>{});
-}
-
-int t5e_block_multiplier(const uint32_t* partials, int32_t count, float* multiplier, void* stream) {
-  using namespace t5e;
-  using namespace t5e::blocks;
-  if (!partials || !multiplier || count < 1 || count > T5E_MAX_PARTIALS) return T5E_ERR_INVALID;
-  return launched(launch_dependent(multiplier_kernel, dim3(1), kThreads, 0, static_cast<cudaStream_t>(stream), partials,
-                                   count, multiplier),
+  const int rc = partial_maxima(type, x, rows, cols, stride, partials, count, s);
+  if (rc != T5E_OK) return rc;
+  return launched(launch_dependent(multiplier_kernel, dim3(1), kThreads, 0, s, partials, count, multiplier),
                   "multiplier_kernel launch");
 }
 
 int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, int32_t rounding,
-                        float* multiplier, const uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
+                        float* multiplier, uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
                         const t5e_blocks* by_cols, void* stream) {
   using namespace t5e;
   using namespace t5e::blocks;
@@ -503,12 +511,15 @@ int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t col
   if (format == T5E_SCALE_UE4M3 ? rounding != T5E_SCALE_ROUND_NEAREST
                                 : rounding != T5E_SCALE_ROUND_FLOOR && rounding != T5E_SCALE_ROUND_CEIL)
     return T5E_ERR_INVALID;
-  if (rows && cols && (!x || (reinterpret_cast<uintptr_t>(x) & (type_bytes(type) - 1)) ||
-                       (rows > 1 && stride < (int64_t)cols)))
-    return T5E_ERR_INVALID;
+  if (!matrix_ok(type, x, rows, cols, stride)) return T5E_ERR_INVALID;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool ceil = rounding == T5E_SCALE_ROUND_CEIL;
-  if (rows == 0 || cols == 0) return partials ? t5e_block_multiplier(partials, count, multiplier, stream) : T5E_OK;
+  if (rows == 0 || cols == 0)
+    return partials ? t5e_block_multiplier(type, x, rows, cols, stride, partials, count, multiplier, stream) : T5E_OK;
+  if (partials) {
+    const int rc = partial_maxima(type, x, rows, cols, stride, partials, count, s);
+    if (rc != T5E_OK) return rc;
+  }
   if (by_rows) {
     const int rc = quantize_rows(type, x, rows, cols, stride, ceil, multiplier, partials, count, *by_rows, s);
     if (rc != T5E_OK) return rc;

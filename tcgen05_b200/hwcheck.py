@@ -573,15 +573,15 @@ def emulated_product(a, b):
     return c[0]
 
 
-def cross_check_product(a, b, split: int = 1) -> dict:
-    """Words of ``block_scaled_mm`` in F32 (K in one part unless `split` says
-    otherwise) and of the emulated chain, multipliers left out."""
+def cross_check_product(a, b, form: int = 1) -> dict:
+    """Words of ``block_scaled_mm`` in F32 (`form` as in t5e_block_mm; 1: K in
+    one part) and of the emulated chain, multipliers left out."""
     import torch
 
     from .blocks import BlockScaledRows, _mm
 
     a, b = (BlockScaledRows(q.data, q.scales, q.k, scaling=q.scaling, scale_vec=q.scale_vec) for q in (a, b))
-    hw = _mm(a, b, None, 1.0, torch.float32, None, split)
+    hw = _mm(a, b, None, 1.0, torch.float32, None, form)
     emu = emulated_product(a, b)
     diff = (hw.view(torch.int32) != emu) & ~(torch.isnan(hw) & torch.isnan(emu.view(torch.float32)))
     return {"product": [a.rows, b.rows, a.k], "scaling": a.scaling, "scale_vec": a.scale_vec, "cases": hw.numel(),

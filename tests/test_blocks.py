@@ -207,9 +207,8 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 128, 0, None, 4096, 4, q, None, None) == nat.ERR_INVALID
     assert lib.t5e_quantize_blocks(0, 4096, 9, 128, 128, 0, None, None, 0, q, None, None) == nat.ERR_INVALID
     assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 128, 0, None, None, 0, None, None, None) == nat.ERR_INVALID
-    assert lib.t5e_block_partials(0, 4096, 8, 128, 128, 4096, 0, None) == nat.ERR_INVALID
-    assert lib.t5e_block_partials(0, 4096, 8, 128, 128, 4096, nat.MAX_PARTIALS + 1, None) == nat.ERR_INVALID
-    assert lib.t5e_block_multiplier(None, 4, 4096, None) == nat.ERR_INVALID
+    for partials, count, out in ((4096, 0, 4096), (4096, nat.MAX_PARTIALS + 1, 4096), (None, 4, 4096), (4096, 4, None)):
+        assert lib.t5e_block_multiplier(0, 4096, 8, 128, 128, partials, count, out, None) == nat.ERR_INVALID
 
     def mm(**kw):
         m = nat.BlockMm(ctypes.pointer(good), ctypes.pointer(blk()), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
@@ -219,7 +218,7 @@ def test_c_entry_points_refuse_bad_arguments():
 
     other = blk(scale_format=nat.SCALE_UE8M0)
     for kw in (dict(d=None), dict(d=4098), dict(d_stride=7), dict(d_type=3), dict(c=4096, c_type=5), dict(c=4098),
-               dict(split=3), dict(split=16), dict(split=2), dict(b=ctypes.pointer(other)), dict(a=None)):
+               dict(form=3), dict(form=16), dict(form=2), dict(b=ctypes.pointer(other)), dict(a=None)):
         assert mm(**kw) == nat.ERR_INVALID, kw
     assert lib.t5e_block_scaled_mm_expired(None) == nat.ERR_INVALID
 
@@ -471,6 +470,47 @@ def test_product_is_the_emulated_chain_word_for_word(form, m, n, k):
     r = hwcheck.cross_check_product(t5.quantize_blocks(make(m, m, k, wide=True), **kw),
                                     t5.quantize_blocks(make(n + 1, n, k), **kw))
     assert r["cases"] == m * n and r["mismatches"] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
+@pytest.mark.parametrize("kernel", [1, 128, 256])
+@pytest.mark.parametrize("m,n,k", [(129, 129, 64), (300, 257, 700), (256, 512, 1344), (700, 1030, 2100), (2600, 3000, 300)])
+def test_every_kernel_form_is_the_emulated_chain(form, kernel, m, n, k):
+    """The tile kernel and both pair kernels, one tile and several per block,
+    K that ends in every step of a stage."""
+    from tcgen05_b200 import hwcheck
+
+    kw = dict(scaling=form[0], scale_vec=form[1])
+    r = hwcheck.cross_check_product(t5.quantize_blocks(make(m, m, k, wide=True), **kw),
+                                    t5.quantize_blocks(make(n + 1, n, k), **kw), kernel)
+    assert r["mismatches"] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", [1, 128, 256])
+@pytest.mark.parametrize("m,n", [(300, 264), (300, 267), (520, 1000)])
+def test_every_kernel_forms_outputs(kernel, m, n):
+    """Result types, rows on and off 16-byte boundaries, addends, into part of a
+    larger tensor."""
+    a, b = t5.quantize_blocks(make(m, m, 500), multiplier="auto"), t5.quantize_blocks(make(n, n, 500), multiplier=0.5)
+    va, vb = t5.dequantize_blocks(a).double(), t5.dequantize_blocks(b).double()
+    exact, err = va @ vb.t(), product_bound(va, vb, 500, 0)
+    for dtype in TYPES:
+        eps, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        for c in (None, make(1, m, n, dtype=dtype), make(2, n), make(3, n, m).t()):
+            for pad in (0, 3, 8):
+                big = torch.full((m + 2, n + 2 * pad), 7.0, dtype=dtype, device="cuda")
+                out = big[1:m + 1, pad:n + pad]
+                got = bk._mm(a, b, c, -0.75, dtype, out, kernel)
+                want = -0.75 * exact + (0 if c is None else c.double())
+                room = 0.75 * err + 1.01 * eps * (want.abs() + err) + tiny
+                if c is not None:
+                    room = room + 2.0 ** -24 * c.double().abs()
+                assert got.data_ptr() == out.data_ptr()
+                assert bool(((got.double() - want).abs() <= room).all())
+                out.fill_(7)
+                assert bool((big == 7).all())
 
 
 @pytest.mark.gpu
