@@ -369,7 +369,7 @@ int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t co
 
 /* Rounds x [rows, cols] (row stride in elements) to blocks along its rows
  * (by_rows: rows = rows, k = cols), along its columns (by_cols: rows = cols,
- * k = rows), or both; the pointer of the one not wanted is NULL.
+ * k = rows), or both; the data pointer of the one not wanted is NULL.
  *   u = F32(x * m), m = *multiplier or 1 (NULL); a = max|u| of a block;
  *   UE4M3: scale = RNE(min(a / 6, 448)); UE8M0: 2^(floor(log2 a) - 2) or
  *   (CEIL) the smallest power of two >= a / 6, held to 2^+-127;
@@ -378,9 +378,24 @@ int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t co
  * scale gets codes that are zeros.  With partials != NULL (a workspace of
  * `count` words) the multiplier is first computed as by t5e_block_multiplier
  * and stored to *multiplier. */
-int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, int32_t rounding,
-                        float* multiplier, uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
-                        const t5e_blocks* by_cols, void* stream);
+typedef struct t5e_quantize {
+    const void* x;
+    uint64_t rows;
+    uint64_t cols;
+    int64_t stride;
+    int32_t type;
+    int32_t rounding;
+    float* multiplier;
+    uint32_t* partials;
+    int32_t count;
+    int32_t reserved;            /* 0 */
+    t5e_blocks by_rows;
+    t5e_blocks by_cols;
+} t5e_quantize;
+
+/* One tensor, or two of one type and one block form in the launches of one
+ * (n = 1 or 2). */
+int t5e_quantize_blocks(const t5e_quantize* q, int32_t n, void* stream);
 
 /* out[r][i] = code * scale * F32(1 / m) rounded to `type`; out_stride in
  * elements. */

@@ -127,6 +127,25 @@ class Blocks(ctypes.Structure):
     ]
 
 
+class Quantize(ctypes.Structure):
+    """t5e_quantize: one tensor to round to blocks."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("cols", ctypes.c_uint64),
+        ("stride", ctypes.c_int64),
+        ("type", ctypes.c_int32),
+        ("rounding", ctypes.c_int32),
+        ("multiplier", ctypes.c_void_p),
+        ("partials", ctypes.c_void_p),
+        ("count", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("by_rows", Blocks),
+        ("by_cols", Blocks),
+    ]
+
+
 class BlockMm(ctypes.Structure):
     """t5e_block_mm: one product of block-scaled rows."""
 
@@ -228,10 +247,7 @@ def load() -> ctypes.CDLL:
                                          ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
                                          ctypes.c_void_p]
     lib.t5e_quantize_blocks.restype = ctypes.c_int
-    lib.t5e_quantize_blocks.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64,
-                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
-                                        ctypes.c_int32, ctypes.POINTER(Blocks), ctypes.POINTER(Blocks),
-                                        ctypes.c_void_p]
+    lib.t5e_quantize_blocks.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
     lib.t5e_dequantize_blocks.restype = ctypes.c_int
     lib.t5e_dequantize_blocks.argtypes = [ctypes.POINTER(Blocks), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
                                           ctypes.c_int64, ctypes.c_void_p]

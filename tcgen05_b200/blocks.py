@@ -198,7 +198,8 @@ class _On:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
+        # torch.cuda.current_stream(index).cuda_stream, without building a Stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
@@ -300,6 +301,9 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
     return _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier)
 
 
+_NO_BLOCKS = nat.Blocks()
+
+
 def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier):
     """quantize_blocks of checked arguments, x as r rows of k: the rows, the
     columns or the pair."""
@@ -314,18 +318,21 @@ def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplie
                 if r:
                     count = _partial_count(r * k)
                     work = torch.empty(1 + count, dtype=torch.float32, device=device)
-                    partials, multiplier = work.data_ptr() + 4, work[:1]
-            elif not isinstance(multiplier, torch.Tensor):
-                multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
-            at = None if multiplier is None else multiplier.data_ptr()
+                    at = work.data_ptr()
+                    partials, multiplier = at + 4, work[:1]
+            else:
+                if not isinstance(multiplier, torch.Tensor):
+                    multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
+                at = multiplier.data_ptr()
         rows = BlockScaledRows._within(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
         cols = BlockScaledRows._within(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
-        along, across = (cols, rows) if turned else (rows, cols)
-        shape = m.shape
-        nat.check(lib.t5e_quantize_blocks(
-            _REAL[m.dtype], m.data_ptr(), shape[0], shape[1], m.stride(0), rounding, at, partials, count,
-            None if along is None else ctypes.byref(along._struct),
-            None if across is None else ctypes.byref(across._struct), handle), "t5e_quantize_blocks")
+        if r:
+            along, across = (cols, rows) if turned else (rows, cols)
+            shape = m.shape
+            nat.check(lib.t5e_quantize_blocks(ctypes.byref(nat.Quantize(
+                m.data_ptr(), shape[0], shape[1], m.stride(0), _REAL[m.dtype], rounding, at, partials, count, 0,
+                _NO_BLOCKS if along is None else along._struct, _NO_BLOCKS if across is None else across._struct)),
+                1, handle), "t5e_quantize_blocks")
     if by_rows and by_cols:
         return rows, cols
     return rows if by_rows else cols
@@ -434,51 +441,137 @@ def _mm(a, b, c, alpha, dtype, out, form):
     return out
 
 
+class _Space:
+    """One allocation for several parts: sizes are added up first, the addresses
+    hold once it is made."""
+
+    __slots__ = ("size", "buffer", "at")
+
+    def __init__(self, at: int = 0):
+        self.size = at
+
+    def take(self, n: int) -> int:
+        """Offset of n more bytes."""
+        at = self.size
+        self.size = (at + n + 255) // 256 * 256
+        return at
+
+    def blocks(self, rows: int, k: int, scaling, scale_vec):
+        """(offset, unfinished t5e_blocks) of rows with their scales."""
+        fmt, block = _FORMS[scaling, scale_vec]
+        stride = (k + 31) // 32 * 16
+        return self.take(rows * stride + (rows + 127) // 128 * (-(-k // (4 * block)) * 512)), \
+            nat.Blocks(0, stride, rows * stride, rows, k, fmt, block)
+
+
+def _placed(part, base: int) -> nat.Blocks:
+    """The t5e_blocks of a `_Space.blocks` part of the allocation at `base`."""
+    at, b = part
+    b.data = base + at
+    b.scales = base + at + b.rows * b.stride
+    return b
+
+
+def _quantize_job(x, form, at, partials, count, rows, cols):
+    m, turned = _matrix_of(x)
+    if turned:
+        rows, cols = cols, rows
+    shape = m.shape
+    # the matrix is returned too: a copy of it has to live until the launch
+    return m, nat.Quantize(m.data_ptr(), shape[0], shape[1], m.stride(0), _REAL[m.dtype], form[2], at, partials, count, 0,
+                           _NO_BLOCKS if rows is None else rows, _NO_BLOCKS if cols is None else cols)
+
+
+def _product(lib, a, b, ma, mb, shape, dtype, device, handle):
+    """block_scaled_mm of t5e_blocks."""
+    out = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    mm = nat.BlockMm(ctypes.pointer(a), ctypes.pointer(b), ma, mb, 1.0, 0, None, 0, _REAL[dtype], 0, 0, out.data_ptr(),
+                     shape[1])
+    nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
+    return out
+
+
 class _Linear(torch.autograd.Function):
+    """The three products of block_scaled_linear.  The calls are those of
+    quantize_blocks and block_scaled_mm, x and w rounded in the same launches
+    and everything a pass needs in one allocation: a small layer's time is
+    its launches."""
+
     @staticmethod
     def forward(ctx, x, w, scaling, scale_vec, rounding, need_x, need_w):
         (n, k), tokens = w.shape, x.numel() // w.shape[1]
-        form = (scaling, scale_vec, rounding, "auto" if scaling == "ue4m3" else None)
-        # blocks run along the contraction: K here, the tokens and N in the
-        # gradients, so what a gradient needs is rounded along the other axis
-        need_x, need_w = need_x and tokens > 0, need_w and tokens > 0
-        qx = _quantize(x, tokens, k, True, need_w, *form)
-        qw = _quantize(w, n, k, True, need_x, *form)
-        ctx.form, ctx.need = form, (need_x, need_w)
-        kept = []
-        if need_w:
-            qx, xt = qx
-            kept += [xt._buffer, xt.multiplier]
-        if need_x:
-            qw, wt = qw
-            kept += [wt._buffer, wt.multiplier]
-        ctx.save_for_backward(*kept)
         ctx.shapes = x.shape, w.shape
-        y = _mm(qx, qw, None, 1.0, x.dtype, None, 0)
+        if not tokens:
+            ctx.form = None
+            return x.new_empty((*x.shape[:-1], n))
+        form = ctx.form = (scaling, scale_vec, rounding)
+        auto = scaling == "ue4m3"
+        # blocks run along the contraction: K here, the tokens and N in the
+        # gradients, so what a gradient needs is rounded along the other axis.
+        # Kept for the backward pass: the multipliers, then the columns
+        kept = _Space(256)
+        xt = kept.blocks(k, tokens, scaling, scale_vec) if need_w else None
+        wt = kept.blocks(k, n, scaling, scale_vec) if need_x else None
+        passing = _Space()
+        xr, wr = passing.blocks(tokens, k, scaling, scale_vec), passing.blocks(n, k, scaling, scale_vec)
+        x_count, w_count = (_partial_count(tokens * k), _partial_count(n * k)) if auto else (0, 0)
+        partials = passing.take(4 * (x_count + w_count))
+        device = x.device
+        lib = nat.load()
+        with _On(device.index) as handle:
+            keep = torch.empty(kept.size, dtype=torch.uint8, device=device)
+            work = torch.empty(passing.size, dtype=torch.uint8, device=device)
+            base, there = keep.data_ptr(), work.data_ptr()
+            xr, wr = _placed(xr, there), _placed(wr, there)
+            partials += there
+            mx, mw = (base, base + 4) if auto else (None, None)
+            x1, jx = _quantize_job(x, form, mx, partials if auto else None, x_count, xr,
+                                   None if xt is None else _placed(xt, base))
+            w1, jw = _quantize_job(w, form, mw, partials + 4 * x_count if auto else None, w_count, wr,
+                                   None if wt is None else _placed(wt, base))
+            nat.check(lib.t5e_quantize_blocks((nat.Quantize * 2)(jx, jw), 2, handle), "t5e_quantize_blocks")
+            y = _product(lib, xr, wr, mx, mw, (tokens, n), x.dtype, device, handle)
+        ctx.parts = xt, wt
+        ctx.save_for_backward(keep)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        (need_x, need_w), form = ctx.need, ctx.form
         x_shape, (n, k) = ctx.shapes
-        tokens = g.numel() // n
-        asked_x, asked_w = ctx.needs_input_grad[:2]
-        dx = g.new_zeros(x_shape) if asked_x and not tokens else None
-        dw = g.new_zeros(n, k) if asked_w and not tokens else None
-        need_x, need_w = need_x and asked_x, need_w and asked_w
+        need_x, need_w = ctx.needs_input_grad[:2]
+        form = ctx.form
+        if form is None:
+            return (g.new_zeros(x_shape) if need_x else None, g.new_zeros(n, k) if need_w else None,
+                    None, None, None, None, None)
+        dx = dw = None
         if need_x or need_w:
-            kept = ctx.saved_tensors
-            q = _quantize(g, tokens, n, need_x, need_w, *form)
-            rows, cols = q if need_x and need_w else (q, q)
-            if need_x:
-                wt = BlockScaledRows._within(kept[-2], k, n, *form[:2], kept[-1])
-                dx = _mm(rows, wt, None, 1.0, g.dtype, None, 0)
-                if len(x_shape) != 2:
-                    dx = dx.view(x_shape)
-            if need_w:
-                xt = BlockScaledRows._within(kept[0], k, tokens, *form[:2], kept[1])
-                dw = _mm(cols, xt, None, 1.0, g.dtype, None, 0)
+            tokens = g.numel() // n
+            scaling, scale_vec, _ = form
+            auto = scaling == "ue4m3"
+            space = _Space()
+            gr = space.blocks(tokens, n, scaling, scale_vec) if need_x else None
+            gt = space.blocks(n, tokens, scaling, scale_vec) if need_w else None
+            count = _partial_count(tokens * n) if auto else 0
+            small = space.take(4 * (1 + count))
+            device = g.device
+            lib = nat.load()
+            keep, = ctx.saved_tensors
+            with _On(device.index) as handle:
+                work = torch.empty(space.size, dtype=torch.uint8, device=device)
+                base, there = keep.data_ptr(), work.data_ptr()
+                mx, mw, mg = (base, base + 4, there + small) if auto else (None, None, None)
+                gr = None if gr is None else _placed(gr, there)
+                gt = None if gt is None else _placed(gt, there)
+                g1, job = _quantize_job(g, form, mg, mg + 4 if auto else None, count, gr, gt)
+                nat.check(lib.t5e_quantize_blocks(ctypes.byref(job), 1, handle), "t5e_quantize_blocks")
+                xt, wt = ctx.parts
+                if need_x:
+                    dx = _product(lib, gr, _placed(wt, base), mg, mw, (tokens, k), g.dtype, device, handle)
+                    if len(x_shape) != 2:
+                        dx = dx.view(x_shape)
+                if need_w:
+                    dw = _product(lib, gt, _placed(xt, base), mg, mx, (n, k), g.dtype, device, handle)
         return dx, dw, None, None, None, None, None
 
 

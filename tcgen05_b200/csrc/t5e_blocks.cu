@@ -67,24 +67,53 @@ __device__ __forceinline__ uint32_t element_bits(const void* x, uint64_t i) {
   else return static_cast<const uint16_t*>(x)[i] & 0x7FFFu;
 }
 
-template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(kThreads) partials_kernel(const void* __restrict__ x, uint64_t rows, uint64_t cols,
-                                                            int64_t stride, uint32_t* __restrict__ partials) {
+// One tensor of a launch: what to read, what to write.  Launches take two, and
+// blocks of the grid from `first_block` on work on the second.
+struct Job {
+  const void* x;
+  uint64_t rows, cols;
+  int64_t stride;
+  float* multiplier;
+  uint32_t* partials;  // NULL: the multiplier is given
+  int32_t count;
+  uint32_t first_block;
+  bool vec;            // rows start on 16-byte boundaries
+  uint8_t* row_data;   // NULL: no blocks along the rows
+  int64_t row_stride;
+  uint8_t* row_scales;
+  uint32_t row_groups;
+  uint8_t* col_data;   // NULL: no blocks along the columns
+  int64_t col_stride;
+  uint8_t* col_scales;
+  uint32_t col_groups;
+};
+struct Jobs {
+  Job job[2];
+};
+
+__device__ __forceinline__ const Job& job_of(const Jobs& jobs) {
+  return jobs.job[blockIdx.x >= jobs.job[1].first_block ? 1 : 0];
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) partials_kernel(const __grid_constant__ Jobs jobs) {
   __shared__ uint32_t shared[kThreads / 32];
+  const Job& J = job_of(jobs);
   let_next_grid_start();
   wait_for_previous_grid();
   constexpr int kPer = 16 / Real<TYPE>::kBytes;
   uint32_t best = 0u;
   // a contiguous tensor comes as one row, which all blocks share; otherwise
   // each block takes whole rows
-  const bool one = rows == 1;
-  const uint64_t first = one ? (uint64_t)blockIdx.x * kThreads + threadIdx.x : threadIdx.x;
-  const uint64_t step = one ? (uint64_t)gridDim.x * kThreads : kThreads;
-  for (uint64_t r = one ? 0 : blockIdx.x; r < rows; r += one ? 1 : gridDim.x) {
-    const char* row = static_cast<const char*>(x) + (int64_t)r * stride * Real<TYPE>::kBytes;
+  const bool one = J.rows == 1;
+  const uint32_t block = blockIdx.x - J.first_block;
+  const uint64_t first = one ? (uint64_t)block * kThreads + threadIdx.x : threadIdx.x;
+  const uint64_t step = one ? (uint64_t)J.count * kThreads : kThreads;
+  for (uint64_t r = one ? 0 : block; r < J.rows; r += one ? 1 : J.count) {
+    const char* row = static_cast<const char*>(J.x) + (int64_t)r * J.stride * Real<TYPE>::kBytes;
     uint64_t done = 0;
-    if constexpr (VEC) {
-      const uint64_t vecs = cols / kPer;
+    if (J.vec) {
+      const uint64_t vecs = J.cols / kPer;
       const uint4* p = reinterpret_cast<const uint4*>(row);
       uint64_t i = first;
       for (; i + 3 * step < vecs; i += 4 * step) {
@@ -103,10 +132,10 @@ __global__ void __launch_bounds__(kThreads) partials_kernel(const void* __restri
       }
       done = vecs * kPer;
     }
-    for (uint64_t i = done + first; i < cols; i += step) best = join_max<TYPE>(best, element_bits<TYPE>(row, i));
+    for (uint64_t i = done + first; i < J.cols; i += step) best = join_max<TYPE>(best, element_bits<TYPE>(row, i));
   }
   const uint32_t m = block_max(final_max<TYPE>(best), shared);
-  if (threadIdx.x == 0) partials[blockIdx.x] = m;
+  if (threadIdx.x == 0) J.partials[block] = m;
 }
 
 __global__ void __launch_bounds__(kThreads) multiplier_kernel(const uint32_t* __restrict__ partials, int count,
@@ -121,18 +150,26 @@ __global__ void __launch_bounds__(kThreads) multiplier_kernel(const uint32_t* __
 }
 
 // The multiplier a quantising block works with: none, given, or taken from the
-// partial maxima (every block joins them for itself, which saves a launch;
-// block 0 stores the result).
-__device__ __forceinline__ float load_multiplier(float* multiplier, const uint32_t* partials, int count,
-                                                 uint32_t* shared) {
-  if (partials != nullptr) {
+// partial maxima (every block joins them for itself, which saves a launch; the
+// job's first block stores the result).
+__device__ __forceinline__ float load_multiplier(const Job& J, uint32_t* shared) {
+  if (J.partials != nullptr) {
     uint32_t best = 0u;
-    for (int i = threadIdx.x; i < count; i += blockDim.x) best = max(best, __ldg(partials + i));
+    for (int i = threadIdx.x; i < J.count; i += kThreads) best = max(best, J.partials[i]);
     const float m = multiplier_of(block_max(best, shared));
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *multiplier = m;
+    if (blockIdx.x == J.first_block && threadIdx.x == 0) *J.multiplier = m;
     return m;
   }
-  return multiplier != nullptr ? *multiplier : 1.f;
+  return J.multiplier != nullptr ? *J.multiplier : 1.f;
+}
+
+// n / d for n < 2^31: mul = floor(2^(31 + shift) / d) + 1 with 2^(shift-1) < d <=
+// 2^shift (d > 1).
+struct Divider {
+  uint32_t d, mul, shift;
+};
+__device__ __forceinline__ uint32_t divided(uint32_t n, const Divider& v) {
+  return v.d == 1u ? n : __umulhi(n, v.mul) >> (v.shift - 1);
 }
 
 // ---- blocks along the rows ---------------------------------------------------
@@ -141,30 +178,23 @@ __device__ __forceinline__ float load_multiplier(float* multiplier, const uint32
 // one whose other half its neighbour lane holds.  Per row the chunks run up
 // to a whole group of four scales, so that four (eight) neighbouring lanes
 // always hold one group and one of them stores its four scale bytes as a word.
-template <int TYPE, bool E8M0, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __restrict__ x, uint32_t rows, uint64_t row0,
-                                                                 uint32_t k, int64_t stride, bool ceil,
-                                                                 float* multiplier, const uint32_t* partials, int count,
-                                                                 uint8_t* __restrict__ data, int64_t data_stride,
-                                                                 uint8_t* __restrict__ scales, uint32_t groups) {
-  __shared__ uint32_t shared[kThreads / 32];
-  let_next_grid_start();
-  wait_for_previous_grid();
-  const float m = load_multiplier(multiplier, partials, count, shared);
-  constexpr uint32_t kLanes = BLOCK / 4;               // lanes of one group of four scales
-  const uint32_t chunks = groups * kLanes;             // 16-element chunks per row
-  const uint32_t stored = ((k + 31u) / 32u) * 2u;      // chunks with codes in `data`
-  const uint32_t total = rows * chunks;
+template <int TYPE, bool E8M0, int BLOCK, int HOW>
+__device__ __forceinline__ void round_rows(const Job& J, uint32_t rows, uint64_t row0, const Divider& chunks, bool ceil,
+                                           float m) {
+  constexpr uint32_t kLanes = BLOCK / 4;  // lanes of one group of four scales
+  const uint32_t k = (uint32_t)J.cols;
+  const uint32_t stored = ((k + 31u) / 32u) * 2u;  // chunks with codes in `data`
+  const uint32_t total = rows * chunks.d;
   const int lane = threadIdx.x & 31;
   for (uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u); base < total; base += gridDim.x * kThreads) {
     const uint32_t item = base + lane;
     const bool in = item < total;
-    const uint32_t row = in ? item / chunks : 0u, chunk = in ? item - row * chunks : 0u;
+    const uint32_t row = in ? divided(item, chunks) : 0u, chunk = in ? item - row * chunks.d : 0u;
     const uint32_t e0 = chunk * 16u;
     float v[16];
     uint32_t top = 0u;
-    const char* src = static_cast<const char*>(x) + ((int64_t)(row0 + row) * stride + e0) * Real<TYPE>::kBytes;
-    if (VEC && in && e0 + 16u <= k) {
+    const char* src = static_cast<const char*>(J.x) + ((int64_t)(row0 + row) * J.stride + e0) * Real<TYPE>::kBytes;
+    if (J.vec && in && e0 + 16u <= k) {
       constexpr int kVecs = Real<TYPE>::kBytes;  // 16-byte vectors of 16 elements
       uint4 w[kVecs];
 #pragma unroll
@@ -187,16 +217,15 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __r
     }
     if constexpr (BLOCK == 32) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     float step, inv;
-    // rounding to F32 is monotonic: the largest product is the product of the largest
-    uint32_t word = block_scale<E8M0>(__uint_as_float(top) * m, ceil, step, inv);
+    uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, step, inv);
     const bool finite = word != (E8M0 ? 0xFFu : 0x7Fu);
     if (e0 / BLOCK * BLOCK >= k) word = 0u;  // a scale behind the last block
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = divide<E8M0>(v[j] * m, step, inv);
+    for (int j = 0; j < 16; ++j) v[j] = divide<E8M0, HOW>(v[j], m, step, inv);
     uint2 codes = make_uint2(e2m1x8(v), e2m1x8(v + 8));
     if (!finite) codes = make_uint2(0u, 0u);
     if (in && chunk < stored)
-      *reinterpret_cast<uint2*>(data + (int64_t)(row0 + row) * data_stride + chunk * 8u) = codes;
+      *reinterpret_cast<uint2*>(J.row_data + (int64_t)(row0 + row) * J.row_stride + chunk * 8u) = codes;
     // four scale bytes to one word
     if constexpr (BLOCK == 16) {
       word <<= 8 * (lane & 3);
@@ -208,57 +237,113 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __r
       word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
     }
     if (in && lane % kLanes == 0)
-      *reinterpret_cast<uint32_t*>(scales + scale_offset(row0 + row, e0 / BLOCK, groups)) = word;
+      *reinterpret_cast<uint32_t*>(J.row_scales + scale_offset(row0 + row, e0 / BLOCK, J.row_groups)) = word;
   }
 }
 
-// ---- blocks along the columns -------------------------------------------------
-//
-// Element i of output row c is x[i][c].  A warp takes 32 rows by 64 columns: a
-// lane holds two neighbouring columns of all 32 rows in registers (two
-// 16-element blocks or one of 32), so the maxima need no exchange and every
-// load is one line of a row.  Eight warps stack to 256 rows; the codes are
-// turned through shared memory so that each output row gets 128 consecutive
-// bytes.
-constexpr int kColTileC = 64, kColTileR = 256, kColPitch = kColTileR / 2 + 16;
-
-template <int TYPE, bool E8M0, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_cols_kernel(const void* __restrict__ x, uint64_t rows, uint64_t cols,
-                                                                 int64_t stride, bool ceil, float* multiplier,
-                                                                 const uint32_t* partials, int count,
-                                                                 uint8_t* __restrict__ data, int64_t data_stride,
-                                                                 uint8_t* __restrict__ scales, uint32_t groups) {
+template <int TYPE, bool E8M0, int BLOCK>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ Jobs jobs, uint32_t rows,
+                                                                 uint64_t row0, Divider chunks, bool ceil) {
   __shared__ uint32_t shared[kThreads / 32];
-  __shared__ __align__(16) uint8_t codes[kColTileC * kColPitch];
-  __shared__ __align__(16) uint8_t steps[kColTileC * (kColTileR / 16)];
+  const Job& J = jobs.job[0];
   let_next_grid_start();
   wait_for_previous_grid();
-  const float m = load_multiplier(multiplier, partials, count, shared);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kSteps = kColTileR / BLOCK;  // scales of a tile per column
-  const uint64_t c0 = (uint64_t)blockIdx.x * kColTileC;
-  const uint64_t padded = (rows + 31) / 32 * 32;
-  for (uint64_t r0 = (uint64_t)blockIdx.y * kColTileR; r0 < padded; r0 += (uint64_t)gridDim.y * kColTileR) {
-    const uint64_t r = r0 + warp * 32, c = c0 + lane * 2;
-    using T = typename Real<TYPE>::type;
-    const T* src = static_cast<const T*>(x) + (int64_t)r * stride + (int64_t)c;
-    float v[2][32];
-    if (VEC && r + 32 <= rows && c + 2 <= cols) {
+  const float m = load_multiplier(J, shared);
+  if (is_narrow<TYPE, E8M0>(m)) round_rows<TYPE, E8M0, BLOCK, kNarrow>(J, rows, row0, chunks, ceil, m);
+  else round_rows<TYPE, E8M0, BLOCK, kExact>(J, rows, row0, chunks, ceil, m);
+}
+
+// ---- blocks along the columns, or along both axes in one read -----------------------
+//
+// A block of 256 threads takes a tile of 128 x 128 elements into shared memory.
+// Along the rows a thread rounds 16 neighbouring elements, four times; along
+// the columns it rounds two neighbouring columns of 32 rows (two 16-element
+// blocks or one of 32), so that neither maximum needs an exchange beyond a
+// neighbour lane.  Codes and scale bytes of the columns are put in order in
+// shared memory: each output row gets 64 consecutive bytes, and the scale
+// tiles of 128 rows leave whole.
+constexpr int kTile = 128, kColPitch = kTile / 2 + 16;
+
+template <int TYPE>
+struct TileBytes {
+  static constexpr int kPitch = kTile * Real<TYPE>::kBytes + 16;
+  static constexpr int kInput = kTile * kPitch;
+  static constexpr int kCodes = kTile * kColPitch;
+  static constexpr int kSteps = kTile * (kTile / 16);  // scale bytes of one axis, in the tiles' order
+  static constexpr int kAll = kInput + kCodes + 2 * kSteps;
+};
+
+// Where scale b (of 8 or 4 per row of the tile) of row r belongs in the tile's
+// own scale tiles.
+__device__ __forceinline__ int step_at(int r, int b) { return (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3); }
+
+template <int TYPE, bool E8M0, int BLOCK, int HOW>
+__device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t r0, uint64_t c0, bool ceil, float m) {
+  using B = TileBytes<TYPE>;
+  uint8_t* input = smem;
+  uint8_t* codes = smem + B::kInput;
+  uint8_t* row_steps = codes + B::kCodes;
+  uint8_t* col_steps = row_steps + B::kSteps;
+  constexpr int kNan = E8M0 ? 0xFF : 0x7F;
+  const int t = threadIdx.x;
+  if (J.row_data != nullptr) {
+    const uint64_t padded = (J.cols + 31) / 32 * 32;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if constexpr (TYPE == T5E_REAL_F32) {
-          const float2 f = __ldg(reinterpret_cast<const float2*>(src + i * stride));
-          v[0][i] = f.x;
-          v[1][i] = f.y;
-        } else {
-          unpack2<TYPE>(__ldg(reinterpret_cast<const uint32_t*>(src + i * stride)), v[0][i], v[1][i]);
-        }
+    for (int i = 0; i < kTile * (kTile / 16) / kThreads; ++i) {
+      const int item = i * kThreads + t, r = item >> 3, chunk = item & 7;
+      const uint4* src = reinterpret_cast<const uint4*>(input + r * B::kPitch + chunk * 16 * Real<TYPE>::kBytes);
+      uint32_t words[4 * Real<TYPE>::kBytes];
+#pragma unroll
+      for (int j = 0; j < Real<TYPE>::kBytes; ++j) reinterpret_cast<uint4*>(words)[j] = src[j];
+      float v[16];
+      uint32_t top = 0u;
+#pragma unroll
+      for (int j = 0; j < 4 * Real<TYPE>::kBytes; ++j) {
+        top = join_max<TYPE>(top, word_max<TYPE>(words[j]));
+        if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(words[j]);
+        else unpack2<TYPE>(words[j], v[2 * j], v[2 * j + 1]);
       }
-    } else {
+      top = final_max<TYPE>(top);
+      if constexpr (BLOCK == 32) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      float step, inv;
+      uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, step, inv);
+      const bool finite = word != (uint32_t)kNan;
+      if (c0 + chunk * 16 / BLOCK * BLOCK >= J.cols) word = 0u;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        v[0][i] = r + i < rows && c < cols ? to_f32(src[i * stride]) : 0.f;
-        v[1][i] = r + i < rows && c + 1 < cols ? to_f32(src[i * stride + 1]) : 0.f;
+      for (int j = 0; j < 16; ++j) v[j] = divide<E8M0, HOW>(v[j], m, step, inv);
+      const uint2 out = finite ? make_uint2(e2m1x8(v), e2m1x8(v + 8)) : make_uint2(0u, 0u);
+      if (r0 + r < J.rows && c0 + chunk * 16 < padded)
+        *reinterpret_cast<uint2*>(J.row_data + (int64_t)(r0 + r) * J.row_stride + (int64_t)(c0 / 2) + chunk * 8) = out;
+      if (BLOCK == 16 || (chunk & 1) == 0) row_steps[step_at(r, chunk * 16 / BLOCK)] = (uint8_t)word;
+    }
+  }
+  if (J.col_data != nullptr) {
+    const int pair = t & 63, part = t >> 6;  // columns 2 pair, 2 pair + 1; rows 32 part ..
+    float v[2][32];
+    uint32_t top[2][32 / BLOCK];
+#pragma unroll
+    for (int b = 0; b < 32 / BLOCK; ++b) top[0][b] = top[1][b] = 0u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint8_t* src = input + (part * 32 + i) * B::kPitch + pair * 2 * Real<TYPE>::kBytes;
+      if constexpr (TYPE == T5E_REAL_F32) {
+        const float2 f = *reinterpret_cast<const float2*>(src);
+        v[0][i] = f.x;
+        v[1][i] = f.y;
+        top[0][i / BLOCK] = max(top[0][i / BLOCK], __float_as_uint(f.x) & 0x7FFFFFFFu);
+        top[1][i / BLOCK] = max(top[1][i / BLOCK], __float_as_uint(f.y) & 0x7FFFFFFFu);
+      } else {  // both columns' maxima in one word
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
+        top[0][i / BLOCK] = join_max<TYPE>(top[0][i / BLOCK], word_max<TYPE>(w));
+        unpack2<TYPE>(w, v[0][i], v[1][i]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 32 / BLOCK; ++b) {
+      if constexpr (TYPE != T5E_REAL_F32) {
+        const uint32_t both = top[0][b];
+        top[0][b] = magnitude_bits<TYPE>(both & 0xFFFFu);
+        top[1][b] = magnitude_bits<TYPE>(both >> 16);
       }
     }
 #pragma unroll
@@ -266,60 +351,104 @@ __global__ void __launch_bounds__(kThreads) quantize_cols_kernel(const void* __r
       uint32_t out[4];
 #pragma unroll
       for (int b = 0; b < 32 / BLOCK; ++b) {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < BLOCK; ++i) top = max(top, __float_as_uint(v[h][b * BLOCK + i]) & 0x7FFFFFFFu);
         float step, inv;
-        uint32_t word = block_scale<E8M0>(__uint_as_float(top) * m, ceil, step, inv);
-        const bool finite = word != (E8M0 ? 0xFFu : 0x7Fu);
-        if (r + b * BLOCK >= rows) word = 0u;
+        uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top[h][b]), m, ceil, step, inv);
+        const bool finite = word != (uint32_t)kNan;
+        if (r0 + part * 32 + b * BLOCK >= J.rows) word = 0u;
 #pragma unroll
-        for (int i = 0; i < BLOCK; ++i) v[h][b * BLOCK + i] = divide<E8M0>(v[h][b * BLOCK + i] * m, step, inv);
+        for (int i = 0; i < BLOCK; ++i) v[h][b * BLOCK + i] = divide<E8M0, HOW>(v[h][b * BLOCK + i], m, step, inv);
 #pragma unroll
         for (int i = 0; i < BLOCK / 8; ++i)
           out[b * (BLOCK / 8) + i] = finite ? e2m1x8(&v[h][b * BLOCK + 8 * i]) : 0u;
-        steps[(lane * 2 + h) * (kColTileR / 16) + warp * (32 / BLOCK) + b] = (uint8_t)word;
+        col_steps[step_at(pair * 2 + h, part * (32 / BLOCK) + b)] = (uint8_t)word;
       }
-      *reinterpret_cast<uint4*>(codes + (lane * 2 + h) * kColPitch + warp * 16) =
-          make_uint4(out[0], out[1], out[2], out[3]);
+      *reinterpret_cast<uint4*>(codes + (pair * 2 + h) * kColPitch + part * 16) = make_uint4(out[0], out[1], out[2], out[3]);
     }
-    __syncthreads();
-    // 64 output rows of 8 vectors of 16 bytes
+  }
+  __syncthreads();
+  constexpr int kGroups = kTile / (4 * BLOCK);  // scale tiles of the tile per axis
+  if (J.row_data != nullptr && t < kGroups * 32) {
+    // a line of 16 bytes: rows r, r + 32, r + 64, r + 96 of the tile; lines of
+    // rows that do not exist belong to the padding of the last scale tile
+    const uint32_t group = (uint32_t)(c0 / (4 * BLOCK)) + t / 32;
+    if (group < J.row_groups)
+      *reinterpret_cast<uint4*>(J.row_scales + ((r0 >> 7) * J.row_groups + group) * 512u + (t & 31) * 16) =
+          *reinterpret_cast<const uint4*>(row_steps + t * 16);
+  }
+  if (J.col_data != nullptr) {
+    const uint64_t padded = (J.rows + 31) / 32 * 32;
 #pragma unroll
-    for (int i = threadIdx.x; i < kColTileC * (kColTileR / 32); i += kThreads) {
-      const int col = i / (kColTileR / 32), part = i % (kColTileR / 32);
-      if (c0 + col < cols && r0 + part * 32 < padded)
-        *reinterpret_cast<uint4*>(data + (int64_t)(c0 + col) * data_stride + (int64_t)(r0 / 2) + part * 16) =
+    for (int i = 0; i < kTile * 4 / kThreads; ++i) {
+      const int item = i * kThreads + t, col = item >> 2, part = item & 3;
+      if (c0 + col < J.cols && r0 + part * 32 < padded)
+        *reinterpret_cast<uint4*>(J.col_data + (int64_t)(c0 + col) * J.col_stride + (int64_t)(r0 / 2) + part * 16) =
             *reinterpret_cast<const uint4*>(codes + col * kColPitch + part * 16);
     }
-    // one word of four scales per column and group
-    for (int i = threadIdx.x; i < kColTileC * (kSteps / 4); i += kThreads) {
-      const int col = i % kColTileC, g = i / kColTileC;
-      const uint32_t group = (uint32_t)(r0 / (4 * BLOCK)) + g;
-      if (c0 + col < cols && group < groups)
-        *reinterpret_cast<uint32_t*>(scales + scale_offset(c0 + col, group * 4, groups)) =
-            *reinterpret_cast<const uint32_t*>(steps + col * (kColTileR / 16) + g * 4);
+    if (t >= kThreads - kGroups * 32) {
+      const int i = t - (kThreads - kGroups * 32);
+      const uint32_t group = (uint32_t)(r0 / (4 * BLOCK)) + i / 32;
+      if (group < J.col_groups)
+        *reinterpret_cast<uint4*>(J.col_scales + ((c0 >> 7) * J.col_groups + group) * 512u + (i & 31) * 16) =
+            *reinterpret_cast<const uint4*>(col_steps + i * 16);
     }
-    __syncthreads();
   }
+}
+
+template <int TYPE, bool E8M0, int BLOCK>
+__global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const __grid_constant__ Jobs jobs, bool ceil) {
+  using B = TileBytes<TYPE>;
+  using T = typename Real<TYPE>::type;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint32_t shared[kThreads / 32];
+  const Job& J = job_of(jobs);
+  let_next_grid_start();
+  wait_for_previous_grid();
+  const uint64_t tile = blockIdx.x - J.first_block, across = (J.cols + kTile - 1) / kTile;
+  const uint64_t r0 = tile / across * kTile, c0 = tile % across * kTile;
+  const T* src = static_cast<const T*>(J.x) + (int64_t)r0 * J.stride + (int64_t)c0;
+  if (J.vec) {
+    constexpr int kPer = 16 / Real<TYPE>::kBytes, kVecs = kTile / kPer;  // elements of a vector, vectors of a row
+#pragma unroll
+    for (int i = 0; i < kTile * kVecs / kThreads; ++i) {
+      const int item = i * kThreads + threadIdx.x, r = item / kVecs, v = item % kVecs;
+      // bytes of the vector that exist; the others become zeros
+      const int64_t have = r0 + r < J.rows ? (int64_t)(J.cols - c0) - v * kPer : 0;
+      const uint32_t bytes = have >= kPer ? 16u : (have > 0 ? (uint32_t)have * Real<TYPE>::kBytes : 0u);
+      const T* from = bytes ? src + (int64_t)r * J.stride + v * kPer : static_cast<const T*>(J.x);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                   :: "r"((uint32_t)__cvta_generic_to_shared(smem + r * B::kPitch + v * 16)), "l"(from), "r"(bytes) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  } else {
+#pragma unroll 16
+    for (int i = 0; i < kTile * kTile / kThreads; ++i) {
+      const int item = i * kThreads + threadIdx.x, r = item / kTile, c = item % kTile;
+      reinterpret_cast<T*>(smem + r * B::kPitch)[c] =
+          r0 + r < J.rows && c0 + c < J.cols ? src[(int64_t)r * J.stride + c] : from_f32<TYPE>(0.f);
+    }
+  }
+  const float m = load_multiplier(J, shared);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  if (is_narrow<TYPE, E8M0>(m)) round_tile<TYPE, E8M0, BLOCK, kNarrow>(J, smem, r0, c0, ceil, m);
+  else round_tile<TYPE, E8M0, BLOCK, kExact>(J, smem, r0, c0, ceil, m);
 }
 
 // ---- back to real values -------------------------------------------------------
 
-template <int TYPE, bool E8M0, int BLOCK, bool VEC>
+template <int TYPE, bool E8M0, int BLOCK>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_stride,
                                                               const uint8_t* __restrict__ scales, uint32_t groups,
-                                                              uint32_t rows, uint64_t row0, uint32_t k,
+                                                              uint32_t rows, uint64_t row0, uint32_t k, Divider chunks,
                                                               const float* multiplier, void* __restrict__ out,
-                                                              int64_t out_stride) {
+                                                              int64_t out_stride, bool vec) {
   let_next_grid_start();
   wait_for_previous_grid();
   const float back = multiplier != nullptr ? 1.f / *multiplier : 1.f;
-  const uint32_t chunks = (k + 15u) / 16u;
-  const uint32_t total = rows * chunks;
+  const uint32_t total = rows * chunks.d;
   using T = typename Real<TYPE>::type;
   for (uint32_t item = blockIdx.x * kThreads + threadIdx.x; item < total; item += gridDim.x * kThreads) {
-    const uint32_t row = item / chunks, chunk = item - row * chunks, e0 = chunk * 16u;
+    const uint32_t row = divided(item, chunks), chunk = item - row * chunks.d, e0 = chunk * 16u;
     const uint2 w = __ldg(reinterpret_cast<const uint2*>(data + (int64_t)(row0 + row) * data_stride + chunk * 8u));
     const float s = scale_value<E8M0>(__ldg(scales + scale_offset(row0 + row, e0 / BLOCK, groups)));
     float v[16];
@@ -328,7 +457,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = v[j] * s * back;
     T* dst = static_cast<T*>(out) + (int64_t)(row0 + row) * out_stride + e0;
-    if (VEC && e0 + 16u <= k) {
+    if (vec && e0 + 16u <= k) {
       if constexpr (TYPE == T5E_REAL_F32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -362,16 +491,13 @@ int launched(cudaError_t err, const char* what) {
   return kernel_status(what);
 }
 
-// Calls f with compile-time (type, UE8M0, block, vector) for a run-time choice.
+// Calls f with compile-time (type, UE8M0, block) for a run-time choice.
 template <typename F>
-int with_form(int32_t type, const t5e_blocks& b, bool vec, F f) {
-  auto by_vec = [&](auto t, auto e8, auto blk) {
-    return vec ? f(t, e8, blk, std::true_type{}) : f(t, e8, blk, std::false_type{});
-  };
+int with_form(int32_t type, int32_t scale_format, int32_t scale_block, F f) {
   auto by_scale = [&](auto t) {
-    if (b.scale_format == T5E_SCALE_UE4M3) return by_vec(t, std::false_type{}, std::integral_constant<int, 16>{});
-    if (b.scale_block == 16) return by_vec(t, std::true_type{}, std::integral_constant<int, 16>{});
-    return by_vec(t, std::true_type{}, std::integral_constant<int, 32>{});
+    if (scale_format == T5E_SCALE_UE4M3) return f(t, std::false_type{}, std::integral_constant<int, 16>{});
+    if (scale_block == 16) return f(t, std::true_type{}, std::integral_constant<int, 16>{});
+    return f(t, std::true_type{}, std::integral_constant<int, 32>{});
   };
   if (type == T5E_REAL_F32) return by_scale(std::integral_constant<int, T5E_REAL_F32>{});
   if (type == T5E_REAL_BF16) return by_scale(std::integral_constant<int, T5E_REAL_BF16>{});
@@ -386,21 +512,28 @@ unsigned grid_of(uint64_t blocks, unsigned per_sm) {
 // Rows of one launch: the kernels count chunks of a launch in 32 bits.
 uint64_t rows_per_launch(uint64_t chunks) { return chunks ? (uint64_t(1) << 30) / chunks : 1; }
 
-int quantize_rows(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, bool ceil, float* multiplier,
-                  const uint32_t* partials, int count, const t5e_blocks& out, cudaStream_t stream) {
-  const uint32_t groups = scale_groups(out);
-  const uint64_t chunks = (uint64_t)groups * (out.scale_block / 4);
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows == 1 || (stride * type_bytes(type)) % 16 == 0);
-  const uint64_t per = rows_per_launch(chunks);
-  for (uint64_t row0 = 0; row0 < rows; row0 += per) {
-    const uint32_t n = (uint32_t)(rows - row0 < per ? rows - row0 : per);
-    const unsigned grid = grid_of(((uint64_t)n * chunks + kThreads - 1) / kThreads, 8);
-    const int rc = with_form(type, out, vec, [&](auto t, auto e8, auto blk, auto v) {
-      return launched(launch_dependent(quantize_rows_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value,
-                                                            decltype(v)::value>,
-                                       grid, kThreads, 0, stream, x, n, row0, (uint32_t)cols, stride, ceil, multiplier,
-                                       partials, count, static_cast<uint8_t*>(out.data), out.stride,
-                                       static_cast<uint8_t*>(out.scales), groups),
+bool rows_aligned(int32_t type, const void* x, uint64_t rows, int64_t stride) {
+  return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows <= 1 || (stride * type_bytes(type)) % 16 == 0);
+}
+
+Divider divider(uint32_t d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return {d, d == 1u ? 0u : (uint32_t)((1ull << (31 + shift)) / d + 1), shift};
+}
+
+constexpr uint32_t kNever = 0xFFFFFFFFu;
+
+int quantize_rows(int32_t type, const Jobs& jobs, const t5e_blocks& out, bool ceil, cudaStream_t stream) {
+  const Job& J = jobs.job[0];
+  const Divider chunks = divider(J.row_groups * (uint32_t)(out.scale_block / 4));
+  const uint64_t per = rows_per_launch(chunks.d);
+  for (uint64_t row0 = 0; row0 < J.rows; row0 += per) {
+    const uint32_t n = (uint32_t)(J.rows - row0 < per ? J.rows - row0 : per);
+    const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 8);
+    const int rc = with_form(type, out.scale_format, out.scale_block, [&](auto t, auto e8, auto blk) {
+      return launched(launch_dependent(quantize_rows_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value>,
+                                       dim3(grid), kThreads, 0, stream, jobs, n, row0, chunks, ceil),
                       "quantize_rows_kernel launch");
     });
     if (rc != T5E_OK) return rc;
@@ -408,19 +541,22 @@ int quantize_rows(int32_t type, const void* x, uint64_t rows, uint64_t cols, int
   return T5E_OK;
 }
 
-int quantize_cols(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, bool ceil, float* multiplier,
-                  const uint32_t* partials, int count, const t5e_blocks& out, cudaStream_t stream) {
-  const int bytes = type_bytes(type);
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & (2 * bytes - 1)) == 0 && (rows == 1 || stride % 2 == 0);
-  const uint64_t tiles = (rows + kColTileR - 1) / kColTileR;
-  dim3 grid((unsigned)((cols + kColTileC - 1) / kColTileC), (unsigned)(tiles < 65535 ? tiles : 65535));
-  return with_form(type, out, vec, [&](auto t, auto e8, auto blk, auto v) {
-    return launched(launch_dependent(quantize_cols_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value,
-                                                          decltype(v)::value>,
-                                     grid, kThreads, 0, stream, x, rows, cols, stride, ceil, multiplier, partials, count,
-                                     static_cast<uint8_t*>(out.data), out.stride, static_cast<uint8_t*>(out.scales),
-                                     scale_groups(out)),
-                    "quantize_cols_kernel launch");
+int quantize_tiles(int32_t type, Jobs& jobs, int n, int32_t scale_format, int32_t scale_block, bool ceil,
+                   cudaStream_t stream) {
+  uint64_t blocks = 0;
+  for (int i = 0; i < 2; ++i) {
+    jobs.job[i].first_block = i < n ? (uint32_t)blocks : kNever;
+    if (i < n)
+      blocks += ((jobs.job[i].rows + kTile - 1) / kTile) * ((jobs.job[i].cols + kTile - 1) / kTile);
+    if (blocks > 0x7FFFFFFFull) return T5E_ERR_INVALID;
+  }
+  return with_form(type, scale_format, scale_block, [&](auto t, auto e8, auto blk) {
+    constexpr auto kernel = quantize_tiles_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value>;
+    constexpr int smem = TileBytes<decltype(t)::value>::kAll;
+    const int rc = raise_smem_limit<kernel>(smem, "quantize_tiles_kernel attribute");
+    if (rc != T5E_OK) return rc;
+    return launched(launch_dependent(kernel, dim3((unsigned)blocks), kThreads, smem, stream, jobs, ceil),
+                    "quantize_tiles_kernel launch");
   });
 }
 
@@ -429,23 +565,33 @@ bool matrix_ok(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_
   return x && (reinterpret_cast<uintptr_t>(x) & (type_bytes(type) - 1)) == 0 && (rows == 1 || stride >= (int64_t)cols);
 }
 
-int partial_maxima(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, uint32_t* partials,
-                   int32_t count, cudaStream_t stream) {
-  if (rows == 0 || cols == 0) rows = cols = 0;
-  if (rows > 1 && stride == (int64_t)cols) {
-    cols *= rows;
-    rows = 1;
+// The partial maxima of the jobs that want them.
+int partial_maxima(int32_t type, const Jobs& jobs, int n, cudaStream_t stream) {
+  Jobs work = {};
+  int wanted = 0;
+  uint32_t blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    if (jobs.job[i].partials == nullptr) continue;
+    Job& J = work.job[wanted++];
+    J = jobs.job[i];
+    J.first_block = blocks;
+    blocks += (uint32_t)J.count;
+    if (J.rows == 0 || J.cols == 0) J.rows = J.cols = 0;
+    if (J.rows > 1 && J.stride == (int64_t)J.cols) {
+      J.cols *= J.rows;
+      J.rows = 1;
+    }
+    J.vec = rows_aligned(type, J.x, J.rows, J.stride);
   }
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows <= 1 || (stride * type_bytes(type)) % 16 == 0);
-  auto go = [&](auto t, auto v) {
-    return launched(launch_dependent(partials_kernel<decltype(t)::value, decltype(v)::value>, dim3((unsigned)count),
-                                     kThreads, 0, stream, x, rows, cols, stride, partials),
+  if (wanted == 0) return T5E_OK;
+  if (wanted == 1) work.job[1].first_block = kNever;
+  auto go = [&](auto t) {
+    return launched(launch_dependent(partials_kernel<decltype(t)::value>, dim3(blocks), kThreads, 0, stream, work),
                     "partials_kernel launch");
   };
-  auto by_vec = [&](auto t) { return vec ? go(t, std::true_type{}) : go(t, std::false_type{}); };
-  if (type == T5E_REAL_F32) return by_vec(std::integral_constant<int, T5E_REAL_F32>{});
-  if (type == T5E_REAL_BF16) return by_vec(std::integral_constant<int, T5E_REAL_BF16>{});
-  return by_vec(std::integral_constant<int, T5E_REAL_F16>{});
+  if (type == T5E_REAL_F32) return go(std::integral_constant<int, T5E_REAL_F32>{});
+  if (type == T5E_REAL_BF16) return go(std::integral_constant<int, T5E_REAL_BF16>{});
+  return go(std::integral_constant<int, T5E_REAL_F16>{});
 }
 
 }  // namespace blocks
@@ -489,43 +635,88 @@ int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t co
       !matrix_ok(type, x, rows, cols, stride))
     return T5E_ERR_INVALID;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rc = partial_maxima(type, x, rows, cols, stride, partials, count, s);
+  Jobs jobs = {};
+  Job& J = jobs.job[0];
+  J.x = x;
+  J.rows = rows;
+  J.cols = cols;
+  J.stride = stride;
+  J.partials = partials;
+  J.count = count;
+  J.vec = rows_aligned(type, x, rows, stride);
+  const int rc = partial_maxima(type, jobs, 1, s);
   if (rc != T5E_OK) return rc;
   return launched(launch_dependent(multiplier_kernel, dim3(1), kThreads, 0, s, partials, count, multiplier),
                   "multiplier_kernel launch");
 }
 
-int t5e_quantize_blocks(int32_t type, const void* x, uint64_t rows, uint64_t cols, int64_t stride, int32_t rounding,
-                        float* multiplier, uint32_t* partials, int32_t count, const t5e_blocks* by_rows,
-                        const t5e_blocks* by_cols, void* stream) {
+int t5e_quantize_blocks(const t5e_quantize* q, int32_t n, void* stream) {
   using namespace t5e;
   using namespace t5e::blocks;
-  if (!type_ok(type) || (!by_rows && !by_cols)) return T5E_ERR_INVALID;
-  if (partials && (!multiplier || count < 1 || count > T5E_MAX_PARTIALS)) return T5E_ERR_INVALID;
-  if (by_rows && (!blocks_ok(by_rows) || by_rows->rows != rows || (uint64_t)by_rows->k != cols)) return T5E_ERR_INVALID;
-  if (by_cols && (!blocks_ok(by_cols) || by_cols->rows != cols || (uint64_t)by_cols->k != rows)) return T5E_ERR_INVALID;
-  if (by_rows && by_cols &&
-      (by_rows->scale_format != by_cols->scale_format || by_rows->scale_block != by_cols->scale_block))
-    return T5E_ERR_INVALID;
-  const int32_t format = (by_rows ? by_rows : by_cols)->scale_format;
-  if (format == T5E_SCALE_UE4M3 ? rounding != T5E_SCALE_ROUND_NEAREST
-                                : rounding != T5E_SCALE_ROUND_FLOOR && rounding != T5E_SCALE_ROUND_CEIL)
-    return T5E_ERR_INVALID;
-  if (!matrix_ok(type, x, rows, cols, stride)) return T5E_ERR_INVALID;
+  if (!q || n < 1 || n > 2) return T5E_ERR_INVALID;
+  Jobs jobs = {};
+  const t5e_blocks* form = nullptr;
+  bool cols = false, empty = true;
+  for (int i = 0; i < n; ++i) {
+    const t5e_quantize& Q = q[i];
+    const bool by_rows = Q.by_rows.data != nullptr, by_cols = Q.by_cols.data != nullptr;
+    if (!type_ok(Q.type) || Q.type != q[0].type || Q.rounding != q[0].rounding || Q.reserved != 0) return T5E_ERR_INVALID;
+    if (Q.partials && (!Q.multiplier || Q.count < 1 || Q.count > T5E_MAX_PARTIALS)) return T5E_ERR_INVALID;
+    if (!matrix_ok(Q.type, Q.x, Q.rows, Q.cols, Q.stride)) return T5E_ERR_INVALID;
+    if (!by_rows && !by_cols) {
+      if (Q.rows && Q.cols) return T5E_ERR_INVALID;
+      continue;  // no element: nothing to write
+    }
+    for (const t5e_blocks* b : {by_rows ? &Q.by_rows : nullptr, by_cols ? &Q.by_cols : nullptr}) {
+      if (!b) continue;
+      if (!form) form = b;
+      const bool mine = b == &Q.by_rows;
+      if (!blocks_ok(b) || b->rows != (mine ? Q.rows : Q.cols) || (uint64_t)b->k != (mine ? Q.cols : Q.rows) ||
+          b->scale_format != form->scale_format || b->scale_block != form->scale_block)
+        return T5E_ERR_INVALID;
+    }
+    if (Q.rows == 0 || Q.cols == 0) continue;
+    empty = false;
+    cols |= by_cols;
+    Job& J = jobs.job[i];
+    J.x = Q.x;
+    J.rows = Q.rows;
+    J.cols = Q.cols;
+    J.stride = Q.stride;
+    J.multiplier = Q.multiplier;
+    J.partials = Q.partials;
+    J.count = Q.count;
+    J.vec = rows_aligned(Q.type, Q.x, Q.rows, Q.stride);
+    if (by_rows) {
+      J.row_data = static_cast<uint8_t*>(Q.by_rows.data);
+      J.row_stride = Q.by_rows.stride;
+      J.row_scales = static_cast<uint8_t*>(Q.by_rows.scales);
+      J.row_groups = scale_groups(Q.by_rows);
+    }
+    if (by_cols) {
+      J.col_data = static_cast<uint8_t*>(Q.by_cols.data);
+      J.col_stride = Q.by_cols.stride;
+      J.col_scales = static_cast<uint8_t*>(Q.by_cols.scales);
+      J.col_groups = scale_groups(Q.by_cols);
+    }
+  }
+  if (form) {
+    const bool nearest = q[0].rounding == T5E_SCALE_ROUND_NEAREST;
+    const bool power = q[0].rounding == T5E_SCALE_ROUND_FLOOR || q[0].rounding == T5E_SCALE_ROUND_CEIL;
+    if (form->scale_format == T5E_SCALE_UE4M3 ? !nearest : !power) return T5E_ERR_INVALID;
+  }
+  if (empty) return T5E_OK;
+  if (n == 2 && (jobs.job[0].x == nullptr || jobs.job[1].x == nullptr)) {  // one of the two is empty
+    if (jobs.job[0].x == nullptr) jobs.job[0] = jobs.job[1];
+    n = 1;
+  }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool ceil = rounding == T5E_SCALE_ROUND_CEIL;
-  if (rows == 0 || cols == 0)
-    return partials ? t5e_block_multiplier(type, x, rows, cols, stride, partials, count, multiplier, stream) : T5E_OK;
-  if (partials) {
-    const int rc = partial_maxima(type, x, rows, cols, stride, partials, count, s);
-    if (rc != T5E_OK) return rc;
-  }
-  if (by_rows) {
-    const int rc = quantize_rows(type, x, rows, cols, stride, ceil, multiplier, partials, count, *by_rows, s);
-    if (rc != T5E_OK) return rc;
-  }
-  if (by_cols) return quantize_cols(type, x, rows, cols, stride, ceil, multiplier, partials, count, *by_cols, s);
-  return T5E_OK;
+  const bool ceil = q[0].rounding == T5E_SCALE_ROUND_CEIL;
+  int rc = partial_maxima(q[0].type, jobs, n, s);
+  if (rc != T5E_OK) return rc;
+  // one tensor's rows alone need no tile in shared memory
+  if (n == 1 && !cols) return quantize_rows(q[0].type, jobs, *form, ceil, s);
+  return quantize_tiles(q[0].type, jobs, n, form->scale_format, form->scale_block, ceil, s);
 }
 
 int t5e_dequantize_blocks(const t5e_blocks* b, const float* multiplier, int32_t type, void* out, int64_t out_stride,
@@ -537,20 +728,18 @@ int t5e_dequantize_blocks(const t5e_blocks* b, const float* multiplier, int32_t 
   if (!out || (reinterpret_cast<uintptr_t>(out) & (type_bytes(type) - 1)) || (b->rows > 1 && out_stride < b->k))
     return T5E_ERR_INVALID;
   const uint32_t groups = scale_groups(*b);
-  const uint64_t chunks = ((uint64_t)b->k + 15) / 16;
-  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 &&
-                   (b->rows == 1 || (out_stride * type_bytes(type)) % 16 == 0);
-  const uint64_t per = rows_per_launch(chunks);
+  const Divider chunks = divider((uint32_t)(((uint64_t)b->k + 15) / 16));
+  const bool vec = rows_aligned(type, out, b->rows, out_stride);
+  const uint64_t per = rows_per_launch(chunks.d);
   for (uint64_t row0 = 0; row0 < b->rows; row0 += per) {
     const uint32_t n = (uint32_t)(b->rows - row0 < per ? b->rows - row0 : per);
-    const unsigned grid = grid_of(((uint64_t)n * chunks + kThreads - 1) / kThreads, 8);
-    const int rc = with_form(type, *b, vec, [&](auto t, auto e8, auto blk, auto v) {
-      return launched(launch_dependent(dequantize_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value,
-                                                         decltype(v)::value>,
+    const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 8);
+    const int rc = with_form(type, b->scale_format, b->scale_block, [&](auto t, auto e8, auto blk) {
+      return launched(launch_dependent(dequantize_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value>,
                                        dim3(grid), kThreads, 0, static_cast<cudaStream_t>(stream),
                                        static_cast<const uint8_t*>(b->data), b->stride,
-                                       static_cast<const uint8_t*>(b->scales), groups, n, row0, (uint32_t)b->k,
-                                       multiplier, out, out_stride),
+                                       static_cast<const uint8_t*>(b->scales), groups, n, row0, (uint32_t)b->k, chunks,
+                                       multiplier, out, out_stride, vec),
                       "dequantize_kernel launch");
     });
     if (rc != T5E_OK) return rc;

@@ -75,58 +75,79 @@ __device__ __forceinline__ uint64_t scale_offset(uint64_t r, uint32_t b, uint32_
   return ((r >> 7) * groups + (b >> 2)) * 512u + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
 }
 
-// Scale of a block from the largest magnitude `a` of its (multiplied)
-// elements; returns the scale byte and the step that elements are divided by,
-// as its reciprocal-or-power in `inv` and its value in `step`.
-//   UE4M3: RNE of min(a / 6, 448).  a / 6 correctly rounded to F32 is a tie
+// How the elements of a tensor are multiplied and divided.
+//
+// General (kExact): u = F32(x * m), then u / step correctly rounded (Markstein's
+// correction of the product with the correctly rounded reciprocal).  A quotient
+// so rounded is an E2M1 tie only where the real one is: a tie times the step has
+// at most 7 significand bits, so an F32 neighbour of it stays off the tie.
+//
+// Narrow (kNarrow): x has at most 11 significand bits and m is a power of two,
+// so u is exact and, where it is not a tie itself, at least 2^-12 away from one:
+// one product, truncated, with the nearest reciprocal is enough.  For the eight
+// significands of a UE4M3 step that reciprocal is never below the real one and
+// above it by less than 2^-24 of its value, so at a tie the product exceeds the
+// tie by less than a unit in its last place and truncates to it.  m is part of
+// the reciprocal; this holds m to 2^+-60.  With UE8M0 steps, whose products are
+// exact, narrow means m = 1, for any type.
+enum { kExact = 0, kNarrow = 1 };
+
+template <int TYPE, bool E8M0>
+__device__ __forceinline__ bool is_narrow(float m) {
+  if constexpr (E8M0) return m == 1.f;
+  const uint32_t b = __float_as_uint(m);
+  return TYPE != T5E_REAL_F32 && (b & 0x007FFFFFu) == 0u && b >= (67u << 23) && b <= (187u << 23);
+}
+
+// Scale of a block from the largest magnitude `a` of its elements before the
+// multiplier; returns the scale byte, and what divide() needs.
+//   UE4M3: RNE of min(am / 6, 448).  am / 6 correctly rounded to F32 is a tie
 //          of the 4-bit rounding only where the real quotient is (6 t has at
-//          most 7 significand bits), so the second rounding is exact.
-//   UE8M0: 2^(floor(log2 a) - 2), or with `ceil` the smallest 2^e >= a / 6.
-// A block with a NaN or an infinity gets the NaN scale and a zero step.
-template <bool E8M0>
-__device__ __forceinline__ uint32_t block_scale(float a, bool ceil, float& step, float& inv) {
-  const uint32_t bits = __float_as_uint(a);
+//          most 7 significand bits); narrow values need only the product with
+//          F32(1/6), which returns t exactly for every am = 6 t.
+//   UE8M0: 2^(floor(log2 am) - 2), or with `ceil` the smallest 2^e >= am / 6.
+// Rounding to F32 is monotonic, so am = F32(a * m) is the largest |u|.  A block
+// with a NaN or an infinity (or a product beyond F32) gets the NaN scale and a
+// zero step.
+template <bool E8M0, int HOW>
+__device__ __forceinline__ uint32_t block_scale(float a, float m, bool ceil, float& step, float& inv) {
+  const float am = a * m;
+  const uint32_t bits = __float_as_uint(am);
   if constexpr (E8M0) {
-    // word = floor(log2 a) - 2 + 127: the F32 exponent field less 2; F32
+    // word = floor(log2 am) - 2 + 127: the F32 exponent field less 2; F32
     // subnormals have field 0 and clamp to word 0 (2^-127), as zero does
-    const int field = (int)(bits >> 23);
-    int w = field - 2;
-    if (ceil && (bits & 0x7FFFFFu) > 0x400000u) w += 1;  // a > 1.5 * 2^floor(log2 a) = 6 * 2^(floor(log2 a) - 2)
+    int w = (int)(bits >> 23) - 2;
+    if (ceil && (bits & 0x7FFFFFu) > 0x400000u) w += 1;  // am > 1.5 * 2^floor(log2 am) = 6 * 2^(floor(log2 am) - 2)
     w = w < 0 ? 0 : w;
-    if (bits >= 0x7F800000u) {
-      step = inv = 0.f;
-      return 0xFFu;
-    }
-    // 2^(127 - w) without leaving F32: w = 0 gives 2^127, w = 254 the
-    // subnormal 2^-127, both exact
-    inv = w == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - w) << 23);
+    const bool finite = bits < 0x7F800000u;
+    // 2^(127 - w) without leaving F32: w = 0 gives 2^127 (w is at most 253)
+    inv = finite ? __uint_as_float((uint32_t)(254 - w) << 23) : 0.f;
     step = 0.f;  // unused: products with inv are exact wherever they reach the E2M1 range
-    return (uint32_t)w;
+    return finite ? (uint32_t)w : 0xFFu;
   } else {
-    if (bits >= 0x7F800000u) {
-      step = inv = 0.f;
-      return 0x7Fu;
-    }
-    const float want = __fdiv_rn(a, 6.f);
+    const bool finite = bits < 0x7F800000u;
+    const float want = HOW == kNarrow ? am * (1.f / 6.f) : __fdiv_rn(am, 6.f);
     uint16_t two;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(want));
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(two));
     step = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
-    inv = step > 0.f ? __frcp_rn(step) : 0.f;
-    return two & 0x7Fu;
+    inv = finite && step > 0.f ? __frcp_rn(step) : 0.f;
+    if constexpr (HOW == kNarrow) inv *= m;
+    return finite ? (uint32_t)(two & 0x7Fu) : 0x7Fu;
   }
 }
 
-// u / step correctly rounded to F32 (Markstein's correction of the product
-// with the correctly rounded reciprocal), for UE4M3 steps.  A quotient so
-// rounded is an E2M1 tie only where the real one is: step has 4 significand
-// bits and a tie 3, so a neighbour of a tie stays one after rounding.
-template <bool E8M0>
-__device__ __forceinline__ float divide(float u, float step, float inv) {
-  const float y = __fmul_rn(u, inv);
-  if constexpr (E8M0) return y;
-  else return __fmaf_rn(-__fmaf_rn(y, step, -u), inv, y);  // this order of signs keeps a negative zero
+template <bool E8M0, int HOW>
+__device__ __forceinline__ float divide(float x, float m, float step, float inv) {
+  if constexpr (E8M0) {
+    return HOW == kNarrow ? x * inv : x * m * inv;
+  } else if constexpr (HOW == kNarrow) {
+    return __fmul_rz(x, inv);
+  } else {
+    const float u = x * m, y = __fmul_rn(u, inv);
+    return __fmaf_rn(-__fmaf_rn(y, step, -u), inv, y);  // this order of signs keeps a negative zero
+  }
 }
 
 // Two values to two E2M1 codes (RNE, magnitudes above 6 become 6): `lo` in

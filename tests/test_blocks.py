@@ -191,22 +191,27 @@ def test_c_entry_points_refuse_bad_arguments():
     bad = [dict(k=0), dict(k=nat.MAX_BLOCK_K + 1), dict(stride=48), dict(stride=72), dict(data=4104), dict(scales=4100),
            dict(scale_block=32), dict(scale_format=0), dict(data=None), dict(scales=None),
            dict(rows=nat.MAX_BLOCK_ROWS + 1)]
+    none = nat.Blocks()
+
+    def quantize(n=1, **kw):
+        q = nat.Quantize(4096, 8, 128, 128, 0, 0, None, None, 0, 0, blk(), none)
+        for name, v in kw.items():
+            setattr(q, name, v)
+        return lib.t5e_quantize_blocks((nat.Quantize * 2)(q, q), n, None)
+
     for kw in bad:
         b = blk(**kw)
         assert lib.t5e_dequantize_blocks(ctypes.byref(b), None, 0, 4096, 128, None) == nat.ERR_INVALID
-        assert lib.t5e_quantize_blocks(0, 4096, b.rows, max(b.k, 0), 128, 0, None, None, 0, ctypes.byref(b), None,
-                                       None) == nat.ERR_INVALID
+        assert quantize(rows=b.rows, cols=max(b.k, 0), by_rows=b) == nat.ERR_INVALID
         mm = nat.BlockMm(ctypes.pointer(b), ctypes.pointer(blk()), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(mm), None) == nat.ERR_INVALID
     good = blk()
-    q = ctypes.byref(good)
-    assert lib.t5e_quantize_blocks(3, 4096, 8, 128, 128, 0, None, None, 0, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 128, 1, None, None, 0, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 127, 0, None, None, 0, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4098, 8, 128, 128, 0, None, None, 0, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 128, 0, None, 4096, 4, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4096, 9, 128, 128, 0, None, None, 0, q, None, None) == nat.ERR_INVALID
-    assert lib.t5e_quantize_blocks(0, 4096, 8, 128, 128, 0, None, None, 0, None, None, None) == nat.ERR_INVALID
+    for kw in (dict(type=3), dict(rounding=1), dict(stride=127), dict(x=4098), dict(x=None), dict(partials=4096, count=4),
+               dict(partials=4096, multiplier=4096, count=0), dict(rows=9), dict(cols=127), dict(by_rows=none),
+               dict(by_cols=blk()), dict(reserved=1), dict(n=0), dict(n=3),
+               dict(by_cols=nat.Blocks(4096, 16, 4096, 128, 8, nat.SCALE_UE8M0, 16))):
+        assert quantize(**kw) == nat.ERR_INVALID, kw
+    assert lib.t5e_quantize_blocks(None, 1, None) == nat.ERR_INVALID
     for partials, count, out in ((4096, 0, 4096), (4096, nat.MAX_PARTIALS + 1, 4096), (None, 4, 4096), (4096, 4, None)):
         assert lib.t5e_block_multiplier(0, 4096, 8, 128, 128, partials, count, out, None) == nat.ERR_INVALID
 
@@ -230,6 +235,8 @@ def test_empty_calls_launch_nothing():
     none = nat.Blocks(None, 64, None, 0, 128, nat.SCALE_UE4M3, 16)
     some = nat.Blocks(4096, 64, 4096, 8, 128, nat.SCALE_UE4M3, 16)
     assert lib.t5e_dequantize_blocks(ctypes.byref(none), None, 0, None, 128, None) == nat.OK
+    q = nat.Quantize(None, 0, 128, 128, 0, 0, None, None, 0, 0, nat.Blocks(), nat.Blocks())
+    assert lib.t5e_quantize_blocks(ctypes.byref(q), 1, None) == nat.OK
     for a, b in ((none, some), (some, none)):
         m = nat.BlockMm(ctypes.pointer(a), ctypes.pointer(b), None, None, 1.0, 0, None, 0, 0, 0, 0, None, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(m), None) == nat.OK
@@ -270,10 +277,17 @@ def test_rows_and_columns_round_as_defined(form, dtype, rows, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
-def test_every_tie_and_its_neighbours(form):
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_every_tie_and_its_neighbours(form, dtype):
     """Blocks whose largest value sets each scale significand, with elements at
-    each rounding border of E2M1 times the scale, and the F32 values next to
-    it on either side."""
+    each rounding border of E2M1 times the scale, and the type's values next to
+    it on either side; also with multipliers that shift the whole block."""
+    def beside(t, side):
+        if side is None:
+            return np.asarray(t, dtype=np.float64)
+        v = torch.nextafter(torch.as_tensor(t).to(dtype), torch.tensor(side, dtype=dtype))
+        return v.double().numpy()
+
     blocks, block = [], BLOCK[form]
     for m in range(8, 16):
         for e in (-6, 0, 5):
@@ -286,12 +300,16 @@ def test_every_tie_and_its_neighbours(form):
                     blocks.append(np.concatenate([[6 * step], sign * t, np.zeros(block - 8)]))
     # borders of the scale's own rounding
     for a in (6 * 17 / 16, 6 * 19 / 16, 6 * 2.0 ** -10, 6 * 1.5 * 2.0 ** -9, 6 * 448.0, 6 * 464.0, 1e5):
-        for v in (np.float32(a), np.nextafter(np.float32(a), np.float32(np.inf)), np.nextafter(np.float32(a), np.float32(0))):
+        for v in (float(beside(a, None)), float(beside(a, np.inf)), float(beside(a, 0.0))):
             blocks.append(np.concatenate([[v, v / 3, -v / 7], np.zeros(block - 3)]))
-    x = torch.tensor(np.array(blocks), dtype=torch.float32, device="cuda")
-    codes, scale, _ = define(x, form)
-    check_rows(t5.quantize_blocks(x, scaling=form[0], scale_vec=form[1]), codes, scale)
-    check_rows(t5.quantize_blocks(x.t().contiguous(), axis=0, scaling=form[0], scale_vec=form[1]), codes, scale)
+    x = torch.tensor(np.array(blocks)).to(dtype).cuda()
+    for m in (1.0, 0.25, 2.0 ** 70, 1.5):
+        codes, scale, _ = define(x, form, m)
+        kw = dict(scaling=form[0], scale_vec=form[1], multiplier=None if m == 1 else m)
+        check_rows(t5.quantize_blocks(x, **kw), codes, scale)
+        check_rows(t5.quantize_blocks(x.t().contiguous(), axis=0, **kw), codes, scale)
+        rows, cols = t5.quantize_blocks(x.t(), axis="both", **kw)
+        check_rows(cols, codes, scale)
 
 
 @pytest.mark.gpu
