@@ -150,8 +150,8 @@ class BlockMm(ctypes.Structure):
     """t5e_block_mm: one product of block-scaled rows."""
 
     _fields_ = [
-        ("a", ctypes.POINTER(Blocks)),
-        ("b", ctypes.POINTER(Blocks)),
+        ("a", ctypes.c_void_p),  # addresses of Blocks
+        ("b", ctypes.c_void_p),
         ("multiplier_a", ctypes.c_void_p),
         ("multiplier_b", ctypes.c_void_p),
         ("alpha", ctypes.c_float),

@@ -430,7 +430,7 @@ def _mm(a, b, c, alpha, dtype, out, form):
             raise ValueError("c overlaps out without being out")
     lib = nat.load()
     mm = nat.BlockMm(
-        ctypes.pointer(a._struct), ctypes.pointer(b._struct), None if a.multiplier is None else a.multiplier.data_ptr(),
+        ctypes.addressof(a._struct), ctypes.addressof(b._struct), None if a.multiplier is None else a.multiplier.data_ptr(),
         None if b.multiplier is None else b.multiplier.data_ptr(), alpha, form, None, 0, _REAL[dtype], 0, 0,
         out.data_ptr(), out.stride(0) if given and shape[0] > 1 else shape[1])
     if c is not None:
@@ -485,7 +485,7 @@ def _quantize_job(x, form, at, partials, count, rows, cols):
 def _product(lib, a, b, ma, mb, shape, dtype, device, handle):
     """block_scaled_mm of t5e_blocks."""
     out = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
-    mm = nat.BlockMm(ctypes.pointer(a), ctypes.pointer(b), ma, mb, 1.0, 0, None, 0, _REAL[dtype], 0, 0, out.data_ptr(),
+    mm = nat.BlockMm(ctypes.addressof(a), ctypes.addressof(b), ma, mb, 1.0, 0, None, 0, _REAL[dtype], 0, 0, out.data_ptr(),
                      shape[1])
     nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
     return out
@@ -536,8 +536,13 @@ class _Linear(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        # grad mode is on here only under create_graph=True; the marked form
+        # then refuses a second derivative, and costs a few microseconds
+        return _marked_backward(ctx, g) if torch.is_grad_enabled() else _Linear._backward(ctx, g)
+
+    @staticmethod
+    def _backward(ctx, g):
         x_shape, (n, k) = ctx.shapes
         need_x, need_w = ctx.needs_input_grad[:2]
         form = ctx.form
@@ -573,6 +578,11 @@ class _Linear(torch.autograd.Function):
                 if need_w:
                     dw = _product(lib, gt, _placed(xt, base), mg, mx, (n, k), g.dtype, device, handle)
         return dx, dw, None, None, None, None, None
+
+
+@torch.autograd.function.once_differentiable
+def _marked_backward(ctx, g):
+    return _Linear._backward(ctx, g)
 
 
 def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None = None,

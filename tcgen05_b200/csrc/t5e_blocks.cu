@@ -32,15 +32,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* shared) {
   return shared[0];
 }
 
-template <int TYPE>
-__device__ __forceinline__ uint32_t word_max(uint32_t w) {
-  if constexpr (TYPE == T5E_REAL_F32) {
-    return w & 0x7FFFFFFFu;
-  } else {  // the two halves' magnitudes, both kept as 16-bit bit patterns
-    return w & 0x7FFF7FFFu;
-  }
-}
-
 // F32 bits of a 16-bit type's magnitude bits.
 template <int TYPE>
 __device__ __forceinline__ uint32_t magnitude_bits(uint32_t h) {
@@ -49,16 +40,28 @@ __device__ __forceinline__ uint32_t magnitude_bits(uint32_t h) {
   else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
 }
 
+// The larger magnitude: of F32 bits as integers (a NaN sorts above infinity);
+// of two 16-bit values at once with the instruction that takes magnitudes and
+// keeps a NaN.  The sign bits of the latter mean nothing.
 template <int TYPE>
-__device__ __forceinline__ uint32_t join_max(uint32_t a, uint32_t b) {
-  if constexpr (TYPE == T5E_REAL_F32) return max(a, b);
-  else return __vmaxu2(a, b);
+__device__ __forceinline__ uint32_t join_max(uint32_t best, uint32_t word) {
+  if constexpr (TYPE == T5E_REAL_F32) {
+    return max(best, word & 0x7FFFFFFFu);
+  } else {
+    uint32_t r;
+    if constexpr (TYPE == T5E_REAL_BF16)
+      asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(best), "r"(word));
+    else
+      asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(best), "r"(word));
+    return r;
+  }
 }
 
+// F32 bits of the largest of the two halves (or of the one F32).
 template <int TYPE>
 __device__ __forceinline__ uint32_t final_max(uint32_t v) {
   if constexpr (TYPE == T5E_REAL_F32) return v;
-  else return magnitude_bits<TYPE>(max(v & 0xFFFFu, v >> 16));
+  else return magnitude_bits<TYPE>(max(v & 0x7FFFu, (v >> 16) & 0x7FFFu));
 }
 
 template <int TYPE>
@@ -78,6 +81,8 @@ struct Job {
   int32_t count;
   uint32_t first_block;
   bool vec;            // rows start on 16-byte boundaries
+  bool wide;           // on 32-byte boundaries
+  bool words;          // on 4-byte boundaries
   uint8_t* row_data;   // NULL: no blocks along the rows
   int64_t row_stride;
   uint8_t* row_scales;
@@ -122,13 +127,11 @@ __global__ void __launch_bounds__(kThreads) partials_kernel(const __grid_constan
         for (int j = 0; j < 4; ++j) v[j] = __ldg(p + i + j * step);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          best = join_max<TYPE>(best, join_max<TYPE>(join_max<TYPE>(word_max<TYPE>(v[j].x), word_max<TYPE>(v[j].y)),
-                                                     join_max<TYPE>(word_max<TYPE>(v[j].z), word_max<TYPE>(v[j].w))));
+          best = join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(best, v[j].x), v[j].y), v[j].z), v[j].w);
       }
       for (; i < vecs; i += step) {
         const uint4 v = __ldg(p + i);
-        best = join_max<TYPE>(best, join_max<TYPE>(join_max<TYPE>(word_max<TYPE>(v.x), word_max<TYPE>(v.y)),
-                                                   join_max<TYPE>(word_max<TYPE>(v.z), word_max<TYPE>(v.w))));
+        best = join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(best, v.x), v.y), v.z), v.w);
       }
       done = vecs * kPer;
     }
@@ -178,54 +181,130 @@ __device__ __forceinline__ uint32_t divided(uint32_t n, const Divider& v) {
 // one whose other half its neighbour lane holds.  Per row the chunks run up
 // to a whole group of four scales, so that four (eight) neighbouring lanes
 // always hold one group and one of them stores its four scale bytes as a word.
-template <int TYPE, bool E8M0, int BLOCK, int HOW>
-__device__ __forceinline__ void round_rows(const Job& J, uint32_t rows, uint64_t row0, const Divider& chunks, bool ceil,
-                                           float m) {
-  constexpr uint32_t kLanes = BLOCK / 4;  // lanes of one group of four scales
+// The next elements are loaded before the present ones are worked on.  Where
+// rows do not start on 16-byte boundaries the lanes load neighbouring elements
+// and exchange them through shared memory.
+template <int TYPE>
+struct Chunk {
+  uint32_t row, e0;  // e0 = k: nothing
+  uint4 w[Real<TYPE>::kBytes];
+};
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load_chunk(const Job& J, uint64_t row0, uint32_t item, uint32_t total, const Divider& chunks,
+                                           Chunk<TYPE>& c) {
+  using T = typename Real<TYPE>::type;
   const uint32_t k = (uint32_t)J.cols;
-  const uint32_t stored = ((k + 31u) / 32u) * 2u;  // chunks with codes in `data`
-  const uint32_t total = rows * chunks.d;
-  const int lane = threadIdx.x & 31;
-  for (uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u); base < total; base += gridDim.x * kThreads) {
-    const uint32_t item = base + lane;
-    const bool in = item < total;
-    const uint32_t row = in ? divided(item, chunks) : 0u, chunk = in ? item - row * chunks.d : 0u;
-    const uint32_t e0 = chunk * 16u;
-    float v[16];
-    uint32_t top = 0u;
-    const char* src = static_cast<const char*>(J.x) + ((int64_t)(row0 + row) * J.stride + e0) * Real<TYPE>::kBytes;
-    if (J.vec && in && e0 + 16u <= k) {
-      constexpr int kVecs = Real<TYPE>::kBytes;  // 16-byte vectors of 16 elements
-      uint4 w[kVecs];
+  const bool in = item < total;
+  c.row = in ? divided(item, chunks) : 0u;
+  c.e0 = in ? (item - c.row * chunks.d) * 16u : 0x7FFFFFFFu;
+  const int64_t at = (int64_t)(row0 + c.row) * J.stride + c.e0;
+  if constexpr (VEC) {
+    constexpr int kVecs = Real<TYPE>::kBytes, kPer = 16 / Real<TYPE>::kBytes;
+    const T* src = static_cast<const T*>(J.x) + at;
+    if (c.e0 + 16u <= k) {
 #pragma unroll
-      for (int j = 0; j < kVecs; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(w);
+      for (int j = 0; j < kVecs; j += 2) load32(reinterpret_cast<const uint4*>(src) + j, J.wide, c.w[j], c.w[j + 1]);
+    } else {  // the end of a row, or behind it: what exists, then zeros
 #pragma unroll
-      for (int j = 0; j < kVecs * 4; ++j) {
-        top = join_max<TYPE>(top, word_max<TYPE>(words[j]));
-        if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(words[j]);
-        else unpack2<TYPE>(words[j], v[2 * j], v[2 * j + 1]);
-      }
-      top = final_max<TYPE>(top);
-    } else {
-      using T = typename Real<TYPE>::type;
+      for (int j = 0; j < kVecs; ++j) {
+        uint32_t words[4] = {0u, 0u, 0u, 0u};
+        if (c.e0 + j * kPer < k) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        v[j] = in && e0 + j < k ? to_f32(reinterpret_cast<const T*>(src)[j]) : 0.f;
-        top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+          for (int i = 0; i < kPer; ++i) {
+            if (c.e0 + j * kPer + i < k) {
+              if constexpr (TYPE == T5E_REAL_F32)
+                words[i] = reinterpret_cast<const uint32_t*>(src)[j * kPer + i];
+              else
+                words[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[j * kPer + i] << (16 * (i & 1));
+            }
+          }
+        }
+        c.w[j] = make_uint4(words[0], words[1], words[2], words[3]);
       }
     }
+  } else {
+    // element j of the exchange: the elements (lane & 15) of the chunks of lanes
+    // 2j and 2j + 1, packed here by pairs of j
+    const int lane = threadIdx.x & 31;
+    uint32_t* words = reinterpret_cast<uint32_t*>(c.w);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int from = 2 * j + (lane >> 4), element = lane & 15;
+      const int64_t place = __shfl_sync(0xFFFFFFFFu, at, from) + element;
+      const uint32_t first = __shfl_sync(0xFFFFFFFFu, c.e0, from);
+      const bool there = first + element < k;
+      if constexpr (TYPE == T5E_REAL_F32) {
+        words[j] = there ? static_cast<const uint32_t*>(J.x)[place] : 0u;
+      } else {
+        const uint32_t h = there ? (uint32_t)static_cast<const uint16_t*>(J.x)[place] : 0u;
+        words[j / 2] = (j & 1) ? words[j / 2] | (h << 16) : h;
+      }
+    }
+  }
+}
+
+// After a load by neighbours: each lane's own 16 elements, through the warp's
+// part of `turn` (32 lanes of kTurn bytes).
+template <int TYPE>
+struct Turn {
+  static constexpr int kBytes = 16 * Real<TYPE>::kBytes + 16;  // a lane's, 16 bytes apart: vectors meet no bank twice
+};
+template <int TYPE>
+__device__ __forceinline__ void turn_chunk(Chunk<TYPE>& c, uint8_t* turn) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(c.w);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    uint8_t* to = turn + (2 * j + (lane >> 4)) * Turn<TYPE>::kBytes + (lane & 15) * Real<TYPE>::kBytes;
+    if constexpr (TYPE == T5E_REAL_F32) *reinterpret_cast<uint32_t*>(to) = words[j];
+    else *reinterpret_cast<uint16_t*>(to) = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < Real<TYPE>::kBytes; ++j)
+    c.w[j] = *reinterpret_cast<const uint4*>(turn + lane * Turn<TYPE>::kBytes + j * 16);
+}
+
+template <int TYPE, bool E8M0, int BLOCK, int HOW, bool VEC>
+__device__ __forceinline__ void round_rows(const Job& J, uint32_t rows, uint64_t row0, const Divider& chunks, bool ceil,
+                                           float m, const float* inverses, uint8_t* turn) {
+  constexpr uint32_t kLanes = BLOCK / 4;  // lanes of one group of four scales
+  const uint32_t k = (uint32_t)J.cols;
+  const uint32_t stored = (k + 31u) / 32u * 32u;  // elements with codes in `data`
+  const uint32_t total = rows * chunks.d;
+  const int lane = threadIdx.x & 31;
+  uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u);
+  Chunk<TYPE> c;
+  if (base < total) load_chunk<TYPE, VEC>(J, row0, base + lane, total, chunks, c);
+  while (base < total) {
+    const uint32_t next = base + gridDim.x * kThreads;
+    if constexpr (!VEC) turn_chunk<TYPE>(c, turn + (threadIdx.x & ~31u) * Turn<TYPE>::kBytes);
+    const uint32_t row = c.row, e0 = c.e0;
+    const bool in = base + lane < total;
+    float v[16];
+    uint32_t top = 0u;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(c.w);
+#pragma unroll
+    for (int j = 0; j < Real<TYPE>::kBytes * 4; ++j) {
+      top = join_max<TYPE>(top, words[j]);
+      if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(words[j]);
+      else unpack2<TYPE>(words[j], v[2 * j], v[2 * j + 1]);
+    }
+    if (next < total) load_chunk<TYPE, VEC>(J, row0, next + lane, total, chunks, c);
+    top = final_max<TYPE>(top);
     if constexpr (BLOCK == 32) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     float step, inv;
-    uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, step, inv);
+    uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, inverses, step, inv);
     const bool finite = word != (E8M0 ? 0xFFu : 0x7Fu);
     if (e0 / BLOCK * BLOCK >= k) word = 0u;  // a scale behind the last block
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = divide<E8M0, HOW>(v[j], m, step, inv);
     uint2 codes = make_uint2(e2m1x8(v), e2m1x8(v + 8));
     if (!finite) codes = make_uint2(0u, 0u);
-    if (in && chunk < stored)
-      *reinterpret_cast<uint2*>(J.row_data + (int64_t)(row0 + row) * J.row_stride + chunk * 8u) = codes;
+    if (in && e0 < stored)
+      *reinterpret_cast<uint2*>(J.row_data + (int64_t)(row0 + row) * J.row_stride + e0 / 2u) = codes;
     // four scale bytes to one word
     if constexpr (BLOCK == 16) {
       word <<= 8 * (lane & 3);
@@ -238,19 +317,29 @@ __device__ __forceinline__ void round_rows(const Job& J, uint32_t rows, uint64_t
     }
     if (in && lane % kLanes == 0)
       *reinterpret_cast<uint32_t*>(J.row_scales + scale_offset(row0 + row, e0 / BLOCK, J.row_groups)) = word;
+    base = next;
   }
 }
 
-template <int TYPE, bool E8M0, int BLOCK>
+template <int TYPE, bool E8M0, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ Jobs jobs, uint32_t rows,
                                                                  uint64_t row0, Divider chunks, bool ceil) {
   __shared__ uint32_t shared[kThreads / 32];
+  __shared__ float inverses[128];
+  __shared__ __align__(16) uint8_t turn[VEC ? 16 : kThreads * Turn<TYPE>::kBytes];
   const Job& J = jobs.job[0];
   let_next_grid_start();
   wait_for_previous_grid();
   const float m = load_multiplier(J, shared);
-  if (is_narrow<TYPE, E8M0>(m)) round_rows<TYPE, E8M0, BLOCK, kNarrow>(J, rows, row0, chunks, ceil, m);
-  else round_rows<TYPE, E8M0, BLOCK, kExact>(J, rows, row0, chunks, ceil, m);
+  if (is_narrow<TYPE, E8M0>(m)) {
+    if constexpr (!E8M0) {
+      fill_inverses(inverses, m);
+      __syncthreads();
+    }
+    round_rows<TYPE, E8M0, BLOCK, kNarrow, VEC>(J, rows, row0, chunks, ceil, m, inverses, turn);
+  } else {
+    round_rows<TYPE, E8M0, BLOCK, kExact, VEC>(J, rows, row0, chunks, ceil, m, inverses, turn);
+  }
 }
 
 // ---- blocks along the columns, or along both axes in one read -----------------------
@@ -278,7 +367,8 @@ struct TileBytes {
 __device__ __forceinline__ int step_at(int r, int b) { return (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3); }
 
 template <int TYPE, bool E8M0, int BLOCK, int HOW>
-__device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t r0, uint64_t c0, bool ceil, float m) {
+__device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t r0, uint64_t c0, bool ceil, float m,
+                                           const float* inverses) {
   using B = TileBytes<TYPE>;
   uint8_t* input = smem;
   uint8_t* codes = smem + B::kInput;
@@ -299,14 +389,14 @@ __device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t
       uint32_t top = 0u;
 #pragma unroll
       for (int j = 0; j < 4 * Real<TYPE>::kBytes; ++j) {
-        top = join_max<TYPE>(top, word_max<TYPE>(words[j]));
+        top = join_max<TYPE>(top, words[j]);
         if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(words[j]);
         else unpack2<TYPE>(words[j], v[2 * j], v[2 * j + 1]);
       }
       top = final_max<TYPE>(top);
       if constexpr (BLOCK == 32) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       float step, inv;
-      uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, step, inv);
+      uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, inverses, step, inv);
       const bool finite = word != (uint32_t)kNan;
       if (c0 + chunk * 16 / BLOCK * BLOCK >= J.cols) word = 0u;
 #pragma unroll
@@ -334,7 +424,7 @@ __device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t
         top[1][i / BLOCK] = max(top[1][i / BLOCK], __float_as_uint(f.y) & 0x7FFFFFFFu);
       } else {  // both columns' maxima in one word
         const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
-        top[0][i / BLOCK] = join_max<TYPE>(top[0][i / BLOCK], word_max<TYPE>(w));
+        top[0][i / BLOCK] = join_max<TYPE>(top[0][i / BLOCK], w);
         unpack2<TYPE>(w, v[0][i], v[1][i]);
       }
     }
@@ -342,8 +432,8 @@ __device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t
     for (int b = 0; b < 32 / BLOCK; ++b) {
       if constexpr (TYPE != T5E_REAL_F32) {
         const uint32_t both = top[0][b];
-        top[0][b] = magnitude_bits<TYPE>(both & 0xFFFFu);
-        top[1][b] = magnitude_bits<TYPE>(both >> 16);
+        top[0][b] = magnitude_bits<TYPE>(both & 0x7FFFu);
+        top[1][b] = magnitude_bits<TYPE>((both >> 16) & 0x7FFFu);
       }
     }
 #pragma unroll
@@ -352,7 +442,7 @@ __device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t
 #pragma unroll
       for (int b = 0; b < 32 / BLOCK; ++b) {
         float step, inv;
-        uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top[h][b]), m, ceil, step, inv);
+        uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top[h][b]), m, ceil, inverses, step, inv);
         const bool finite = word != (uint32_t)kNan;
         if (r0 + part * 32 + b * BLOCK >= J.rows) word = 0u;
 #pragma unroll
@@ -395,11 +485,12 @@ __device__ __forceinline__ void round_tile(const Job& J, uint8_t* smem, uint64_t
 }
 
 template <int TYPE, bool E8M0, int BLOCK>
-__global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const __grid_constant__ Jobs jobs, bool ceil) {
+__global__ void __launch_bounds__(kThreads, TYPE == T5E_REAL_BF16 ? 4 : TYPE == T5E_REAL_F16 ? 3 : 2) quantize_tiles_kernel(const __grid_constant__ Jobs jobs, bool ceil) {
   using B = TileBytes<TYPE>;
   using T = typename Real<TYPE>::type;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint32_t shared[kThreads / 32];
+  __shared__ float inverses[128];
   const Job& J = job_of(jobs);
   let_next_grid_start();
   wait_for_previous_grid();
@@ -419,6 +510,18 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const __grid_c
                    :: "r"((uint32_t)__cvta_generic_to_shared(smem + r * B::kPitch + v * 16)), "l"(from), "r"(bytes) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+  } else if (J.words) {  // rows on 4-byte boundaries: words, all in flight at once
+    constexpr int kPer = 4 / Real<TYPE>::kBytes, kWords = kTile / kPer;
+#pragma unroll 4
+    for (int i = 0; i < kTile * kWords / kThreads; ++i) {
+      const int item = i * kThreads + threadIdx.x, r = item / kWords, v = item % kWords;
+      const int64_t have = r0 + r < J.rows ? (int64_t)(J.cols - c0) - v * kPer : 0;
+      const uint32_t bytes = have >= kPer ? 4u : (have > 0 ? (uint32_t)have * Real<TYPE>::kBytes : 0u);
+      const T* from = bytes ? src + (int64_t)r * J.stride + v * kPer : static_cast<const T*>(J.x);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                   :: "r"((uint32_t)__cvta_generic_to_shared(smem + r * B::kPitch + v * 4)), "l"(from), "r"(bytes) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   } else {
 #pragma unroll 16
     for (int i = 0; i < kTile * kTile / kThreads; ++i) {
@@ -428,51 +531,94 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const __grid_c
     }
   }
   const float m = load_multiplier(J, shared);
+  if constexpr (!E8M0) fill_inverses(inverses, m);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  if (is_narrow<TYPE, E8M0>(m)) round_tile<TYPE, E8M0, BLOCK, kNarrow>(J, smem, r0, c0, ceil, m);
-  else round_tile<TYPE, E8M0, BLOCK, kExact>(J, smem, r0, c0, ceil, m);
+  if (is_narrow<TYPE, E8M0>(m)) round_tile<TYPE, E8M0, BLOCK, kNarrow>(J, smem, r0, c0, ceil, m, inverses);
+  else round_tile<TYPE, E8M0, BLOCK, kExact>(J, smem, r0, c0, ceil, m, inverses);
 }
 
 // ---- back to real values -------------------------------------------------------
 
-template <int TYPE, bool E8M0, int BLOCK>
+// A thread takes 16 codes of four places of the launch at a time, all loaded
+// before the first is worked on.  Rows of `out` on 16-byte boundaries take
+// vectors; others pass through shared memory, so that the lanes' stores are
+// neighbours.
+template <int TYPE, bool E8M0, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_stride,
                                                               const uint8_t* __restrict__ scales, uint32_t groups,
                                                               uint32_t rows, uint64_t row0, uint32_t k, Divider chunks,
                                                               const float* multiplier, void* __restrict__ out,
-                                                              int64_t out_stride, bool vec) {
+                                                              int64_t out_stride, bool wide) {
+  constexpr int kAtOnce = 4, kPitch = 20;  // a lane's 16 floats 20 apart: vectors of a warp meet no bank twice
+  __shared__ __align__(16) float turn[VEC ? 4 : kThreads * kPitch];
   let_next_grid_start();
   wait_for_previous_grid();
   const float back = multiplier != nullptr ? 1.f / *multiplier : 1.f;
-  const uint32_t total = rows * chunks.d;
+  const uint32_t total = rows * chunks.d, step = gridDim.x * kThreads;
+  const int lane = threadIdx.x & 31;
   using T = typename Real<TYPE>::type;
-  for (uint32_t item = blockIdx.x * kThreads + threadIdx.x; item < total; item += gridDim.x * kThreads) {
-    const uint32_t row = divided(item, chunks), chunk = item - row * chunks.d, e0 = chunk * 16u;
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(data + (int64_t)(row0 + row) * data_stride + chunk * 8u));
-    const float s = scale_value<E8M0>(__ldg(scales + scale_offset(row0 + row, e0 / BLOCK, groups)));
-    float v[16];
-    from_e2m1x8(w.x, v);
-    from_e2m1x8(w.y, v + 8);
+  for (uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u); base < total; base += kAtOnce * step) {
+    uint32_t row[kAtOnce], e0[kAtOnce], byte[kAtOnce];
+    uint2 w[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = v[j] * s * back;
-    T* dst = static_cast<T*>(out) + (int64_t)(row0 + row) * out_stride + e0;
-    if (vec && e0 + 16u <= k) {
-      if constexpr (TYPE == T5E_REAL_F32) {
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t item = base + i * step + lane;
+      const bool in = item < total;
+      row[i] = in ? divided(item, chunks) : 0u;
+      e0[i] = in ? (item - row[i] * chunks.d) * 16u : k;  // k: nothing to store
+      if (in) {
+        w[i] = __ldg(reinterpret_cast<const uint2*>(data + (int64_t)(row0 + row[i]) * data_stride + e0[i] / 2u));
+        byte[i] = __ldg(scales + scale_offset(row0 + row[i], e0[i] / BLOCK, groups));
+      } else {
+        w[i] = make_uint2(0u, 0u);
+        byte[i] = 0u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (base + i * step >= total) break;
+      const float s = scale_value<E8M0>(byte[i]);
+      float v[16];
+      from_e2m1x8(w[i].x, v);
+      from_e2m1x8(w[i].y, v + 8);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = v[j] * s * back;
+      const int64_t at = (int64_t)(row0 + row[i]) * out_stride + e0[i];
+      T* dst = static_cast<T*>(out) + at;
+      if constexpr (VEC) {
+        if (e0[i] + 16u <= k) {
+          uint4 o[Real<TYPE>::kBytes];
+          uint32_t* words = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+          for (int j = 0; j < 4 * Real<TYPE>::kBytes; ++j) {
+            if constexpr (TYPE == T5E_REAL_F32) words[j] = __float_as_uint(v[j]);
+            else words[j] = pack2<TYPE>(v[2 * j], v[2 * j + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < Real<TYPE>::kBytes; j += 2) store32(reinterpret_cast<uint4*>(dst) + j, wide, o[j], o[j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (e0[i] + j < k) dst[j] = from_f32<TYPE>(v[j]);
+        }
+      } else {
+        float* mine = turn + threadIdx.x * kPitch;
+        const float* warp = turn + (threadIdx.x & ~31) * kPitch;
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-      } else {
+          reinterpret_cast<float4*>(mine)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        __syncwarp();
+        // two lanes' 16 elements at a time
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          reinterpret_cast<uint4*>(dst)[j] =
-              make_uint4(pack2<TYPE>(v[8 * j], v[8 * j + 1]), pack2<TYPE>(v[8 * j + 2], v[8 * j + 3]),
-                         pack2<TYPE>(v[8 * j + 4], v[8 * j + 5]), pack2<TYPE>(v[8 * j + 6], v[8 * j + 7]));
+        for (int j = 0; j < 16; ++j) {
+          const int from = 2 * j + (lane >> 4), element = lane & 15;
+          const int64_t place = __shfl_sync(0xFFFFFFFFu, at, from) + element;
+          const uint32_t first = __shfl_sync(0xFFFFFFFFu, e0[i], from);
+          if (first + element < k) static_cast<T*>(out)[place] = from_f32<TYPE>(warp[from * kPitch + element]);
+        }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (e0 + j < k) dst[j] = from_f32<TYPE>(v[j]);
     }
   }
 }
@@ -512,8 +658,8 @@ unsigned grid_of(uint64_t blocks, unsigned per_sm) {
 // Rows of one launch: the kernels count chunks of a launch in 32 bits.
 uint64_t rows_per_launch(uint64_t chunks) { return chunks ? (uint64_t(1) << 30) / chunks : 1; }
 
-bool rows_aligned(int32_t type, const void* x, uint64_t rows, int64_t stride) {
-  return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows <= 1 || (stride * type_bytes(type)) % 16 == 0);
+bool rows_aligned(int32_t type, const void* x, uint64_t rows, int64_t stride, unsigned bytes = 16) {
+  return reinterpret_cast<uintptr_t>(x) % bytes == 0 && (rows <= 1 || (stride * type_bytes(type)) % bytes == 0);
 }
 
 Divider divider(uint32_t d) {
@@ -530,11 +676,15 @@ int quantize_rows(int32_t type, const Jobs& jobs, const t5e_blocks& out, bool ce
   const uint64_t per = rows_per_launch(chunks.d);
   for (uint64_t row0 = 0; row0 < J.rows; row0 += per) {
     const uint32_t n = (uint32_t)(J.rows - row0 < per ? J.rows - row0 : per);
-    const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 8);
+    const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 6);
     const int rc = with_form(type, out.scale_format, out.scale_block, [&](auto t, auto e8, auto blk) {
-      return launched(launch_dependent(quantize_rows_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value>,
-                                       dim3(grid), kThreads, 0, stream, jobs, n, row0, chunks, ceil),
-                      "quantize_rows_kernel launch");
+      auto go = [&](auto v) {
+        return launched(launch_dependent(quantize_rows_kernel<decltype(t)::value, decltype(e8)::value,
+                                                              decltype(blk)::value, decltype(v)::value>,
+                                         dim3(grid), kThreads, 0, stream, jobs, n, row0, chunks, ceil),
+                        "quantize_rows_kernel launch");
+      };
+      return J.vec ? go(std::true_type{}) : go(std::false_type{});
     });
     if (rc != T5E_OK) return rc;
   }
@@ -687,6 +837,8 @@ int t5e_quantize_blocks(const t5e_quantize* q, int32_t n, void* stream) {
     J.partials = Q.partials;
     J.count = Q.count;
     J.vec = rows_aligned(Q.type, Q.x, Q.rows, Q.stride);
+    J.wide = rows_aligned(Q.type, Q.x, Q.rows, Q.stride, 32);
+    J.words = rows_aligned(Q.type, Q.x, Q.rows, Q.stride, 4);
     if (by_rows) {
       J.row_data = static_cast<uint8_t*>(Q.by_rows.data);
       J.row_stride = Q.by_rows.stride;
@@ -729,18 +881,22 @@ int t5e_dequantize_blocks(const t5e_blocks* b, const float* multiplier, int32_t 
     return T5E_ERR_INVALID;
   const uint32_t groups = scale_groups(*b);
   const Divider chunks = divider((uint32_t)(((uint64_t)b->k + 15) / 16));
-  const bool vec = rows_aligned(type, out, b->rows, out_stride);
+  const bool vec = rows_aligned(type, out, b->rows, out_stride), wide = rows_aligned(type, out, b->rows, out_stride, 32);
   const uint64_t per = rows_per_launch(chunks.d);
   for (uint64_t row0 = 0; row0 < b->rows; row0 += per) {
     const uint32_t n = (uint32_t)(b->rows - row0 < per ? b->rows - row0 : per);
     const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 8);
     const int rc = with_form(type, b->scale_format, b->scale_block, [&](auto t, auto e8, auto blk) {
-      return launched(launch_dependent(dequantize_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value>,
-                                       dim3(grid), kThreads, 0, static_cast<cudaStream_t>(stream),
-                                       static_cast<const uint8_t*>(b->data), b->stride,
-                                       static_cast<const uint8_t*>(b->scales), groups, n, row0, (uint32_t)b->k, chunks,
-                                       multiplier, out, out_stride, vec),
-                      "dequantize_kernel launch");
+      auto go = [&](auto v) {
+        return launched(launch_dependent(dequantize_kernel<decltype(t)::value, decltype(e8)::value, decltype(blk)::value,
+                                                           decltype(v)::value>,
+                                         dim3(grid), kThreads, 0, static_cast<cudaStream_t>(stream),
+                                         static_cast<const uint8_t*>(b->data), b->stride,
+                                         static_cast<const uint8_t*>(b->scales), groups, n, row0, (uint32_t)b->k, chunks,
+                                         multiplier, out, out_stride, wide),
+                        "dequantize_kernel launch");
+      };
+      return vec ? go(std::true_type{}) : go(std::false_type{});
     });
     if (rc != T5E_OK) return rc;
   }

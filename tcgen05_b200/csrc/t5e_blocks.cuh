@@ -67,12 +67,47 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// 32 bytes of a lane in one access (32-byte aligned) or two (16-byte aligned): a
+// warp whose lanes take neighbouring 32 bytes then touches whole lines.
+__device__ __forceinline__ void load32(const void* p, bool wide, uint4& a, uint4& b) {
+  if (wide) {
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+  } else {
+    a = __ldg(static_cast<const uint4*>(p));
+    b = __ldg(static_cast<const uint4*>(p) + 1);
+  }
+}
+__device__ __forceinline__ void store32(void* p, bool wide, const uint4& a, const uint4& b) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = a;
+    static_cast<uint4*>(p)[1] = b;
+  }
+}
+
 // Byte offset of scale b of row r in the scale tiles: 128 rows by 4 scales
 // are 512 consecutive bytes, ordered so that one 16-byte line holds the four
 // scales of rows r, r + 32, r + 64 and r + 96 (the order in which the tensor
 // cores take them from tensor memory).  `groups` = ceil(scales per row / 4).
 __device__ __forceinline__ uint64_t scale_offset(uint64_t r, uint32_t b, uint32_t groups) {
   return ((r >> 7) * groups + (b >> 2)) * 512u + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
+}
+
+// Value of a scale byte (NaN for the NaN codes; the sign bit of a UE4M3 byte
+// is ignored, as by the tensor cores).
+template <bool E8M0>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  if constexpr (E8M0) {
+    if (byte == 0xFFu) return __uint_as_float(0x7FC00000u);
+    return byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+  } else {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(byte & 0x7Fu)));
+    return __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
+  }
 }
 
 // How the elements of a tensor are multiplied and divided.
@@ -109,8 +144,12 @@ __device__ __forceinline__ bool is_narrow(float m) {
 // Rounding to F32 is monotonic, so am = F32(a * m) is the largest |u|.  A block
 // with a NaN or an infinity (or a product beyond F32) gets the NaN scale and a
 // zero step.
+//
+// `inverses`: for narrow UE4M3 blocks, m / scale for every scale byte (0 for a
+// zero scale and for NaN) in shared memory, see fill_inverses.
 template <bool E8M0, int HOW>
-__device__ __forceinline__ uint32_t block_scale(float a, float m, bool ceil, float& step, float& inv) {
+__device__ __forceinline__ uint32_t block_scale(float a, float m, bool ceil, const float* inverses, float& step,
+                                                float& inv) {
   const float am = a * m;
   const uint32_t bits = __float_as_uint(am);
   if constexpr (E8M0) {
@@ -125,16 +164,30 @@ __device__ __forceinline__ uint32_t block_scale(float a, float m, bool ceil, flo
     step = 0.f;  // unused: products with inv are exact wherever they reach the E2M1 range
     return finite ? (uint32_t)w : 0xFFu;
   } else {
-    const bool finite = bits < 0x7F800000u;
-    const float want = HOW == kNarrow ? am * (1.f / 6.f) : __fdiv_rn(am, 6.f);
-    uint16_t two;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(want));
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(two));
-    step = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
-    inv = finite && step > 0.f ? __frcp_rn(step) : 0.f;
-    if constexpr (HOW == kNarrow) inv *= m;
-    return finite ? (uint32_t)(two & 0x7Fu) : 0x7Fu;
+    if constexpr (HOW == kNarrow) {
+      uint16_t two;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(am * (1.f / 6.f)));
+      const uint32_t word = bits < 0x7F800000u ? (uint32_t)two : 0x7Fu;
+      inv = inverses[word];
+      step = 0.f;  // unused
+      return word;
+    } else {
+      const bool finite = bits < 0x7F800000u;
+      uint16_t two;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(__fdiv_rn(am, 6.f)));
+      step = scale_value<false>(two);
+      inv = finite && step > 0.f ? __frcp_rn(step) : 0.f;
+      return finite ? (uint32_t)two : 0x7Fu;
+    }
+  }
+}
+
+// The 128 entries of block_scale's table, by the block's threads; a barrier has
+// to follow.
+__device__ __forceinline__ void fill_inverses(float* inverses, float m) {
+  for (uint32_t i = threadIdx.x; i < 128u; i += blockDim.x) {
+    const float step = scale_value<false>(i);
+    inverses[i] = i == 0u || i == 0x7Fu ? 0.f : __frcp_rn(step) * m;
   }
 }
 
@@ -187,20 +240,6 @@ __device__ __forceinline__ void from_e2m1x8(uint32_t w, float* v) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
     v[2 * i] = f.x;
     v[2 * i + 1] = f.y;
-  }
-}
-
-// Value of a scale byte (NaN for the NaN codes; the sign bit of a UE4M3 byte
-// is ignored, as by the tensor cores).
-template <bool E8M0>
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-  if constexpr (E8M0) {
-    if (byte == 0xFFu) return __uint_as_float(0x7FC00000u);
-    return byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
-  } else {
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(byte & 0x7Fu)));
-    return __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
   }
 }
 

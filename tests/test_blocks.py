@@ -191,7 +191,7 @@ def test_c_entry_points_refuse_bad_arguments():
     bad = [dict(k=0), dict(k=nat.MAX_BLOCK_K + 1), dict(stride=48), dict(stride=72), dict(data=4104), dict(scales=4100),
            dict(scale_block=32), dict(scale_format=0), dict(data=None), dict(scales=None),
            dict(rows=nat.MAX_BLOCK_ROWS + 1)]
-    none = nat.Blocks()
+    none, second = nat.Blocks(), blk()
 
     def quantize(n=1, **kw):
         q = nat.Quantize(4096, 8, 128, 128, 0, 0, None, None, 0, 0, blk(), none)
@@ -203,7 +203,7 @@ def test_c_entry_points_refuse_bad_arguments():
         b = blk(**kw)
         assert lib.t5e_dequantize_blocks(ctypes.byref(b), None, 0, 4096, 128, None) == nat.ERR_INVALID
         assert quantize(rows=b.rows, cols=max(b.k, 0), by_rows=b) == nat.ERR_INVALID
-        mm = nat.BlockMm(ctypes.pointer(b), ctypes.pointer(blk()), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
+        mm = nat.BlockMm(ctypes.addressof(b), ctypes.addressof(second), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(mm), None) == nat.ERR_INVALID
     good = blk()
     for kw in (dict(type=3), dict(rounding=1), dict(stride=127), dict(x=4098), dict(x=None), dict(partials=4096, count=4),
@@ -216,14 +216,14 @@ def test_c_entry_points_refuse_bad_arguments():
         assert lib.t5e_block_multiplier(0, 4096, 8, 128, 128, partials, count, out, None) == nat.ERR_INVALID
 
     def mm(**kw):
-        m = nat.BlockMm(ctypes.pointer(good), ctypes.pointer(blk()), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
+        m = nat.BlockMm(ctypes.addressof(good), ctypes.addressof(second), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
         for name, v in kw.items():
             setattr(m, name, v)
         return lib.t5e_block_scaled_mm(ctypes.byref(m), None)
 
     other = blk(scale_format=nat.SCALE_UE8M0)
     for kw in (dict(d=None), dict(d=4098), dict(d_stride=7), dict(d_type=3), dict(c=4096, c_type=5), dict(c=4098),
-               dict(form=3), dict(form=16), dict(form=2), dict(b=ctypes.pointer(other)), dict(a=None)):
+               dict(form=3), dict(form=16), dict(form=2), dict(b=ctypes.addressof(other)), dict(a=None)):
         assert mm(**kw) == nat.ERR_INVALID, kw
     assert lib.t5e_block_scaled_mm_expired(None) == nat.ERR_INVALID
 
@@ -238,7 +238,7 @@ def test_empty_calls_launch_nothing():
     q = nat.Quantize(None, 0, 128, 128, 0, 0, None, None, 0, 0, nat.Blocks(), nat.Blocks())
     assert lib.t5e_quantize_blocks(ctypes.byref(q), 1, None) == nat.OK
     for a, b in ((none, some), (some, none)):
-        m = nat.BlockMm(ctypes.pointer(a), ctypes.pointer(b), None, None, 1.0, 0, None, 0, 0, 0, 0, None, 8)
+        m = nat.BlockMm(ctypes.addressof(a), ctypes.addressof(b), None, None, 1.0, 0, None, 0, 0, 0, 0, None, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(m), None) == nat.OK
 
 
