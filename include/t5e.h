@@ -347,7 +347,7 @@ enum { T5E_SCALE_ROUND_NEAREST = 0, T5E_SCALE_ROUND_FLOOR = 1, T5E_SCALE_ROUND_C
  * scale_format/scale_block: T5E_SCALE_UE4M3 with 16, T5E_SCALE_UE8M0 with 16
  * or 32 (make_model's scaling and scale_vec 4 or 2).
  */
-#define T5E_MAX_BLOCK_K (1ll << 28)
+#define T5E_MAX_BLOCK_K (1ll << 27)
 #define T5E_MAX_BLOCK_ROWS (1ull << 30)
 typedef struct t5e_blocks {
     void* data;

@@ -57,7 +57,7 @@ NOALLOC_STAGE_BYTES = 32 * 1024 * 1024
 REAL_F32, REAL_BF16, REAL_F16 = 0, 1, 2
 SCALE_ROUND_NEAREST, SCALE_ROUND_FLOOR, SCALE_ROUND_CEIL = 0, 1, 2
 MAX_PARTIALS = 1024
-MAX_BLOCK_K = 1 << 28
+MAX_BLOCK_K = 1 << 27
 MAX_BLOCK_ROWS = 1 << 30
 
 CASE_OK, CASE_BAD_SELECTOR, CASE_EMPTY, CASE_SCALE_COVER, CASE_META_WORDS, CASE_TIMEOUT = 0, 1, 2, 3, 4, 5

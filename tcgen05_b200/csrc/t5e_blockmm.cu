@@ -827,28 +827,41 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
       fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (count & 1u) * L::kSecond;
       const uint32_t free_bar = in_block(smem_u32(&acc_free[count & 1u]), 0);
-      // chunks of 32 columns, the shared ones first: they are the last of the
-      // first accumulator and the first of the second
+      // chunks of 32 columns.  The shared ones (the last of the first accumulator,
+      // the first of the second) are all read at once, and let the next tile
+      // start before anything is done with them
       constexpr int kChunks = BN / 32, kFirst = L::kShared / 32;
-#pragma unroll 1
-      for (int i = 0; i < kChunks; ++i) {
-        int chunk = i;
-        if (L::kShared && (count & 1u) == 0u) chunk = i < kFirst ? kChunks - kFirst + i : i - kFirst;
-        float v[32];
-        load_acc32(acc + chunk * 32, v);
-        acc_loaded();
-        if (i == (L::kShared ? kFirst - 1 : kChunks - 1)) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_in(free_bar);
-        }
+      auto finish = [&](int chunk, int turn, float* v) {
         if (!ok) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
         const uint32_t q = q0 + chunk * 32;
-        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box + (i & 1) * 4096);
+        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box + (turn & 1) * 4096);
         else store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
+      };
+      auto release = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_in(free_bar);
+      };
+      const int first_shared = (count & 1u) == 0u ? kChunks - kFirst : 0, first_own = (count & 1u) == 0u ? 0 : kFirst;
+      if constexpr (kFirst > 0) {
+        float head[kFirst * 32];
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) load_acc32(acc + (first_shared + i) * 32, head + i * 32);
+        acc_loaded();
+        release();
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) finish(first_shared + i, i, head + i * 32);
+      }
+#pragma unroll 1
+      for (int i = kFirst; i < kChunks; ++i) {
+        float v[32];
+        load_acc32(acc + (first_own + i - kFirst) * 32, v);
+        acc_loaded();
+        if (kFirst == 0 && i == kChunks - 1) release();
+        finish(first_own + i - kFirst, i, v);
       }
     }
     if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

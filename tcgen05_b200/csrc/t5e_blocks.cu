@@ -177,32 +177,53 @@ __device__ __forceinline__ uint32_t divided(uint32_t n, const Divider& v) {
 
 // ---- blocks along the rows ---------------------------------------------------
 //
-// A thread takes 16 consecutive elements: one block, or half of a 32-element
-// one whose other half its neighbour lane holds.  Per row the chunks run up
-// to a whole group of four scales, so that four (eight) neighbouring lanes
-// always hold one group and one of them stores its four scale bytes as a word.
-// The next elements are loaded before the present ones are worked on.  Where
-// rows do not start on 16-byte boundaries the lanes load neighbouring elements
-// and exchange them through shared memory.
+// A thread takes 32 consecutive elements: two blocks of 16 or one of 32, so
+// that no maximum needs an exchange, and what a chunk costs besides its
+// elements (places, scales) is paid half as often as with 16 (11 thread
+// instructions per element there, which bound the kernel: 8192 x 8192 BF16 to
+// UE4M3 blocks 37 us).  Per row the chunks run up to a whole group of four
+// scales: two (four) neighbouring lanes hold one group, and one of them stores
+// its four scale bytes as a word.  The next elements are loaded before the
+// present ones are worked on.  Where rows do not start on 16-byte boundaries
+// the lanes load neighbouring elements and exchange them through shared
+// memory.
+constexpr int kChunk = 32;
+
 template <int TYPE>
 struct Chunk {
-  uint32_t row, e0;  // e0 = k: nothing
-  uint4 w[Real<TYPE>::kBytes];
+  uint32_t row, e0;  // e0 beyond k: nothing
+  uint4 w[2 * Real<TYPE>::kBytes];
+};
+
+// Places of a thread's chunks, a launch's threads apart from one to the next.
+struct Walk {
+  uint32_t row, chunk;
+  __device__ __forceinline__ void start(uint32_t item, const Divider& chunks) {
+    row = divided(item, chunks);
+    chunk = item - row * chunks.d;
+  }
+  __device__ __forceinline__ void advance(uint32_t rows_on, uint32_t chunks_on, uint32_t per_row) {
+    row += rows_on;
+    chunk += chunks_on;
+    if (chunk >= per_row) {
+      chunk -= per_row;
+      ++row;
+    }
+  }
 };
 
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void load_chunk(const Job& J, uint64_t row0, uint32_t item, uint32_t total, const Divider& chunks,
-                                           Chunk<TYPE>& c) {
+__device__ __forceinline__ void load_chunk(const Job& J, uint64_t row0, const Walk& at, uint32_t rows, Chunk<TYPE>& c) {
   using T = typename Real<TYPE>::type;
   const uint32_t k = (uint32_t)J.cols;
-  const bool in = item < total;
-  c.row = in ? divided(item, chunks) : 0u;
-  c.e0 = in ? (item - c.row * chunks.d) * 16u : 0x7FFFFFFFu;
-  const int64_t at = (int64_t)(row0 + c.row) * J.stride + c.e0;
+  // after a pass for the largest value the last rows are the likeliest in L2
+  c.row = J.partials != nullptr ? rows - 1u - at.row : at.row;
+  c.e0 = at.row < rows ? at.chunk * kChunk : 0x7FFFFFFFu;
+  const int64_t place = (int64_t)(row0 + c.row) * J.stride + c.e0;
   if constexpr (VEC) {
-    constexpr int kVecs = Real<TYPE>::kBytes, kPer = 16 / Real<TYPE>::kBytes;
-    const T* src = static_cast<const T*>(J.x) + at;
-    if (c.e0 + 16u <= k) {
+    constexpr int kVecs = 2 * Real<TYPE>::kBytes, kPer = 16 / Real<TYPE>::kBytes;
+    const T* src = static_cast<const T*>(J.x) + place;
+    if (c.e0 + kChunk <= k) {
 #pragma unroll
       for (int j = 0; j < kVecs; j += 2) load32(reinterpret_cast<const uint4*>(src) + j, J.wide, c.w[j], c.w[j + 1]);
     } else {  // the end of a row, or behind it: what exists, then zeros
@@ -224,31 +245,28 @@ __device__ __forceinline__ void load_chunk(const Job& J, uint64_t row0, uint32_t
       }
     }
   } else {
-    // element j of the exchange: the elements (lane & 15) of the chunks of lanes
-    // 2j and 2j + 1, packed here by pairs of j
+    // turn j: the lanes take the 32 elements of lane j's chunk
     const int lane = threadIdx.x & 31;
     uint32_t* words = reinterpret_cast<uint32_t*>(c.w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int from = 2 * j + (lane >> 4), element = lane & 15;
-      const int64_t place = __shfl_sync(0xFFFFFFFFu, at, from) + element;
-      const uint32_t first = __shfl_sync(0xFFFFFFFFu, c.e0, from);
-      const bool there = first + element < k;
+    for (int j = 0; j < kChunk; ++j) {
+      const int64_t from = __shfl_sync(0xFFFFFFFFu, place, j) + lane;
+      const bool there = __shfl_sync(0xFFFFFFFFu, c.e0, j) + lane < k;
       if constexpr (TYPE == T5E_REAL_F32) {
-        words[j] = there ? static_cast<const uint32_t*>(J.x)[place] : 0u;
+        words[j] = there ? static_cast<const uint32_t*>(J.x)[from] : 0u;
       } else {
-        const uint32_t h = there ? (uint32_t)static_cast<const uint16_t*>(J.x)[place] : 0u;
+        const uint32_t h = there ? (uint32_t)static_cast<const uint16_t*>(J.x)[from] : 0u;
         words[j / 2] = (j & 1) ? words[j / 2] | (h << 16) : h;
       }
     }
   }
 }
 
-// After a load by neighbours: each lane's own 16 elements, through the warp's
-// part of `turn` (32 lanes of kTurn bytes).
+// After a load by neighbours: each lane's own 32 elements, through the warp's
+// part of `turn`.
 template <int TYPE>
 struct Turn {
-  static constexpr int kBytes = 16 * Real<TYPE>::kBytes + 16;  // a lane's, 16 bytes apart: vectors meet no bank twice
+  static constexpr int kBytes = kChunk * Real<TYPE>::kBytes + 16;  // a lane's, 16 bytes apart: vectors meet no bank twice
 };
 template <int TYPE>
 __device__ __forceinline__ void turn_chunk(Chunk<TYPE>& c, uint8_t* turn) {
@@ -256,73 +274,92 @@ __device__ __forceinline__ void turn_chunk(Chunk<TYPE>& c, uint8_t* turn) {
   const uint32_t* words = reinterpret_cast<const uint32_t*>(c.w);
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    uint8_t* to = turn + (2 * j + (lane >> 4)) * Turn<TYPE>::kBytes + (lane & 15) * Real<TYPE>::kBytes;
+  for (int j = 0; j < kChunk; ++j) {
+    uint8_t* to = turn + j * Turn<TYPE>::kBytes + lane * Real<TYPE>::kBytes;
     if constexpr (TYPE == T5E_REAL_F32) *reinterpret_cast<uint32_t*>(to) = words[j];
     else *reinterpret_cast<uint16_t*>(to) = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
   }
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < Real<TYPE>::kBytes; ++j)
+  for (int j = 0; j < 2 * Real<TYPE>::kBytes; ++j)
     c.w[j] = *reinterpret_cast<const uint4*>(turn + lane * Turn<TYPE>::kBytes + j * 16);
 }
 
 template <int TYPE, bool E8M0, int BLOCK, int HOW, bool VEC>
 __device__ __forceinline__ void round_rows(const Job& J, uint32_t rows, uint64_t row0, const Divider& chunks, bool ceil,
                                            float m, const float* inverses, uint8_t* turn) {
-  constexpr uint32_t kLanes = BLOCK / 4;  // lanes of one group of four scales
+  constexpr int kWords = kChunk * Real<TYPE>::kBytes / 4, kBlocks = kChunk / BLOCK;
   const uint32_t k = (uint32_t)J.cols;
-  const uint32_t stored = (k + 31u) / 32u * 32u;  // elements with codes in `data`
-  const uint32_t total = rows * chunks.d;
+  const uint32_t total = rows * chunks.d, step = gridDim.x * kThreads;
+  const uint32_t rows_on = divided(step, chunks), chunks_on = step - rows_on * chunks.d;
   const int lane = threadIdx.x & 31;
+  uint8_t* scales = J.row_scales + scale_offset(row0, 0, J.row_groups);  // row0 is a multiple of 128
   uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u);
+  Walk at;
+  at.start(base + lane, chunks);
   Chunk<TYPE> c;
-  if (base < total) load_chunk<TYPE, VEC>(J, row0, base + lane, total, chunks, c);
-  while (base < total) {
-    const uint32_t next = base + gridDim.x * kThreads;
+  if (base < total) load_chunk<TYPE, VEC>(J, row0, at, rows, c);
+  for (; base < total; base += step) {
     if constexpr (!VEC) turn_chunk<TYPE>(c, turn + (threadIdx.x & ~31u) * Turn<TYPE>::kBytes);
     const uint32_t row = c.row, e0 = c.e0;
-    const bool in = base + lane < total;
-    float v[16];
-    uint32_t top = 0u;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(c.w);
+    uint32_t words[kWords];
 #pragma unroll
-    for (int j = 0; j < Real<TYPE>::kBytes * 4; ++j) {
-      top = join_max<TYPE>(top, words[j]);
-      if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(words[j]);
-      else unpack2<TYPE>(words[j], v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < kWords / 4; ++j) {
+      words[4 * j] = c.w[j].x;
+      words[4 * j + 1] = c.w[j].y;
+      words[4 * j + 2] = c.w[j].z;
+      words[4 * j + 3] = c.w[j].w;
     }
-    if (next < total) load_chunk<TYPE, VEC>(J, row0, next + lane, total, chunks, c);
-    top = final_max<TYPE>(top);
-    if constexpr (BLOCK == 32) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    float step, inv;
-    uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(top), m, ceil, inverses, step, inv);
-    const bool finite = word != (E8M0 ? 0xFFu : 0x7Fu);
-    if (e0 / BLOCK * BLOCK >= k) word = 0u;  // a scale behind the last block
+    at.advance(rows_on, chunks_on, chunks.d);
+    if (base + step < total) load_chunk<TYPE, VEC>(J, row0, at, rows, c);
+    uint32_t out[4], bytes = 0u;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = divide<E8M0, HOW>(v[j], m, step, inv);
-    uint2 codes = make_uint2(e2m1x8(v), e2m1x8(v + 8));
-    if (!finite) codes = make_uint2(0u, 0u);
-    if (in && e0 < stored)
-      *reinterpret_cast<uint2*>(J.row_data + (int64_t)(row0 + row) * J.row_stride + e0 / 2u) = codes;
+    for (int b = 0; b < kBlocks; ++b) {
+      constexpr int kIn = kWords / kBlocks;
+      const uint32_t* mine = words + b * kIn;
+      uint32_t top = 0u;
+#pragma unroll
+      for (int j = 0; j < kIn; ++j) top = join_max<TYPE>(top, mine[j]);
+      float step_value, inv;
+      uint32_t word = block_scale<E8M0, HOW>(__uint_as_float(final_max<TYPE>(top)), m, ceil, inverses, step_value, inv);
+      const bool finite = word != (E8M0 ? 0xFFu : 0x7Fu);
+      if (e0 + b * BLOCK >= k) word = 0u;  // a scale behind the last block
+      bytes |= word << (8 * b);
+#pragma unroll
+      for (int h = 0; h < BLOCK / 8; ++h) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8 * Real<TYPE>::kBytes / 4; ++j) {
+          const uint32_t w = mine[h * 8 * Real<TYPE>::kBytes / 4 + j];
+          if constexpr (TYPE == T5E_REAL_F32) v[j] = __uint_as_float(w);
+          else unpack2<TYPE>(w, v[2 * j], v[2 * j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = divide<E8M0, HOW>(v[j], m, step_value, inv);
+        out[b * (BLOCK / 8) + h] = finite ? e2m1x8(v) : 0u;
+      }
+    }
+    if (e0 < k) {  // chunks are the rows' groups of 32 codes
+      *reinterpret_cast<uint4*>(J.row_data + (int64_t)(row0 + row) * J.row_stride + e0 / 2u) =
+          make_uint4(out[0], out[1], out[2], out[3]);
+    }
     // four scale bytes to one word
     if constexpr (BLOCK == 16) {
-      word <<= 8 * (lane & 3);
-      word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
-      word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+      bytes <<= 16 * (lane & 1);
+      bytes |= __shfl_xor_sync(0xFFFFFFFFu, bytes, 1);
     } else {
-      word <<= 8 * ((lane >> 1) & 3);
-      word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
-      word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+      bytes <<= 8 * (lane & 3);
+      bytes |= __shfl_xor_sync(0xFFFFFFFFu, bytes, 1);
+      bytes |= __shfl_xor_sync(0xFFFFFFFFu, bytes, 2);
     }
-    if (in && lane % kLanes == 0)
-      *reinterpret_cast<uint32_t*>(J.row_scales + scale_offset(row0 + row, e0 / BLOCK, J.row_groups)) = word;
-    base = next;
+    if (lane % (BLOCK / 8) == 0 && row < rows)
+      *reinterpret_cast<uint32_t*>(scales + ((row >> 7) * J.row_groups + e0 / (4 * BLOCK)) * 512u + (row & 31u) * 16u +
+                                   ((row >> 5) & 3u) * 4u) = bytes;
   }
 }
 
 template <int TYPE, bool E8M0, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ Jobs jobs, uint32_t rows,
+__global__ void __launch_bounds__(kThreads, VEC ? 1 : 3) quantize_rows_kernel(const __grid_constant__ Jobs jobs, uint32_t rows,
                                                                  uint64_t row0, Divider chunks, bool ceil) {
   __shared__ uint32_t shared[kThreads / 32];
   __shared__ float inverses[128];
@@ -494,12 +531,25 @@ __global__ void __launch_bounds__(kThreads, TYPE == T5E_REAL_BF16 ? 4 : TYPE == 
   const Job& J = job_of(jobs);
   let_next_grid_start();
   wait_for_previous_grid();
-  const uint64_t tile = blockIdx.x - J.first_block, across = (J.cols + kTile - 1) / kTile;
+  const uint64_t across = (J.cols + kTile - 1) / kTile;
+  uint64_t tile = blockIdx.x - J.first_block;
+  // after a pass for the largest value the last rows are the likeliest in L2
+  if (J.partials != nullptr) tile = across * ((J.rows + kTile - 1) / kTile) - 1 - tile;
   const uint64_t r0 = tile / across * kTile, c0 = tile % across * kTile;
   const T* src = static_cast<const T*>(J.x) + (int64_t)r0 * J.stride + (int64_t)c0;
-  if (J.vec) {
-    constexpr int kPer = 16 / Real<TYPE>::kBytes, kVecs = kTile / kPer;  // elements of a vector, vectors of a row
+  const bool whole = r0 + kTile <= J.rows && c0 + kTile <= J.cols;
+  if (J.vec && whole) {
+    constexpr int kPer = 16 / Real<TYPE>::kBytes, kVecs = kTile / kPer, kRows = kThreads / kVecs;
+    const int r = threadIdx.x / kVecs, v = threadIdx.x % kVecs;
+    const T* from = src + (int64_t)r * J.stride + v * kPer;
+    uint32_t to = (uint32_t)__cvta_generic_to_shared(smem + r * B::kPitch + v * 16);
 #pragma unroll
+    for (int i = 0; i < kTile / kRows; ++i, from += kRows * J.stride, to += kRows * B::kPitch)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  } else if (J.vec) {
+    constexpr int kPer = 16 / Real<TYPE>::kBytes, kVecs = kTile / kPer;  // elements of a vector, vectors of a row
+#pragma unroll 2
     for (int i = 0; i < kTile * kVecs / kThreads; ++i) {
       const int item = i * kThreads + threadIdx.x, r = item / kVecs, v = item % kVecs;
       // bytes of the vector that exist; the others become zeros
@@ -540,87 +590,114 @@ __global__ void __launch_bounds__(kThreads, TYPE == T5E_REAL_BF16 ? 4 : TYPE == 
 
 // ---- back to real values -------------------------------------------------------
 
-// A thread takes 16 codes of four places of the launch at a time, all loaded
+// A thread takes 32 codes of two places of the launch at a time, all loaded
 // before the first is worked on.  Rows of `out` on 16-byte boundaries take
 // vectors; others pass through shared memory, so that the lanes' stores are
-// neighbours.
+// neighbours.  FOLD: 1 / m is a power of two near 1, so its product with the
+// scale is exact and one product per element is enough.
+template <int TYPE, bool E8M0, int BLOCK, bool VEC, bool FOLD>
+__device__ __forceinline__ void open_rows(const uint8_t* __restrict__ data, int64_t data_stride,
+                                          const uint8_t* __restrict__ scales, uint32_t groups, uint32_t rows, uint64_t row0,
+                                          uint32_t k, const Divider& chunks, float back, void* __restrict__ out,
+                                          int64_t out_stride, bool wide, float* turn) {
+  constexpr int kAtOnce = 2, kBlocks = kChunk / BLOCK;
+  const uint32_t total = rows * chunks.d, step = gridDim.x * kThreads;
+  const uint32_t rows_on = divided(step, chunks), chunks_on = step - rows_on * chunks.d;
+  const int lane = threadIdx.x & 31;
+  using T = typename Real<TYPE>::type;
+  scales += scale_offset(row0, 0, groups);  // row0 is a multiple of 128
+  uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u);
+  Walk walk;
+  walk.start(base + lane, chunks);
+  for (; base < total; base += kAtOnce * step) {
+    uint32_t row[kAtOnce], e0[kAtOnce], bytes[kAtOnce];
+    uint4 w[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const bool in = walk.row < rows;
+      row[i] = walk.row;
+      e0[i] = in ? walk.chunk * kChunk : 0x7FFFFFFFu;  // nothing to store
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      bytes[i] = 0u;
+      if (in) {
+        w[i] = __ldg(reinterpret_cast<const uint4*>(data + (int64_t)(row0 + row[i]) * data_stride + e0[i] / 2u));
+        const uint32_t b = e0[i] / BLOCK;
+        const uint8_t* at = scales + ((row[i] >> 7) * groups + (b >> 2)) * 512u + (row[i] & 31u) * 16u +
+                            ((row[i] >> 5) & 3u) * 4u + (b & 3u);
+        if constexpr (BLOCK == 16) bytes[i] = __ldg(reinterpret_cast<const uint16_t*>(at));
+        else bytes[i] = __ldg(at);
+      }
+      walk.advance(rows_on, chunks_on, chunks.d);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (base + i * step >= total) break;
+      float v[32];
+      from_e2m1x8(w[i].x, v);
+      from_e2m1x8(w[i].y, v + 8);
+      from_e2m1x8(w[i].z, v + 16);
+      from_e2m1x8(w[i].w, v + 24);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const float s = scale_value<E8M0>((bytes[i] >> (8 * b)) & 0xFFu);
+        const float f = FOLD ? s * back : s;
+#pragma unroll
+        for (int j = 0; j < BLOCK; ++j) v[b * BLOCK + j] = FOLD ? v[b * BLOCK + j] * f : v[b * BLOCK + j] * f * back;
+      }
+      const int64_t at = (int64_t)(row0 + row[i]) * out_stride + e0[i];
+      if constexpr (VEC) {
+        T* dst = static_cast<T*>(out) + at;
+        if (e0[i] + kChunk <= k) {
+          uint4 o[2 * Real<TYPE>::kBytes];
+          uint32_t* words = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+          for (int j = 0; j < 8 * Real<TYPE>::kBytes; ++j) {
+            if constexpr (TYPE == T5E_REAL_F32) words[j] = __float_as_uint(v[j]);
+            else words[j] = pack2<TYPE>(v[2 * j], v[2 * j + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 2 * Real<TYPE>::kBytes; j += 2)
+            store32(reinterpret_cast<uint4*>(dst) + j, wide, o[j], o[j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j)
+            if (e0[i] + j < k) dst[j] = from_f32<TYPE>(v[j]);
+        }
+      } else {
+        constexpr int kPitch = 36;  // floats of a lane: vectors of a warp meet no bank twice
+        float* mine = turn + threadIdx.x * kPitch;
+        const float* warp = turn + (threadIdx.x & ~31) * kPitch;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          reinterpret_cast<float4*>(mine)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {  // lane j's 32 elements
+          const int64_t place = __shfl_sync(0xFFFFFFFFu, at, j) + lane;
+          if (__shfl_sync(0xFFFFFFFFu, e0[i], j) + lane < k) static_cast<T*>(out)[place] = from_f32<TYPE>(warp[j * kPitch + lane]);
+        }
+      }
+    }
+  }
+}
+
 template <int TYPE, bool E8M0, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_stride,
                                                               const uint8_t* __restrict__ scales, uint32_t groups,
                                                               uint32_t rows, uint64_t row0, uint32_t k, Divider chunks,
                                                               const float* multiplier, void* __restrict__ out,
                                                               int64_t out_stride, bool wide) {
-  constexpr int kAtOnce = 4, kPitch = 20;  // a lane's 16 floats 20 apart: vectors of a warp meet no bank twice
-  __shared__ __align__(16) float turn[VEC ? 4 : kThreads * kPitch];
+  __shared__ __align__(16) float turn[VEC ? 4 : kThreads * 36];
   let_next_grid_start();
   wait_for_previous_grid();
   const float back = multiplier != nullptr ? 1.f / *multiplier : 1.f;
-  const uint32_t total = rows * chunks.d, step = gridDim.x * kThreads;
-  const int lane = threadIdx.x & 31;
-  using T = typename Real<TYPE>::type;
-  for (uint32_t base = blockIdx.x * kThreads + (threadIdx.x & ~31u); base < total; base += kAtOnce * step) {
-    uint32_t row[kAtOnce], e0[kAtOnce], byte[kAtOnce];
-    uint2 w[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const uint32_t item = base + i * step + lane;
-      const bool in = item < total;
-      row[i] = in ? divided(item, chunks) : 0u;
-      e0[i] = in ? (item - row[i] * chunks.d) * 16u : k;  // k: nothing to store
-      if (in) {
-        w[i] = __ldg(reinterpret_cast<const uint2*>(data + (int64_t)(row0 + row[i]) * data_stride + e0[i] / 2u));
-        byte[i] = __ldg(scales + scale_offset(row0 + row[i], e0[i] / BLOCK, groups));
-      } else {
-        w[i] = make_uint2(0u, 0u);
-        byte[i] = 0u;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      if (base + i * step >= total) break;
-      const float s = scale_value<E8M0>(byte[i]);
-      float v[16];
-      from_e2m1x8(w[i].x, v);
-      from_e2m1x8(w[i].y, v + 8);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = v[j] * s * back;
-      const int64_t at = (int64_t)(row0 + row[i]) * out_stride + e0[i];
-      T* dst = static_cast<T*>(out) + at;
-      if constexpr (VEC) {
-        if (e0[i] + 16u <= k) {
-          uint4 o[Real<TYPE>::kBytes];
-          uint32_t* words = reinterpret_cast<uint32_t*>(o);
-#pragma unroll
-          for (int j = 0; j < 4 * Real<TYPE>::kBytes; ++j) {
-            if constexpr (TYPE == T5E_REAL_F32) words[j] = __float_as_uint(v[j]);
-            else words[j] = pack2<TYPE>(v[2 * j], v[2 * j + 1]);
-          }
-#pragma unroll
-          for (int j = 0; j < Real<TYPE>::kBytes; j += 2) store32(reinterpret_cast<uint4*>(dst) + j, wide, o[j], o[j + 1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (e0[i] + j < k) dst[j] = from_f32<TYPE>(v[j]);
-        }
-      } else {
-        float* mine = turn + threadIdx.x * kPitch;
-        const float* warp = turn + (threadIdx.x & ~31) * kPitch;
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          reinterpret_cast<float4*>(mine)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        __syncwarp();
-        // two lanes' 16 elements at a time
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int from = 2 * j + (lane >> 4), element = lane & 15;
-          const int64_t place = __shfl_sync(0xFFFFFFFFu, at, from) + element;
-          const uint32_t first = __shfl_sync(0xFFFFFFFFu, e0[i], from);
-          if (first + element < k) static_cast<T*>(out)[place] = from_f32<TYPE>(warp[from * kPitch + element]);
-        }
-      }
-    }
-  }
+  if (is_narrow<T5E_REAL_BF16, E8M0>(back))
+    open_rows<TYPE, E8M0, BLOCK, VEC, true>(data, data_stride, scales, groups, rows, row0, k, chunks, back, out, out_stride,
+                                            wide, turn);
+  else
+    open_rows<TYPE, E8M0, BLOCK, VEC, false>(data, data_stride, scales, groups, rows, row0, k, chunks, back, out,
+                                             out_stride, wide, turn);
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -655,8 +732,9 @@ unsigned grid_of(uint64_t blocks, unsigned per_sm) {
   return (unsigned)(blocks < cap ? (blocks ? blocks : 1) : cap);
 }
 
-// Rows of one launch: the kernels count chunks of a launch in 32 bits.
-uint64_t rows_per_launch(uint64_t chunks) { return chunks ? (uint64_t(1) << 30) / chunks : 1; }
+// Rows of one launch: the kernels count chunks and scale bytes of a launch in 32
+// bits.  T5E_MAX_BLOCK_K leaves at least 128 rows.
+uint64_t rows_per_launch(uint64_t chunks) { return (uint64_t(1) << 30) / chunks; }
 
 bool rows_aligned(int32_t type, const void* x, uint64_t rows, int64_t stride, unsigned bytes = 16) {
   return reinterpret_cast<uintptr_t>(x) % bytes == 0 && (rows <= 1 || (stride * type_bytes(type)) % bytes == 0);
@@ -672,8 +750,8 @@ constexpr uint32_t kNever = 0xFFFFFFFFu;
 
 int quantize_rows(int32_t type, const Jobs& jobs, const t5e_blocks& out, bool ceil, cudaStream_t stream) {
   const Job& J = jobs.job[0];
-  const Divider chunks = divider(J.row_groups * (uint32_t)(out.scale_block / 4));
-  const uint64_t per = rows_per_launch(chunks.d);
+  const Divider chunks = divider(J.row_groups * (uint32_t)(out.scale_block / 8));
+  const uint64_t per = rows_per_launch(chunks.d) / 128 * 128;
   for (uint64_t row0 = 0; row0 < J.rows; row0 += per) {
     const uint32_t n = (uint32_t)(J.rows - row0 < per ? J.rows - row0 : per);
     const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 6);
@@ -880,9 +958,9 @@ int t5e_dequantize_blocks(const t5e_blocks* b, const float* multiplier, int32_t 
   if (!out || (reinterpret_cast<uintptr_t>(out) & (type_bytes(type) - 1)) || (b->rows > 1 && out_stride < b->k))
     return T5E_ERR_INVALID;
   const uint32_t groups = scale_groups(*b);
-  const Divider chunks = divider((uint32_t)(((uint64_t)b->k + 15) / 16));
+  const Divider chunks = divider((uint32_t)(((uint64_t)b->k + kChunk - 1) / kChunk));
   const bool vec = rows_aligned(type, out, b->rows, out_stride), wide = rows_aligned(type, out, b->rows, out_stride, 32);
-  const uint64_t per = rows_per_launch(chunks.d);
+  const uint64_t per = rows_per_launch(chunks.d) / 128 * 128;
   for (uint64_t row0 = 0; row0 < b->rows; row0 += per) {
     const uint32_t n = (uint32_t)(b->rows - row0 < per ? b->rows - row0 : per);
     const unsigned grid = grid_of(((uint64_t)n * chunks.d + kThreads - 1) / kThreads, 8);
