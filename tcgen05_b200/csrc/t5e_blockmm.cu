@@ -300,6 +300,30 @@ __device__ __forceinline__ void store_results(const Params& P, float alpha, uint
 // own): lane r brings row p + r, columns q .. q + 31; the stores, and the loads
 // of C, then run along the rows, 32 neighbouring elements at a time, whatever
 // the alignment.
+template <int TYPE, bool ADD>
+__device__ __forceinline__ void turned_rows(const Params& P, float alpha, uint32_t p, uint32_t col, int rows,
+                                            const float* column) {
+  using T = typename blocks::Real<TYPE>::type;
+  T* dst = static_cast<T*>(P.d) + (int64_t)p * P.d_stride + col;
+  int64_t from = ADD ? (int64_t)p * P.c_p_stride + (int64_t)col * P.c_q_stride : 0;
+#pragma unroll 1
+  for (int r = 0; r < rows; r += 8) {  // eight rows' loads, then their stores
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = column[(r + j) * 33];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float add = 0.f;
+      if (ADD && r + j < rows) add = read_real(P.c, from + j * P.c_p_stride, P.c_type);
+      x[j] = ADD ? __fmaf_rn(x[j], alpha, add) : x[j] * alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j, dst += P.d_stride)
+      if (r + j < rows) *dst = from_f32<TYPE>(x[j]);
+    from += 8 * P.c_p_stride;
+  }
+}
+
 __device__ __forceinline__ void store_turned(const Params& P, float alpha, uint32_t p, uint32_t q, const float* v,
                                              float* buffer) {
   const int lane = threadIdx.x & 31;
@@ -310,26 +334,32 @@ __device__ __forceinline__ void store_turned(const Params& P, float alpha, uint3
   const uint32_t col = q + lane;
   if (col >= P.q_rows || p >= P.p_rows) return;
   const int rows = P.p_rows - p < 32u ? (int)(P.p_rows - p) : 32;
-#pragma unroll 8
-  for (int r = 0; r < rows; ++r) {
-    float x = buffer[r * 33 + lane];
-    x = P.c != nullptr ? __fmaf_rn(x, alpha, read_real(P.c, (int64_t)(p + r) * P.c_p_stride + (int64_t)col * P.c_q_stride,
-                                                       P.c_type))
-                       : x * alpha;
-    write_real(P.d, (int64_t)(p + r) * P.d_stride + col, P.d_type, x);
+  if (P.c != nullptr) {
+    if (P.d_type == T5E_REAL_F32) turned_rows<T5E_REAL_F32, true>(P, alpha, p, col, rows, buffer + lane);
+    else if (P.d_type == T5E_REAL_BF16) turned_rows<T5E_REAL_BF16, true>(P, alpha, p, col, rows, buffer + lane);
+    else turned_rows<T5E_REAL_F16, true>(P, alpha, p, col, rows, buffer + lane);
+  } else {
+    if (P.d_type == T5E_REAL_F32) turned_rows<T5E_REAL_F32, false>(P, alpha, p, col, rows, buffer + lane);
+    else if (P.d_type == T5E_REAL_BF16) turned_rows<T5E_REAL_BF16, false>(P, alpha, p, col, rows, buffer + lane);
+    else turned_rows<T5E_REAL_F16, false>(P, alpha, p, col, rows, buffer + lane);
   }
 }
 
 // The same results, without C, through a box of 32 rows that TMA writes: rows
 // of 64 bytes (16-bit results) or 128, swizzled as the map says, so that the
-// lanes' 16-byte stores meet no bank twice.  `box` is the box to fill; the
-// caller alternates between two.
+// lanes' 16-byte stores meet no bank twice.  `boxes` are the warp's 4 KB: two
+// boxes of 16-bit results that take turns, or one of F32.
 __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* map, float alpha, uint32_t p, uint32_t q,
-                                          const float* v, uint8_t* box) {
+                                          const float* v, uint8_t* boxes, int turn) {
   const int lane = threadIdx.x & 31;
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the box before the last has been read
+  const bool wide = P.d_type == T5E_REAL_F32;
+  uint8_t* box = wide ? boxes : boxes + (turn & 1) * 2048;
+  if (lane == 0) {  // what was in the box has been read
+    if (wide) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  }
   __syncwarp();
-  if (P.d_type == T5E_REAL_F32) {
+  if (wide) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) =
@@ -379,6 +409,8 @@ __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* ma
 // In a pair (PAIR) both blocks load their own parts, and the first block
 // spreads and issues for both; its barriers count the bytes of both, and its
 // commits arrive in both.
+// STAGES and SCALE_STAGES are the most that the barriers provide for; a launch
+// says how many it has room for (Depth).
 template <bool PAIR_, int BN_, int BLOCK_, int STAGES_, int SCALE_STAGES_, int TMEM_>
 struct Pipe {
   static constexpr bool PAIR = PAIR_;
@@ -394,7 +426,6 @@ struct Pipe {
   static constexpr int kUnitCols = kUnitGroups * 4 * (1 + kQTiles);
   static constexpr int kUnits = 4;
   static constexpr int kScaleCol = kTmem - kUnits * kUnitCols;   // first column of the unit buffers
-  static constexpr int kBytes = STAGES * kStageBytes + SCALE_STAGES * kScaleBytes;
   static constexpr int kBlocks = PAIR ? 2 : 1;
 };
 
@@ -432,13 +463,29 @@ __device__ __forceinline__ void prefetch_maps(const Maps& m) {
   asm volatile("prefetch.tensormap [%0];" :: "l"(&m.qs));
 }
 
-// Waits until the slot of use `n` of a ring of `size` stages has been released
-// by its use before (at once the first time round).
-__device__ __forceinline__ bool wait_slot(uint64_t* empty, uint32_t n, uint32_t size, int* failed) {
-  return barrier_wait(smem_u32(empty + n % size), ((n / size) & 1u) ^ 1u, failed);
+struct Depth {
+  uint32_t stages, scale_stages;
+};
+
+// A role's place in a ring: the slot, the parity of the round, uses so far.
+struct Use {
+  uint32_t slot = 0, parity = 0, count = 0;
+  __device__ __forceinline__ void next(uint32_t size) {
+    ++count;
+    if (++slot == size) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// Waits until the slot has been released by its use before (at once the first
+// time round); until it has been filled.
+__device__ __forceinline__ bool wait_slot(uint64_t* empty, const Use& u, int* failed) {
+  return barrier_wait(smem_u32(empty + u.slot), u.parity ^ 1u, failed);
 }
-__device__ __forceinline__ bool wait_use(uint64_t* full, uint32_t n, uint32_t size, int* failed) {
-  return barrier_wait(smem_u32(full + n % size), (n / size) & 1u, failed);
+__device__ __forceinline__ bool wait_use(uint64_t* full, const Use& u, int* failed) {
+  return barrier_wait(smem_u32(full + u.slot), u.parity, failed);
 }
 
 // Announces `bytes` per block and returns the barrier that the copies arrive
@@ -450,14 +497,14 @@ __device__ __forceinline__ uint32_t announce(uint64_t* full, uint32_t rank, uint
   return S::PAIR ? in_block(bar, 0) : bar;
 }
 
-// Stages first .. last - 1 of a tile; `n` counts the uses of the ring.
+// Stages first .. last - 1 of a tile.
 template <typename S>
-__device__ __forceinline__ bool load_operands(const Maps& m, Barriers<S>& b, uint8_t* ring, uint32_t rank, uint32_t first,
-                                              uint32_t last, int32_t p0, int32_t q0, uint32_t& n, int* failed) {
-  for (uint32_t st = first; st < last; ++st, ++n) {
-    if (!wait_slot(b.empty, n, S::STAGES, failed)) return false;
-    const uint32_t slot = n % S::STAGES, at = smem_u32(ring) + slot * S::kStageBytes;
-    const uint32_t bar = announce<S>(&b.full[slot], rank, S::kStageBytes);
+__device__ __forceinline__ bool load_operands(const Maps& m, Barriers<S>& b, uint8_t* ring, const Depth& depth, uint32_t rank,
+                                              uint32_t first, uint32_t last, int32_t p0, int32_t q0, Use& u, int* failed) {
+  for (uint32_t st = first; st < last; ++st, u.next(depth.stages)) {
+    if (!wait_slot(b.empty, u, failed)) return false;
+    const uint32_t at = smem_u32(ring) + u.slot * S::kStageBytes;
+    const uint32_t bar = announce<S>(&b.full[u.slot], rank, S::kStageBytes);
     load_2d<S::PAIR>(at, &m.p, (int32_t)(st * kRowBytes), p0, bar);
     load_2d<S::PAIR>(at + S::kPBytes, &m.q, (int32_t)(st * kRowBytes), q0, bar);
   }
@@ -465,12 +512,13 @@ __device__ __forceinline__ bool load_operands(const Maps& m, Barriers<S>& b, uin
 }
 
 template <typename S>
-__device__ __forceinline__ bool load_scales(const Maps& m, Barriers<S>& b, uint8_t* ring, uint32_t rank, uint32_t first,
-                                            uint32_t last, int32_t p_tile, int32_t q_tile, uint32_t& n, int* failed) {
-  for (uint32_t st = first; st < last; ++st, ++n) {
-    if (!wait_slot(b.scale_empty, n, S::SCALE_STAGES, failed)) return false;
-    const uint32_t slot = n % S::SCALE_STAGES, at = smem_u32(ring) + slot * S::kScaleBytes;
-    const uint32_t bar = announce<S>(&b.scale_full[slot], rank, S::kScaleBytes);
+__device__ __forceinline__ bool load_scales(const Maps& m, Barriers<S>& b, uint8_t* ring, const Depth& depth, uint32_t rank,
+                                            uint32_t first, uint32_t last, int32_t p_tile, int32_t q_tile, Use& u,
+                                            int* failed) {
+  for (uint32_t st = first; st < last; ++st, u.next(depth.scale_stages)) {
+    if (!wait_slot(b.scale_empty, u, failed)) return false;
+    const uint32_t at = smem_u32(ring) + u.slot * S::kScaleBytes;
+    const uint32_t bar = announce<S>(&b.scale_full[u.slot], rank, S::kScaleBytes);
     load_3d<S::PAIR>(at, &m.ps, 0, (int32_t)(st * S::kGroups), p_tile, bar);
     load_3d<S::PAIR>(at + S::kGroups * 512, &m.qs, 0, (int32_t)(st * S::kGroups), q_tile, bar);
   }
@@ -484,74 +532,75 @@ __device__ __forceinline__ uint32_t steps_in(uint32_t k, uint32_t st) {
 }
 
 template <typename S>
-__device__ __forceinline__ bool spread_scales(Barriers<S>& b, uint8_t* ring, uint32_t tmem, uint32_t k, uint32_t first,
-                                              uint32_t last, uint32_t& n, uint32_t& unit, int* failed) {
-  for (uint32_t st = first; st < last; ++st, ++n) {
-    if (!wait_use(b.scale_full, n, S::SCALE_STAGES, failed)) return false;
-    const uint32_t slot = n % S::SCALE_STAGES, at = smem_u32(ring) + slot * S::kScaleBytes;
+__device__ __forceinline__ bool spread_scales(Barriers<S>& b, uint8_t* ring, const Depth& depth, uint32_t tmem, uint32_t k,
+                                              uint32_t first, uint32_t last, Use& u, Use& unit, int* failed) {
+  for (uint32_t st = first; st < last; ++st, u.next(depth.scale_stages)) {
+    if (!wait_use(b.scale_full, u, failed)) return false;
+    const uint32_t at = smem_u32(ring) + u.slot * S::kScaleBytes;
     const uint32_t steps = steps_in(k, st);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (u * 2 >= (int)steps) break;
-      if (!wait_slot(b.unit_empty, unit, S::kUnits, failed)) return false;
+    for (int half = 0; half < 2; ++half) {
+      if (half * 2 >= (int)steps) break;
+      if (!wait_slot(b.unit_empty, unit, failed)) return false;
       fence_after();
-      const uint32_t to = tmem + S::kScaleCol + unit % S::kUnits * S::kUnitCols;
+      const uint32_t to = tmem + S::kScaleCol + unit.slot * S::kUnitCols;
 #pragma unroll
       for (int g = 0; g < S::kUnitGroups; ++g) {
-        const int from = u * S::kUnitGroups + g;
+        const int from = half * S::kUnitGroups + g;
         copy_scales<S::PAIR>(to + g * 4, at + from * 512);
         // Q's scales of one group side by side: 4 columns per 128 rows
 #pragma unroll
         for (int h = 0; h < S::kQTiles; ++h)
           copy_scales<S::PAIR>(to + (S::kUnitGroups + g * S::kQTiles + h) * 4, at + (S::kGroups * (1 + h) + from) * 512);
       }
-      commit_here<S::PAIR>(smem_u32(&b.unit_full[unit % S::kUnits]));
-      ++unit;
+      commit_here<S::PAIR>(smem_u32(&b.unit_full[unit.slot]));
+      unit.next(S::kUnits);
     }
-    commit_all<S::PAIR>(smem_u32(&b.scale_empty[slot]));
+    commit_all<S::PAIR>(smem_u32(&b.scale_empty[u.slot]));
   }
   return true;
 }
 
 template <typename S>
-__device__ __forceinline__ bool issue_products(Barriers<S>& b, uint8_t* ring, uint32_t acc, uint32_t tmem, uint32_t k,
-                                               uint32_t idesc, uint32_t first, uint32_t last, uint32_t& n, uint32_t& unit,
+__device__ __forceinline__ bool issue_products(Barriers<S>& b, uint8_t* ring, const Depth& depth, uint32_t acc, uint32_t tmem,
+                                               uint32_t k, uint32_t idesc, uint32_t first, uint32_t last, Use& u, Use& unit,
                                                int* failed) {
-  for (uint32_t st = first; st < last; ++st, ++n) {
-    if (!wait_use(b.full, n, S::STAGES, failed)) return false;
-    const uint32_t slot = n % S::STAGES, at = smem_u32(ring) + slot * S::kStageBytes;
+  for (uint32_t st = first; st < last; ++st, u.next(depth.stages)) {
+    if (!wait_use(b.full, u, failed)) return false;
+    const uint32_t at = smem_u32(ring) + u.slot * S::kStageBytes;
     const uint64_t dp = operand_desc(at), dq = operand_desc(at + S::kPBytes);
     const uint32_t steps = steps_in(k, st);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (u * 2 >= (int)steps) break;
-      if (!wait_use(b.unit_full, unit, S::kUnits, failed)) return false;
+    for (int half = 0; half < 2; ++half) {
+      if (half * 2 >= (int)steps) break;
+      if (!wait_use(b.unit_full, unit, failed)) return false;
       fence_after();
-      const uint32_t tsp = tmem + S::kScaleCol + unit % S::kUnits * S::kUnitCols, tsq = tsp + S::kUnitGroups * 4;
+      const uint32_t tsp = tmem + S::kScaleCol + unit.slot * S::kUnitCols, tsq = tsp + S::kUnitGroups * 4;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (u * 2 + j < (int)steps) {
+        if (half * 2 + j < (int)steps) {
           // a column of scales holds four bytes per row: one product's with
           // blocks of 16, two products' (bytes 0-1, 2-3) with blocks of 32
           const int g = S::BLOCK == 16 ? j : 0;
           const uint32_t id = S::BLOCK == 16 ? 0u : (uint32_t)j * 2u;
-          mma<S::PAIR, S::BLOCK>(acc, dp + (u * 2 + j) * 2, dq + (u * 2 + j) * 2, idesc | (id << 4) | (id << 29),
-                                 tsp + g * 4, tsq + g * S::kQTiles * 4, st != first || u + j != 0);
+          mma<S::PAIR, S::BLOCK>(acc, dp + (half * 2 + j) * 2, dq + (half * 2 + j) * 2, idesc | (id << 4) | (id << 29),
+                                 tsp + g * 4, tsq + g * S::kQTiles * 4, st != first || half + j != 0);
         }
       }
-      commit_here<S::PAIR>(smem_u32(&b.unit_empty[unit % S::kUnits]));
-      ++unit;
+      commit_here<S::PAIR>(smem_u32(&b.unit_empty[unit.slot]));
+      unit.next(S::kUnits);
     }
-    commit_all<S::PAIR>(smem_u32(&b.empty[slot]));
+    commit_all<S::PAIR>(smem_u32(&b.empty[u.slot]));
   }
   return true;
 }
 
-// Waits until the last uses of a ring (`n` so far) have been released: no copy
-// into it is in flight then.
-__device__ __forceinline__ bool drain_ring(uint64_t* empty, uint32_t n, uint32_t size) {
+// Waits until the last uses of a ring have been released: no copy into it is in
+// flight then.
+__device__ __forceinline__ bool drain_ring(uint64_t* empty, const Use& u, uint32_t size) {
   bool ok = true;
-  for (uint32_t i = n > size ? n - size : 0u; i < n; ++i) ok &= wait_use(empty, i, size, nullptr);
+  for (uint32_t i = u.count > size ? u.count - size : 0u; i < u.count; ++i)
+    ok &= barrier_wait(smem_u32(empty + i % size), (i / size) & 1u, nullptr);
   return ok;
 }
 
@@ -563,20 +612,28 @@ __device__ __forceinline__ bool drain_ring(uint64_t* empty, uint32_t n, uint32_t
 // shares one tile, each with its part of K; the partial sums meet in shared
 // memory and each block finishes BN / split columns, adding the parts in rank
 // order.
+//
+// Depth of the rings: half of the shared memory where two blocks share an SM,
+// all of it where there are no more blocks than SMs; a row of tiles that streams
+// a weight matrix past a few rows is bound by the bytes in flight.
 template <int BN, int BLOCK>
 struct TileShape {
-  static constexpr int kScaleStages = 3;
-  static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * 2;
-  static constexpr int kStages = (110 * 1024 - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN * kRowBytes);
-  using Pipe = blockmm::Pipe<false, BN, BLOCK, kStages, kScaleStages, BN <= 64 ? 128 : 256>;
-  static constexpr int kSmem = Pipe::kBytes + 1024;  // two blocks fit an SM
-  static_assert(kStages * Pipe::kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
+  static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * 2, kStageBytes = (128 + BN) * kRowBytes;
+  static constexpr int kHalf = 110 * 1024, kWhole = 222 * 1024;
+  static constexpr uint32_t kScaleStages = 3, kDeepScaleStages = 8;
+  static constexpr uint32_t kStages = (kHalf - kScaleStages * kScaleBytes) / kStageBytes;
+  static constexpr uint32_t kDeepStages = (kWhole - kDeepScaleStages * kScaleBytes) / kStageBytes;
+  using Pipe = blockmm::Pipe<false, BN, BLOCK, kDeepStages, kDeepScaleStages, BN <= 64 ? 128 : 256>;
+  static constexpr int kSmem = kHalf + 1024, kDeepSmem = kWhole + 1024;
+  static_assert(Pipe::kStageBytes == kStageBytes && Pipe::kScaleBytes == kScaleBytes, "sizes");
+  static_assert(kStages * kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
   static_assert(Pipe::kScaleCol >= BN, "accumulators and scales share tensor memory");
 };
 
 struct TileParams {
   Maps maps;
   Params r;
+  Depth depth;
 };
 
 template <int BN, int BLOCK, bool SWAP>
@@ -590,7 +647,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   __shared__ int failed;
   const int t = threadIdx.x, warp = warp_index();
   uint8_t* stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* scale_stages = stages + S::STAGES * S::kStageBytes;
+  uint8_t* scale_stages = stages + T.depth.stages * S::kStageBytes;
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmem));
@@ -616,18 +673,19 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   const uint32_t last = (uint32_t)((uint64_t)P.stages * (rank + 1) / split);
   bool ok = true;
   if (elected()) {
-    uint32_t n = 0, unit = 0;
+    Use u, unit;
     if (warp == 0) {
-      ok = load_operands<S>(T.maps, bars, stages, 0, first, last, (int32_t)p0, (int32_t)q0, n, &failed);
-      ok &= drain_ring(bars.empty, n, S::STAGES);
+      ok = load_operands<S>(T.maps, bars, stages, T.depth, 0, first, last, (int32_t)p0, (int32_t)q0, u, &failed);
+      ok &= drain_ring(bars.empty, u, T.depth.stages);
     } else if (warp == 1) {
-      ok = issue_products<S>(bars, stages, tmem, tmem, P.k, P.idesc, first, last, n, unit, &failed);
+      ok = issue_products<S>(bars, stages, T.depth, tmem, tmem, P.k, P.idesc, first, last, u, unit, &failed);
       commit_here<false>(smem_u32(&finished));  // after a wait that ran out too: what was issued completes
     } else if (warp == 2) {
-      ok = load_scales<S>(T.maps, bars, scale_stages, 0, first, last, (int32_t)(p0 >> 7), (int32_t)(q0 >> 7), n, &failed);
-      ok &= drain_ring(bars.scale_empty, n, S::SCALE_STAGES);
+      ok = load_scales<S>(T.maps, bars, scale_stages, T.depth, 0, first, last, (int32_t)(p0 >> 7), (int32_t)(q0 >> 7), u,
+                          &failed);
+      ok &= drain_ring(bars.scale_empty, u, T.depth.scale_stages);
     } else {
-      ok = spread_scales<S>(bars, scale_stages, tmem, P.k, first, last, n, unit, &failed);
+      ok = spread_scales<S>(bars, scale_stages, T.depth, tmem, P.k, first, last, u, unit, &failed);
     }
   }
   __syncwarp();
@@ -714,7 +772,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
 // block holds its 128 rows of A and half of B's rows, so B crosses shared
 // memory once for both, and accumulates its 128 x BN part in its own tensor
 // memory.  The blocks are persistent (tile = cluster, cluster + clusters, ...)
-// and specialised: four warps are the pipeline's roles, four take results out,
+// and specialised: four warps are the pipeline's roles, eight take results out,
 // so that the results of a tile leave while the next one is computed.
 //
 // Tensor memory (512 columns): two accumulators of BN columns and the unit
@@ -724,11 +782,11 @@ template <int BN, int BLOCK>
 struct PairShape {
   static constexpr int kScaleStages = 4;
   static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * (1 + BN / 128);
-  static constexpr int kBoxBytes = 8192;  // a results warp's shared memory: two boxes, or the 32 x 33 buffer
+  static constexpr int kBoxBytes = 5120;  // a results warp's shared memory: its boxes, or the 32 x 33 buffer
   static constexpr int kStages =
-      (226 * 1024 - 1024 - 4 * kBoxBytes - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN / 2 * kRowBytes);
+      (226 * 1024 - 1024 - 8 * kBoxBytes - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN / 2 * kRowBytes);
   using Pipe = blockmm::Pipe<true, BN, BLOCK, kStages, kScaleStages, 512>;
-  static constexpr int kSmem = Pipe::kBytes + 4 * kBoxBytes + 1024;
+  static constexpr int kSmem = kStages * Pipe::kStageBytes + kScaleStages * Pipe::kScaleBytes + 8 * kBoxBytes + 1024;
   static constexpr int kSecond = BN <= 128 ? BN : (Pipe::kScaleCol - BN) / 32 * 32;  // column of the second accumulator
   static constexpr int kShared = BN - kSecond;  // columns both use (0: none)
   static_assert(kSecond + BN <= Pipe::kScaleCol && kShared % 32 == 0 && kShared >= 0, "tensor memory");
@@ -742,7 +800,7 @@ struct PairParams {
   int32_t boxed;  // results leave through d_map: rows on 16-byte boundaries, no C
 };
 
-constexpr int kPairThreads = 256;  // warps 0-3 the roles, 4-7 the results
+constexpr int kPairThreads = 384;  // warps 0-3 the roles, 4-11 the results: two warps for each 32 rows
 
 template <int BN, int BLOCK>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pair_kernel(const __grid_constant__ PairParams P) {
@@ -756,7 +814,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
   const int t = threadIdx.x, warp = warp_index(), lane = t & 31;
   const uint32_t rank = cluster_rank();
   uint8_t* boxes = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* stages = boxes + 4 * L::kBoxBytes;
+  uint8_t* stages = boxes + 8 * L::kBoxBytes;
   uint8_t* scale_stages = stages + S::STAGES * S::kStageBytes;
   if (warp == 4) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -767,7 +825,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
     init_barriers(bars);
     for (int i = 0; i < 2; ++i) {
       barrier_init(smem_u32(&acc_full[i]), 1);
-      barrier_init(smem_u32(&acc_free[i]), 8);  // four warps of each block
+      barrier_init(smem_u32(&acc_free[i]), 16);  // eight warps of each block
     }
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -783,17 +841,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
   bool ok = true;
   if (warp < 4) {
     if ((rank == 0 || warp == 0 || warp == 2) && elected()) {
-      uint32_t n = 0, unit = 0, count = 0;
+      constexpr Depth depth = {S::STAGES, S::SCALE_STAGES};
+      Use u, unit;
+      uint32_t count = 0;
       for (uint32_t tile = blockIdx.x / 2; ok && tile < tiles; tile += clusters, ++count) {
         const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
         const int32_t p0 = (int32_t)(pt * 256u + rank * 128u), q0 = (int32_t)(qt * BN + rank * (BN / 2));
         if (warp == 0) {
-          ok = load_operands<S>(P.maps, bars, stages, rank, 0, stage_count, p0, q0, n, &failed);
+          ok = load_operands<S>(P.maps, bars, stages, depth, rank, 0, stage_count, p0, q0, u, &failed);
         } else if (warp == 2) {
-          ok = load_scales<S>(P.maps, bars, scale_stages, rank, 0, stage_count, p0 >> 7, (int32_t)(qt * S::kQTiles), n,
-                              &failed);
+          ok = load_scales<S>(P.maps, bars, scale_stages, depth, rank, 0, stage_count, p0 >> 7, (int32_t)(qt * S::kQTiles),
+                              u, &failed);
         } else if (warp == 3) {
-          ok = spread_scales<S>(bars, scale_stages, tmem, P.r.k, 0, stage_count, n, unit, &failed);
+          ok = spread_scales<S>(bars, scale_stages, depth, tmem, P.r.k, 0, stage_count, u, unit, &failed);
         } else {
           // the columns shared with the tile before are free (and all of the
           // one before that, whose results were taken out first), or without
@@ -805,19 +865,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
             if (!ok) break;
             fence_after();
           }
-          ok = issue_products<S>(bars, stages, tmem + (count & 1u) * L::kSecond, tmem, P.r.k, P.r.idesc, 0, stage_count, n,
-                                 unit, &failed);
+          ok = issue_products<S>(bars, stages, depth, tmem + (count & 1u) * L::kSecond, tmem, P.r.k, P.r.idesc, 0,
+                                 stage_count, u, unit, &failed);
           if (ok) commit_all<true>(smem_u32(&acc_full[count & 1u]));  // if not, the results' waits run out too
         }
       }
-      if (warp == 0) ok &= drain_ring(bars.empty, n, S::STAGES);
-      if (warp == 2) ok &= drain_ring(bars.scale_empty, n, S::SCALE_STAGES);
+      if (warp == 0) ok &= drain_ring(bars.empty, u, S::STAGES);
+      if (warp == 2) ok &= drain_ring(bars.scale_empty, u, S::SCALE_STAGES);
     }
   } else {
     const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
     const float alpha = P.r.alpha * (P.r.multiplier_a != nullptr ? 1.f / *P.r.multiplier_a : 1.f) *
                         (P.r.multiplier_b != nullptr ? 1.f / *P.r.multiplier_b : 1.f);
-    uint8_t* box = boxes + quarter * L::kBoxBytes;
+    const int side = warp >= 8;     // of the two warps of these lanes: every other chunk
+    uint8_t* box = boxes + (quarter * 2 + side) * L::kBoxBytes;
     uint32_t count = 0;
     for (uint32_t tile = blockIdx.x / 2; ok && tile < tiles; tile += clusters, ++count) {
       const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
@@ -837,7 +898,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
         const uint32_t q = q0 + chunk * 32;
-        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box + (turn & 1) * 4096);
+        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box, turn);
         else store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
       };
       auto release = [&] {
@@ -846,22 +907,26 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
         if (lane == 0) arrive_in(free_bar);
       };
       const int first_shared = (count & 1u) == 0u ? kChunks - kFirst : 0, first_own = (count & 1u) == 0u ? 0 : kFirst;
+      int turn = 0;
       if constexpr (kFirst > 0) {
-        float head[kFirst * 32];
+        constexpr int kHead = (kFirst + 1) / 2;  // of one warp at most
+        float head[kHead * 32];
 #pragma unroll
-        for (int i = 0; i < kFirst; ++i) load_acc32(acc + (first_shared + i) * 32, head + i * 32);
+        for (int i = 0; i < kHead; ++i)
+          if (2 * i + side < kFirst) load_acc32(acc + (first_shared + 2 * i + side) * 32, head + i * 32);
         acc_loaded();
         release();
 #pragma unroll
-        for (int i = 0; i < kFirst; ++i) finish(first_shared + i, i, head + i * 32);
+        for (int i = 0; i < kHead; ++i)
+          if (2 * i + side < kFirst) finish(first_shared + 2 * i + side, turn++, head + i * 32);
       }
 #pragma unroll 1
-      for (int i = kFirst; i < kChunks; ++i) {
+      for (int i = side; i < kChunks - kFirst; i += 2) {
         float v[32];
-        load_acc32(acc + (first_own + i - kFirst) * 32, v);
+        load_acc32(acc + (first_own + i) * 32, v);
         acc_loaded();
-        if (kFirst == 0 && i == kChunks - 1) release();
-        finish(first_own + i - kFirst, i, v);
+        if (kFirst == 0 && i + 2 >= kChunks) release();
+        finish(first_own + i, turn++, v);
       }
     }
     if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -989,15 +1054,17 @@ int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, 
   TileParams P;
   P.r = params;
   int rc = encode_maps<typename S::Pipe>(&P.maps, p, q);
-  if (rc == T5E_OK) rc = raise_smem_limit<tile_kernel<BN, BLOCK, SWAP>>(S::kSmem, "block product attribute");
+  if (rc == T5E_OK) rc = raise_smem_limit<tile_kernel<BN, BLOCK, SWAP>>(S::kDeepSmem, "block product attribute");
   if (rc != T5E_OK) return rc;
   P.r.idesc = instruction(p, BN);
   cudaLaunchConfig_t cfg = {};
   const uint64_t grid = ((p.rows + 127) / 128) * ((q.rows + BN - 1) / BN) * split;
   if (grid > 0x7FFFFFFFull) return T5E_ERR_INVALID;
+  const bool deep = grid <= (uint64_t)sm_count();
+  P.depth = deep ? Depth{S::kDeepStages, S::kDeepScaleStages} : Depth{S::kStages, S::kScaleStages};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.dynamicSmemBytes = deep ? S::kDeepSmem : S::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
