@@ -418,8 +418,8 @@ int t5e_dequantize_blocks(const t5e_blocks* blocks, const float* multiplier, int
  * t5e_block_scaled_mm_expired reports it.
  */
 typedef struct t5e_block_mm {
-    const t5e_blocks* a;
-    const t5e_blocks* b;
+    t5e_blocks a;
+    t5e_blocks b;
     const float* multiplier_a;   /* device scalars or NULL (1) */
     const float* multiplier_b;
     float alpha;

@@ -150,8 +150,8 @@ class BlockMm(ctypes.Structure):
     """t5e_block_mm: one product of block-scaled rows."""
 
     _fields_ = [
-        ("a", ctypes.c_void_p),  # addresses of Blocks
-        ("b", ctypes.c_void_p),
+        ("a", Blocks),
+        ("b", Blocks),
         ("multiplier_a", ctypes.c_void_p),
         ("multiplier_b", ctypes.c_void_p),
         ("alpha", ctypes.c_float),
@@ -165,6 +165,12 @@ class BlockMm(ctypes.Structure):
         ("d_stride", ctypes.c_int64),
     ]
 
+
+# The same structs for struct.pack, which fills one in a fraction of the time a
+# ctypes.Structure takes: a small call's time is the host's.
+BLOCKS_FORMAT = "PqPQqii"
+QUANTIZE_FORMAT = "PQQqiiPPii" + 2 * BLOCKS_FORMAT
+BLOCK_MM_FORMAT = 2 * BLOCKS_FORMAT + "PPfiPiiqqPq"
 
 # every symbol include/t5e.h declares
 EXPORTED = (
@@ -249,10 +255,10 @@ def load() -> ctypes.CDLL:
     lib.t5e_quantize_blocks.restype = ctypes.c_int
     lib.t5e_quantize_blocks.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
     lib.t5e_dequantize_blocks.restype = ctypes.c_int
-    lib.t5e_dequantize_blocks.argtypes = [ctypes.POINTER(Blocks), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+    lib.t5e_dequantize_blocks.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
                                           ctypes.c_int64, ctypes.c_void_p]
     lib.t5e_block_scaled_mm.restype = ctypes.c_int
-    lib.t5e_block_scaled_mm.argtypes = [ctypes.POINTER(BlockMm), ctypes.c_void_p]
+    lib.t5e_block_scaled_mm.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     lib.t5e_block_scaled_mm_expired.restype = ctypes.c_int
     lib.t5e_block_scaled_mm_expired.argtypes = [ctypes.POINTER(ctypes.c_int32)]
     version = lib.t5e_abi_version()

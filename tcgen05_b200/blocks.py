@@ -19,7 +19,7 @@ CPU fallback.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -34,6 +34,10 @@ _FORMS = {
     ("ue8m0", 2): (nat.SCALE_UE8M0, 32),
     ("ue8m0", 4): (nat.SCALE_UE8M0, 16),
 }
+_pack_blocks = struct.Struct(nat.BLOCKS_FORMAT).pack
+_pack_quantize = struct.Struct(nat.QUANTIZE_FORMAT).pack
+_pack_mm = struct.Struct(nat.BLOCK_MM_FORMAT).pack
+_NO_BLOCKS = (0, 0, 0, 0, 0, 0, 0)
 _ROUNDINGS = {"nearest": nat.SCALE_ROUND_NEAREST, "floor": nat.SCALE_ROUND_FLOOR, "ceil": nat.SCALE_ROUND_CEIL}
 
 
@@ -85,7 +89,7 @@ class BlockScaledRows:
     multiplied by before rounding, or None: element i of row r stands for
     code * scale / multiplier."""
 
-    __slots__ = ("rows", "k", "scaling", "scale_vec", "device", "multiplier", "_data", "_scales", "_buffer", "_struct")
+    __slots__ = ("rows", "k", "scaling", "scale_vec", "device", "multiplier", "_data", "_scales", "_buffer", "_fields")
 
     def __init__(self, data, scales, k: int, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
         scaling, scale_vec = _form(scaling, scale_vec)
@@ -114,24 +118,23 @@ class BlockScaledRows:
         self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
         self.device, self.multiplier = data.device, multiplier
         self._data, self._scales, self._buffer = data, scales, None
-        self._struct = nat.Blocks(at, stride, scales_at, rows, k, fmt, block)
+        self._fields = (at, stride, scales_at, rows, k, fmt, block)  # t5e_blocks
 
     @classmethod
-    def _within(cls, buffer, rows, k, scaling, scale_vec, multiplier):
-        """An instance over one uint8 buffer (a new one if None): the rows, then
-        the scale tiles.  The views are made when they are asked for."""
+    def _new(cls, device, rows, k, scaling, scale_vec, multiplier):
+        """An instance over one new allocation: the rows, then the scale tiles.
+        The views are made when they are asked for."""
         self = cls.__new__(cls)
         fmt, block = _FORMS[scaling, scale_vec]
         stride = (k + 31) // 32 * 16
-        if not isinstance(buffer, torch.Tensor):
-            buffer = torch.empty(rows * stride + (rows + 127) // 128 * (-(-k // (4 * block)) * 512), dtype=torch.uint8,
-                                 device=buffer)
+        size = rows * stride
+        self._buffer = buffer = torch.empty(size + (rows + 127) // 128 * (-(-k // (4 * block)) * 512), dtype=torch.uint8,
+                                            device=device)
         self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
-        self.device, self.multiplier = buffer.device, multiplier
+        self.device, self.multiplier = device, multiplier
         self._data = self._scales = None
-        self._buffer = buffer
         at = buffer.data_ptr()
-        self._struct = nat.Blocks(at, stride, at + rows * stride, rows, k, fmt, block)
+        self._fields = (at, stride, at + size, rows, k, fmt, block)
         return self
 
     @classmethod
@@ -156,21 +159,21 @@ class BlockScaledRows:
     @property
     def data(self) -> torch.Tensor:
         if self._data is None:
-            stride = self._struct.stride
+            stride = self._fields[1]
             self._data = self._buffer[:self.rows * stride].view(self.rows, stride)
         return self._data
 
     @property
     def scales(self) -> torch.Tensor:
         if self._scales is None:
-            self._scales = self._buffer[self.rows * self._struct.stride:].view(
+            self._scales = self._buffer[self.rows * self._fields[1]:].view(
                 (self.rows + 127) // 128, -(-self.k // (4 * self.block)), 512)
         return self._scales
 
     @property
     def block(self) -> int:
         """Elements per scale."""
-        return self._struct.scale_block
+        return self._fields[6]
 
     def packed(self) -> PackedRows:
         """The codes as the emulator's operand rows."""
@@ -185,25 +188,17 @@ class BlockScaledRows:
                 f"device={self.device})")
 
 
-class _On:
-    """Makes the device of index `index` current for a library call, and gives
-    its current stream."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
+def _call(fn, index, *args):
+    """A library call on the current stream of the device of index `index`, which
+    is made current for it."""
+    if torch._C._cuda_getDevice() == index:
         # torch.cuda.current_stream(index).cuda_stream, without building a Stream
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        nat.check(rc, fn.__name__)
 
 
 def _real_tensor(x, name: str):
@@ -216,16 +211,18 @@ def _real_tensor(x, name: str):
 
 
 def _matrix_of(x):
-    """(matrix, turned): x as rows of its last dimension with unit column
+    """(matrix, stride, turned): x as rows of its last dimension with unit column
     stride, or `turned`, the matrix whose columns those rows are (no copy of a
     transposed matrix); other layouts are copied."""
-    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    rows, cols = m.shape
-    if (m.stride(1) == 1 or cols == 1) and (rows == 1 or m.stride(0) >= cols):
-        return m, False
-    if m.stride(0) == 1 and m.stride(1) >= rows:
-        return m.t(), True
-    return m.contiguous(), False
+    if x.dim() != 2:
+        x = x.detach().reshape(-1, x.shape[-1])
+    rows, cols = x.shape
+    down, across = x.stride()
+    if (across == 1 or cols == 1) and (rows == 1 or down >= cols):
+        return x, rows, cols, down, False
+    if down == 1 and across >= rows:
+        return x, cols, rows, across, True
+    return x.detach().contiguous(), rows, cols, cols, False
 
 
 def _partial_count(n: int) -> int:
@@ -244,15 +241,14 @@ def block_multiplier(x) -> torch.Tensor:
     if x.dim() == 0:
         x = x.reshape(1)
     lib = nat.load()
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return torch.ones(1, dtype=torch.float32, device=x.device)
-    with _On(x.device.index) as handle:
-        m, _ = _matrix_of(x.detach())
-        count = _partial_count(m.numel())
-        work = torch.empty(1 + count, dtype=torch.float32, device=m.device)
-        at = work.data_ptr()
-        nat.check(lib.t5e_block_multiplier(_REAL[m.dtype], m.data_ptr(), m.shape[0], m.shape[1], m.stride(0), at + 4,
-                                           count, at, handle), "t5e_block_multiplier")
+    m, rows, cols, stride, _ = _matrix_of(x)
+    count = _partial_count(n)
+    work = torch.empty(1 + count, dtype=torch.float32, device=m.device)
+    at = work.data_ptr()
+    _call(lib.t5e_block_multiplier, x.device.index, _REAL[m.dtype], m.data_ptr(), rows, cols, stride, at + 4, count, at)
     return work[:1]
 
 
@@ -301,38 +297,34 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
     return _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier)
 
 
-_NO_BLOCKS = nat.Blocks()
-
-
 def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier):
     """quantize_blocks of checked arguments, x as r rows of k: the rows, the
     columns or the pair."""
-    lib = nat.load()
     device = x.device
-    with _On(device.index) as handle:
-        m, turned = _matrix_of(x.detach())
-        partials, count, at = None, 0, None
-        if multiplier is not None:
-            if isinstance(multiplier, str):
-                multiplier = None
-                if r:
-                    count = _partial_count(r * k)
-                    work = torch.empty(1 + count, dtype=torch.float32, device=device)
-                    at = work.data_ptr()
-                    partials, multiplier = at + 4, work[:1]
-            else:
-                if not isinstance(multiplier, torch.Tensor):
-                    multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
-                at = multiplier.data_ptr()
-        rows = BlockScaledRows._within(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
-        cols = BlockScaledRows._within(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
-        if r:
-            along, across = (cols, rows) if turned else (rows, cols)
-            shape = m.shape
-            nat.check(lib.t5e_quantize_blocks(ctypes.byref(nat.Quantize(
-                m.data_ptr(), shape[0], shape[1], m.stride(0), _REAL[m.dtype], rounding, at, partials, count, 0,
-                _NO_BLOCKS if along is None else along._struct, _NO_BLOCKS if across is None else across._struct)),
-                1, handle), "t5e_quantize_blocks")
+    partials = count = at = 0
+    if multiplier is not None:
+        if isinstance(multiplier, str):
+            multiplier = None
+            if r:
+                count = _partial_count(r * k)
+                work = torch.empty(1 + count, dtype=torch.float32, device=device)
+                at = work.data_ptr()
+                partials, multiplier = at + 4, work[:1]
+        else:
+            if not isinstance(multiplier, torch.Tensor):
+                multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
+            at = multiplier.data_ptr()
+    rows = BlockScaledRows._new(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
+    cols = BlockScaledRows._new(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
+    if r:
+        m, m_rows, m_cols, stride, turned = _matrix_of(x)
+        along = _NO_BLOCKS if rows is None else rows._fields
+        across = _NO_BLOCKS if cols is None else cols._fields
+        if turned:
+            along, across = across, along
+        _call(nat.load().t5e_quantize_blocks, device.index,
+              _pack_quantize(m.data_ptr(), m_rows, m_cols, stride, _REAL[m.dtype], rounding, at, partials, count, 0, *along,
+                             *across), 1)
     if by_rows and by_cols:
         return rows, cols
     return rows if by_rows else cols
@@ -365,13 +357,12 @@ def dequantize_blocks(blocks: BlockScaledRows, *, dtype=torch.float32, out=None)
     _check_blocks(blocks, "blocks")
     if dtype not in _REAL:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    given = out is not None
     out = _result(out, (blocks.rows, blocks.k), dtype, blocks.device)
-    lib = nat.load()
-    with _On(blocks.device.index) as handle:
-        m = blocks.multiplier
-        nat.check(lib.t5e_dequantize_blocks(ctypes.byref(blocks._struct), None if m is None else m.data_ptr(),
-                                            _REAL[dtype], out.data_ptr(), out.stride(0) if blocks.rows > 1 else blocks.k,
-                                            handle), "t5e_dequantize_blocks")
+    m = blocks.multiplier
+    _call(nat.load().t5e_dequantize_blocks, blocks.device.index, _pack_blocks(*blocks._fields),
+          None if m is None else m.data_ptr(), _REAL[dtype], out.data_ptr(),
+          out.stride(0) if given and blocks.rows > 1 else blocks.k)
     return out
 
 
@@ -428,66 +419,44 @@ def _mm(a, b, c, alpha, dtype, out, form):
                                                          zip(shape, c.stride(), out.stride()))
         if c0 < d1 and d0 < c1 and not same:
             raise ValueError("c overlaps out without being out")
-    lib = nat.load()
-    mm = nat.BlockMm(
-        ctypes.addressof(a._struct), ctypes.addressof(b._struct), None if a.multiplier is None else a.multiplier.data_ptr(),
-        None if b.multiplier is None else b.multiplier.data_ptr(), alpha, form, None, 0, _REAL[dtype], 0, 0,
-        out.data_ptr(), out.stride(0) if given and shape[0] > 1 else shape[1])
-    if c is not None:
-        mm.c, mm.c_type = c.data_ptr(), _REAL[c.dtype]
-        mm.c_row_stride, mm.c_col_stride = c.stride()
-    with _On(a.device.index) as handle:
-        nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
+    ma, mb = a.multiplier, b.multiplier
+    c_at, c_type, c_rows, c_cols = (0, 0, 0, 0) if c is None else (c.data_ptr(), _REAL[c.dtype], *c.stride())
+    _call(nat.load().t5e_block_scaled_mm, a.device.index,
+          _pack_mm(*a._fields, *b._fields, 0 if ma is None else ma.data_ptr(), 0 if mb is None else mb.data_ptr(), alpha, form,
+                   c_at, c_type, _REAL[dtype], c_rows, c_cols, out.data_ptr(),
+                   out.stride(0) if given and shape[0] > 1 else shape[1]))
     return out
 
 
-class _Space:
-    """One allocation for several parts: sizes are added up first, the addresses
-    hold once it is made."""
-
-    __slots__ = ("size", "buffer", "at")
-
-    def __init__(self, at: int = 0):
-        self.size = at
-
-    def take(self, n: int) -> int:
-        """Offset of n more bytes."""
-        at = self.size
-        self.size = (at + n + 255) // 256 * 256
-        return at
-
-    def blocks(self, rows: int, k: int, scaling, scale_vec):
-        """(offset, unfinished t5e_blocks) of rows with their scales."""
-        fmt, block = _FORMS[scaling, scale_vec]
-        stride = (k + 31) // 32 * 16
-        return self.take(rows * stride + (rows + 127) // 128 * (-(-k // (4 * block)) * 512)), \
-            nat.Blocks(0, stride, rows * stride, rows, k, fmt, block)
+def _part(at, rows, k, fmt, block):
+    """(t5e_blocks fields without an address, offset, end) of rows with their
+    scales at an offset of an allocation."""
+    stride = (k + 31) // 32 * 16
+    size = rows * stride
+    end = at + size + (rows + 127) // 128 * (-(-k // (4 * block)) * 512)
+    return (at, stride, at + size, rows, k, fmt, block), (end + 255) // 256 * 256
 
 
-def _placed(part, base: int) -> nat.Blocks:
-    """The t5e_blocks of a `_Space.blocks` part of the allocation at `base`."""
-    at, b = part
-    b.data = base + at
-    b.scales = base + at + b.rows * b.stride
-    return b
+def _placed(part, base):
+    """The fields of a part of the allocation at `base`."""
+    at, stride, scales, rows, k, fmt, block = part
+    return base + at, stride, base + scales, rows, k, fmt, block
 
 
-def _quantize_job(x, form, at, partials, count, rows, cols):
-    m, turned = _matrix_of(x)
+def _job(x, rounding, multiplier, partials, count, rows, cols):
+    """(a tensor that has to live until the launch, t5e_quantize)."""
+    m, m_rows, m_cols, stride, turned = _matrix_of(x)
     if turned:
         rows, cols = cols, rows
-    shape = m.shape
-    # the matrix is returned too: a copy of it has to live until the launch
-    return m, nat.Quantize(m.data_ptr(), shape[0], shape[1], m.stride(0), _REAL[m.dtype], form[2], at, partials, count, 0,
-                           _NO_BLOCKS if rows is None else rows, _NO_BLOCKS if cols is None else cols)
+    return m, _pack_quantize(m.data_ptr(), m_rows, m_cols, stride, _REAL[m.dtype], rounding, multiplier, partials, count, 0,
+                             *rows, *cols)
 
 
-def _product(lib, a, b, ma, mb, shape, dtype, device, handle):
-    """block_scaled_mm of t5e_blocks."""
-    out = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
-    mm = nat.BlockMm(ctypes.addressof(a), ctypes.addressof(b), ma, mb, 1.0, 0, None, 0, _REAL[dtype], 0, 0, out.data_ptr(),
-                     shape[1])
-    nat.check(lib.t5e_block_scaled_mm(ctypes.byref(mm), handle), "t5e_block_scaled_mm")
+def _product(a, b, ma, mb, rows, cols, dtype, device):
+    """block_scaled_mm of t5e_blocks fields."""
+    out = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+    _call(nat.load().t5e_block_scaled_mm, device.index,
+          _pack_mm(*a, *b, ma, mb, 1.0, 0, 0, 0, _REAL[dtype], 0, 0, out.data_ptr(), cols))
     return out
 
 
@@ -499,38 +468,35 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, scaling, scale_vec, rounding, need_x, need_w):
-        (n, k), tokens = w.shape, x.numel() // w.shape[1]
-        ctx.shapes = x.shape, w.shape
+        (n, k), tokens, device = w.shape, x.numel() // w.shape[1], x.device
+        ctx.shapes = x.shape, n, k
         if not tokens:
             ctx.form = None
             return x.new_empty((*x.shape[:-1], n))
-        form = ctx.form = (scaling, scale_vec, rounding)
+        fmt, block = _FORMS[scaling, scale_vec]
         auto = scaling == "ue4m3"
-        # blocks run along the contraction: K here, the tokens and N in the
+        ctx.form = rounding, auto, fmt, block
+        # Blocks run along the contraction: K here, the tokens and N in the
         # gradients, so what a gradient needs is rounded along the other axis.
-        # Kept for the backward pass: the multipliers, then the columns
-        kept = _Space(256)
-        xt = kept.blocks(k, tokens, scaling, scale_vec) if need_w else None
-        wt = kept.blocks(k, n, scaling, scale_vec) if need_x else None
-        passing = _Space()
-        xr, wr = passing.blocks(tokens, k, scaling, scale_vec), passing.blocks(n, k, scaling, scale_vec)
+        # Kept for the backward pass: the multipliers, then the columns.
+        xt = wt = None
+        end = 256
+        if need_w:
+            xt, end = _part(end, k, tokens, fmt, block)
+        if need_x:
+            wt, end = _part(end, k, n, fmt, block)
+        keep = torch.empty(end, dtype=torch.uint8, device=device)
+        xr, end = _part(0, tokens, k, fmt, block)
+        wr, partials = _part(end, n, k, fmt, block)
         x_count, w_count = (_partial_count(tokens * k), _partial_count(n * k)) if auto else (0, 0)
-        partials = passing.take(4 * (x_count + w_count))
-        device = x.device
-        lib = nat.load()
-        with _On(device.index) as handle:
-            keep = torch.empty(kept.size, dtype=torch.uint8, device=device)
-            work = torch.empty(passing.size, dtype=torch.uint8, device=device)
-            base, there = keep.data_ptr(), work.data_ptr()
-            xr, wr = _placed(xr, there), _placed(wr, there)
-            partials += there
-            mx, mw = (base, base + 4) if auto else (None, None)
-            x1, jx = _quantize_job(x, form, mx, partials if auto else None, x_count, xr,
-                                   None if xt is None else _placed(xt, base))
-            w1, jw = _quantize_job(w, form, mw, partials + 4 * x_count if auto else None, w_count, wr,
-                                   None if wt is None else _placed(wt, base))
-            nat.check(lib.t5e_quantize_blocks((nat.Quantize * 2)(jx, jw), 2, handle), "t5e_quantize_blocks")
-            y = _product(lib, xr, wr, mx, mw, (tokens, n), x.dtype, device, handle)
+        work = torch.empty(partials + 4 * (x_count + w_count), dtype=torch.uint8, device=device)
+        base, there = keep.data_ptr(), work.data_ptr()
+        xr, wr = _placed(xr, there), _placed(wr, there)
+        mx, mw, px, pw = (base, base + 4, there + partials, there + partials + 4 * x_count) if auto else (0, 0, 0, 0)
+        x1, x_job = _job(x, rounding, mx, px, x_count, xr, _NO_BLOCKS if xt is None else _placed(xt, base))
+        w1, w_job = _job(w, rounding, mw, pw, w_count, wr, _NO_BLOCKS if wt is None else _placed(wt, base))
+        _call(nat.load().t5e_quantize_blocks, device.index, x_job + w_job, 2)
+        y = _product(xr, wr, mx, mw, tokens, n, x.dtype, device)
         ctx.parts = xt, wt
         ctx.save_for_backward(keep)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
@@ -543,40 +509,37 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, g):
-        x_shape, (n, k) = ctx.shapes
+        x_shape, n, k = ctx.shapes
         need_x, need_w = ctx.needs_input_grad[:2]
-        form = ctx.form
-        if form is None:
+        if ctx.form is None:
             return (g.new_zeros(x_shape) if need_x else None, g.new_zeros(n, k) if need_w else None,
                     None, None, None, None, None)
         dx = dw = None
         if need_x or need_w:
-            tokens = g.numel() // n
-            scaling, scale_vec, _ = form
-            auto = scaling == "ue4m3"
-            space = _Space()
-            gr = space.blocks(tokens, n, scaling, scale_vec) if need_x else None
-            gt = space.blocks(n, tokens, scaling, scale_vec) if need_w else None
-            count = _partial_count(tokens * n) if auto else 0
-            small = space.take(4 * (1 + count))
-            device = g.device
-            lib = nat.load()
+            rounding, auto, fmt, block = ctx.form
+            tokens, device, dtype = g.numel() // n, g.device, g.dtype
             keep, = ctx.saved_tensors
-            with _On(device.index) as handle:
-                work = torch.empty(space.size, dtype=torch.uint8, device=device)
-                base, there = keep.data_ptr(), work.data_ptr()
-                mx, mw, mg = (base, base + 4, there + small) if auto else (None, None, None)
-                gr = None if gr is None else _placed(gr, there)
-                gt = None if gt is None else _placed(gt, there)
-                g1, job = _quantize_job(g, form, mg, mg + 4 if auto else None, count, gr, gt)
-                nat.check(lib.t5e_quantize_blocks(ctypes.byref(job), 1, handle), "t5e_quantize_blocks")
-                xt, wt = ctx.parts
-                if need_x:
-                    dx = _product(lib, gr, _placed(wt, base), mg, mw, (tokens, k), g.dtype, device, handle)
-                    if len(x_shape) != 2:
-                        dx = dx.view(x_shape)
-                if need_w:
-                    dw = _product(lib, gt, _placed(xt, base), mg, mx, (n, k), g.dtype, device, handle)
+            gr = gt = _NO_BLOCKS
+            end = 0
+            if need_x:
+                gr, end = _part(end, tokens, n, fmt, block)
+            if need_w:
+                gt, end = _part(end, n, tokens, fmt, block)
+            count = _partial_count(tokens * n) if auto else 0
+            work = torch.empty(end + 4 * (1 + count), dtype=torch.uint8, device=device)
+            base, there = keep.data_ptr(), work.data_ptr()
+            gr = _placed(gr, there) if need_x else gr
+            gt = _placed(gt, there) if need_w else gt
+            mx, mw, mg, pg = (base, base + 4, there + end, there + end + 4) if auto else (0, 0, 0, 0)
+            g1, job = _job(g, rounding, mg, pg, count, gr, gt)
+            _call(nat.load().t5e_quantize_blocks, device.index, job, 1)
+            xt, wt = ctx.parts
+            if need_x:
+                dx = _product(gr, _placed(wt, base), mg, mw, tokens, k, dtype, device)
+                if len(x_shape) != 2:
+                    dx = dx.view(x_shape)
+            if need_w:
+                dw = _product(gt, _placed(xt, base), mg, mx, n, k, dtype, device)
         return dx, dw, None, None, None, None, None
 
 

@@ -1113,12 +1113,17 @@ int launch_pair(const Params& params, const t5e_blocks& a, const t5e_blocks& b, 
 uint32_t choose_form(uint64_t p_rows, uint64_t q_rows, uint32_t stages, bool swap) {
   const uint64_t sms = (uint64_t)sm_count(), pairs = sms / 2;
   auto tiles = [&](uint64_t rows, uint64_t cols) { return ((p_rows + rows - 1) / rows) * ((q_rows + cols - 1) / cols); };
+  // Parts of K: as many as fill the SMs with four stages or more each; up to 32
+  // rows, whose tiles cost little to join, two blocks an SM (1 x 8192 x 8192 in
+  // 4 parts 11.4 us, in 2 parts 12.0; 48 x 14336 x 4096 whole 13.3 us, in 2
+  // parts 14.2)
+  const uint64_t room = q_rows <= 32 ? 2 * sms : sms;
   uint32_t split = 1;
-  while (split < 8 && tiles(128, 128) * split * 2 <= sms && stages >= split * 4) split *= 2;
+  while (split < 8 && tiles(128, 128) * split * 2 <= room && stages >= split * 4) split *= 2;
   if (swap || q_rows <= 64 || split >= 4) return split;
-  // waves of tiles over the pairs, a 256-wide tile taking 1.6 times a 128-wide
-  // one (1536 x 1536 x 8192: 16.9 us in 36 tiles of 256, 15.7 in 72 of 128;
-  // 8192 x 4096 x 4096: 60 us in 7 waves, 82 in 14)
+  // Whole K in pairs: waves of tiles over the pairs, a 256-wide tile taking 1.6
+  // times a 128-wide one (1536 x 1536 x 8192: 16.7 us in 36 tiles of 256, 15.8
+  // in 72 of 128; 8192 x 4096 x 4096: 59 us in 7 waves, 81 in 14)
   const uint64_t wide = (tiles(256, 256) + pairs - 1) / pairs * 16, narrow = (tiles(256, 128) + pairs - 1) / pairs * 10;
   return wide < narrow ? 256 : 128;
 }
@@ -1131,8 +1136,8 @@ extern "C" {
 int t5e_block_scaled_mm(const t5e_block_mm* mm, void* stream) {
   using namespace t5e;
   using namespace t5e::blockmm;
-  if (!mm || !blocks_ok(mm->a) || !blocks_ok(mm->b)) return T5E_ERR_INVALID;
-  const t5e_blocks &a = *mm->a, &b = *mm->b;
+  if (!mm || !blocks_ok(&mm->a) || !blocks_ok(&mm->b)) return T5E_ERR_INVALID;
+  const t5e_blocks &a = mm->a, &b = mm->b;
   auto real = [](int32_t t) { return t == T5E_REAL_F32 || t == T5E_REAL_BF16 || t == T5E_REAL_F16; };
   if (a.k != b.k || a.scale_format != b.scale_format || a.scale_block != b.scale_block || !real(mm->d_type) ||
       (mm->c && !real(mm->c_type)))

@@ -203,7 +203,7 @@ def test_c_entry_points_refuse_bad_arguments():
         b = blk(**kw)
         assert lib.t5e_dequantize_blocks(ctypes.byref(b), None, 0, 4096, 128, None) == nat.ERR_INVALID
         assert quantize(rows=b.rows, cols=max(b.k, 0), by_rows=b) == nat.ERR_INVALID
-        mm = nat.BlockMm(ctypes.addressof(b), ctypes.addressof(second), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
+        mm = nat.BlockMm(b, second, None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(mm), None) == nat.ERR_INVALID
     good = blk()
     for kw in (dict(type=3), dict(rounding=1), dict(stride=127), dict(x=4098), dict(x=None), dict(partials=4096, count=4),
@@ -216,16 +216,45 @@ def test_c_entry_points_refuse_bad_arguments():
         assert lib.t5e_block_multiplier(0, 4096, 8, 128, 128, partials, count, out, None) == nat.ERR_INVALID
 
     def mm(**kw):
-        m = nat.BlockMm(ctypes.addressof(good), ctypes.addressof(second), None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
+        m = nat.BlockMm(good, second, None, None, 1.0, 0, None, 0, 0, 0, 0, 4096, 8)
         for name, v in kw.items():
             setattr(m, name, v)
         return lib.t5e_block_scaled_mm(ctypes.byref(m), None)
 
     other = blk(scale_format=nat.SCALE_UE8M0)
     for kw in (dict(d=None), dict(d=4098), dict(d_stride=7), dict(d_type=3), dict(c=4096, c_type=5), dict(c=4098),
-               dict(form=3), dict(form=16), dict(form=2), dict(b=ctypes.addressof(other)), dict(a=None)):
+               dict(form=3), dict(form=16), dict(form=2), dict(b=other), dict(a=none)):
         assert mm(**kw) == nat.ERR_INVALID, kw
     assert lib.t5e_block_scaled_mm_expired(None) == nat.ERR_INVALID
+
+
+def test_packed_structs_match_the_header(tmp_path):
+    """The struct.pack formats and the ctypes structures lay t5e_blocks,
+    t5e_quantize and t5e_block_mm out as the C compiler does."""
+    import ctypes
+    import struct
+    import subprocess
+    from pathlib import Path
+
+    src = tmp_path / "layout.c"
+    src.write_text(
+        '#include <stdio.h>\n#include <stddef.h>\n#include "t5e.h"\n'
+        'int main(void){printf("%zu %zu %zu %zu %zu %zu %zu\\n", sizeof(t5e_blocks), sizeof(t5e_quantize),'
+        ' sizeof(t5e_block_mm), offsetof(t5e_quantize, by_cols), offsetof(t5e_block_mm, c),'
+        ' offsetof(t5e_block_mm, d), offsetof(t5e_blocks, scale_block));return 0;}\n')
+    exe = tmp_path / "layout"
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", "-I", str(include), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(nat.Blocks), ctypes.sizeof(nat.Quantize), ctypes.sizeof(nat.BlockMm),
+                   nat.Quantize.by_cols.offset, nat.BlockMm.c.offset, nat.BlockMm.d.offset, nat.Blocks.scale_block.offset]
+    for fmt, cls in ((nat.BLOCKS_FORMAT, nat.Blocks), (nat.QUANTIZE_FORMAT, nat.Quantize), (nat.BLOCK_MM_FORMAT, nat.BlockMm)):
+        assert struct.calcsize(fmt) == ctypes.sizeof(cls)
+    q = nat.Quantize(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, nat.Blocks(11, 12, 13, 14, 15, 16, 17), nat.Blocks(18, 19, 20, 21, 22, 23, 24))
+    assert bytes(q) == struct.pack(nat.QUANTIZE_FORMAT, *range(1, 25))
+    m = nat.BlockMm(nat.Blocks(1, 2, 3, 4, 5, 6, 7), nat.Blocks(8, 9, 10, 11, 12, 13, 14), 15, 16, 17.0, 18, 19, 20, 21, 22,
+                    23, 24, 25)
+    assert bytes(m) == struct.pack(nat.BLOCK_MM_FORMAT, *range(1, 17), 17.0, *range(18, 26))
 
 
 def test_empty_calls_launch_nothing():
@@ -238,7 +267,7 @@ def test_empty_calls_launch_nothing():
     q = nat.Quantize(None, 0, 128, 128, 0, 0, None, None, 0, 0, nat.Blocks(), nat.Blocks())
     assert lib.t5e_quantize_blocks(ctypes.byref(q), 1, None) == nat.OK
     for a, b in ((none, some), (some, none)):
-        m = nat.BlockMm(ctypes.addressof(a), ctypes.addressof(b), None, None, 1.0, 0, None, 0, 0, 0, 0, None, 8)
+        m = nat.BlockMm(a, b, None, None, 1.0, 0, None, 0, 0, 0, 0, None, 8)
         assert lib.t5e_block_scaled_mm(ctypes.byref(m), None) == nat.OK
 
 
