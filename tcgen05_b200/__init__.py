@@ -20,6 +20,7 @@ from .blocks import (
     block_multiplier,
     block_scaled_linear,
     block_scaled_mm,
+    block_scaled_mm_expired,
     dequantize_blocks,
     quantize_blocks,
 )
@@ -50,6 +51,7 @@ __all__ = [
     "block_multiplier",
     "block_scaled_linear",
     "block_scaled_mm",
+    "block_scaled_mm_expired",
     "dequantize_blocks",
     "f32_to_bits",
     "make_model",

@@ -19,12 +19,14 @@ CPU fallback.
 
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import torch
 
 from . import _native as nat
 from . import packing
+from .runtime import require_device
 from .simulator import PackedRows
 
 _REAL = {torch.float32: nat.REAL_F32, torch.bfloat16: nat.REAL_BF16, torch.float16: nat.REAL_F16}
@@ -39,6 +41,9 @@ _pack_quantize = struct.Struct(nat.QUANTIZE_FORMAT).pack
 _pack_mm = struct.Struct(nat.BLOCK_MM_FORMAT).pack
 _NO_BLOCKS = (0, 0, 0, 0, 0, 0, 0)
 _ROUNDINGS = {"nearest": nat.SCALE_ROUND_NEAREST, "floor": nat.SCALE_ROUND_FLOOR, "ceil": nat.SCALE_ROUND_CEIL}
+
+
+_F32_LARGEST, _F32_SMALLEST = torch.finfo(torch.float32).max, torch.finfo(torch.float32).smallest_normal
 
 
 def _form(scaling, scale_vec) -> tuple[str, int]:
@@ -214,6 +219,8 @@ def _matrix_of(x):
     """(matrix, stride, turned): x as rows of its last dimension with unit column
     stride, or `turned`, the matrix whose columns those rows are (no copy of a
     transposed matrix); other layouts are copied."""
+    if x.is_neg():
+        x = x.detach().resolve_neg()
     if x.dim() != 2:
         x = x.detach().reshape(-1, x.shape[-1])
     rows, cols = x.shape
@@ -279,8 +286,10 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
         raise ValueError(f"axis is -1, 0 or 'both', not {axis!r}")
     if isinstance(multiplier, str) and multiplier != "auto":
         raise ValueError(f"multiplier is a number, a tensor, 'auto' or None, not {multiplier!r}")
-    if isinstance(multiplier, (int, float)) and not 0 < multiplier < float("inf"):
-        raise ValueError(f"multiplier must be positive and finite, not {multiplier!r}")
+    if multiplier is not None and not isinstance(multiplier, (str, torch.Tensor)):
+        multiplier = float(multiplier)
+        if not _F32_SMALLEST <= multiplier <= _F32_LARGEST:
+            raise ValueError(f"multiplier must be positive, finite and a normal float32, not {multiplier!r}")
     _real_tensor(x, "x")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("x must have at least one dimension and a non-empty last one")
@@ -312,7 +321,7 @@ def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplie
                 partials, multiplier = at + 4, work[:1]
         else:
             if not isinstance(multiplier, torch.Tensor):
-                multiplier = torch.full((1,), float(multiplier), dtype=torch.float32, device=device)
+                multiplier = torch.full((1,), multiplier, dtype=torch.float32, device=device)
             at = multiplier.data_ptr()
     rows = BlockScaledRows._new(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
     cols = BlockScaledRows._new(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
@@ -359,6 +368,8 @@ def dequantize_blocks(blocks: BlockScaledRows, *, dtype=torch.float32, out=None)
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     given = out is not None
     out = _result(out, (blocks.rows, blocks.k), dtype, blocks.device)
+    if given:
+        _apart(out, blocks, "blocks")
     m = blocks.multiplier
     _call(nat.load().t5e_dequantize_blocks, blocks.device.index, _pack_blocks(*blocks._fields),
           None if m is None else m.data_ptr(), _REAL[dtype], out.data_ptr(),
@@ -370,6 +381,16 @@ def _span(t):
     """[first, behind the last) byte of a tensor's elements."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(out, blocks, name):
+    """Refuses an `out` that shares memory with the blocks it is computed from."""
+    if out.numel():
+        d0, d1 = _span(out)
+        at, stride, scales, rows, k, _, block = blocks._fields
+        for lo, hi in ((at, at + rows * stride), (scales, scales + (rows + 127) // 128 * (-(-k // (4 * block)) * 512))):
+            if lo < d1 and d0 < hi:
+                raise ValueError(f"out overlaps {name}")
 
 
 def block_scaled_mm(a: BlockScaledRows, b: BlockScaledRows, c=None, *, alpha: float = 1.0, dtype=torch.bfloat16,
@@ -400,6 +421,9 @@ def _mm(a, b, c, alpha, dtype, out, form):
         raise ValueError("a and b are on different devices")
     if dtype not in _REAL:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    alpha = float(alpha)
+    if _F32_LARGEST < abs(alpha) < float("inf"):
+        raise ValueError(f"alpha={alpha!r} is not a float32")
     shape = (a.rows, b.rows)
     if c is not None:
         _real_tensor(c, "c")
@@ -408,11 +432,14 @@ def _mm(a, b, c, alpha, dtype, out, form):
         if c.requires_grad and torch.is_grad_enabled():
             raise ValueError("block_scaled_mm gives c no gradient; detach it or use block_scaled_linear")
         try:
-            c = c.detach().expand(shape)
+            c = c.detach().resolve_neg().expand(shape)
         except RuntimeError:
             raise ValueError(f"c of shape {tuple(c.shape)} does not broadcast to {shape}") from None
     given = out is not None
     out = _result(out, shape, dtype, a.device)
+    if given:
+        _apart(out, a, "a")
+        _apart(out, b, "b")
     if given and c is not None and out.numel():
         (c0, c1), (d0, d1) = _span(c), _span(out)
         same = c0 == d0 and c.dtype == out.dtype and all(n == 1 or s == t for n, s, t in
@@ -426,6 +453,16 @@ def _mm(a, b, c, alpha, dtype, out, form):
                    c_at, c_type, _REAL[dtype], c_rows, c_cols, out.data_ptr(),
                    out.stride(0) if given and shape[0] > 1 else shape[1]))
     return out
+
+
+def block_scaled_mm_expired(device=None) -> bool:
+    """Whether a bounded wait inside a product ran out on the device since the
+    library was loaded (the tile concerned holds NaN); synchronizes the device."""
+    device = require_device(device)
+    flag = ctypes.c_int32(0)
+    with torch.cuda.device(device):
+        nat.check(nat.load().t5e_block_scaled_mm_expired(ctypes.byref(flag)), "t5e_block_scaled_mm_expired")
+    return flag.value != 0
 
 
 def _part(at, rows, k, fmt, block):

@@ -19,8 +19,8 @@ using blocks::to_f32;
 constexpr int kStageK = 256;      // elements of K per pipeline stage: 128 bytes, one swizzle atom wide
 constexpr int kInstrK = 64;       // elements of K per tcgen05.mma
 constexpr int kRowBytes = 128;    // bytes of a row in a stage
-// Bounded waits: after this long (2 s) the tile is given up.
-constexpr uint64_t kWaitNs = 2000000000ull;
+// Bounded waits: after this long (4 s) the tile is given up.
+constexpr uint64_t kWaitNs = 4000000000ull;
 
 __device__ int g_expired;  // 1 once a wait ran out on this device
 
@@ -739,19 +739,24 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
     for (int q = w0; q < w0 + width; q += 8) {
       if (q0 + q >= P.q_rows) break;
       const int count = width < 8 ? width : 8;
+      const uint32_t here = smem_u32(part + q * 128 + t);
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      for (uint32_t r = 0; r < split; ++r) {
-        const uint32_t there = in_block(smem_u32(part + q * 128 + t), r);
+      for (uint32_t r = 0; r < split; r += 2) {  // two blocks' parts in flight
+        float x[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i < count) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(there + i * 512) : "memory");
-            v[i] += x;
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t there = in_block(here, r + s);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[s][i] = 0.f;
+            if (i < count)
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[s][i]) : "r"(there + i * 512) : "memory");
           }
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (v[i] + x[0][i]) + x[1][i];
       }
       store_results<SWAP, 8>(P, alpha, p0 + t, q0 + q, count, v);
     }

@@ -203,15 +203,8 @@ __device__ __forceinline__ float divide(float x, float m, float step, float inv)
   }
 }
 
-// Two values to two E2M1 codes (RNE, magnitudes above 6 become 6): `lo` in
-// the low nibble.
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}\n"
-      : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
+// Eight values to eight E2M1 codes (RNE, magnitudes above 6 become 6), the first in
+// the lowest nibble.
 __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
