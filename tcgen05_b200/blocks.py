@@ -43,6 +43,7 @@ _NO_BLOCKS = (0, 0, 0, 0, 0, 0, 0)
 _ROUNDINGS = {"nearest": nat.SCALE_ROUND_NEAREST, "floor": nat.SCALE_ROUND_FLOOR, "ceil": nat.SCALE_ROUND_CEIL}
 
 
+_MOST = min(nat.MAX_BLOCK_K, nat.MAX_BLOCK_ROWS)
 _F32_LARGEST, _F32_SMALLEST = torch.finfo(torch.float32).max, torch.finfo(torch.float32).smallest_normal
 
 
@@ -63,6 +64,23 @@ def _rounding(scaling: str, scale_rounding) -> int:
         raise ValueError(f"scale_rounding is 'floor' or 'ceil' for ue8m0 and 'nearest' for ue4m3, "
                          f"not {scale_rounding!r} for {scaling}")
     return _ROUNDINGS[scale_rounding]
+
+
+# (scaling, scale_vec, scale_rounding) as a caller gives them -> what they mean
+_CHOICES: dict = {}
+
+
+def _choice(scaling, scale_vec, scale_rounding):
+    """(scaling, scale_vec, rounding, scale format, elements per block)."""
+    try:
+        return _CHOICES[scaling, scale_vec, scale_rounding]
+    except (KeyError, TypeError):
+        pass
+    name, vec = _form(scaling, scale_vec)
+    found = (name, vec, _rounding(name, scale_rounding), *_FORMS[name, vec])
+    if len(_CHOICES) < 64:
+        _CHOICES[scaling, scale_vec, scale_rounding] = found
+    return found
 
 
 def tile_scales(words: torch.Tensor) -> torch.Tensor:
@@ -94,7 +112,7 @@ class BlockScaledRows:
     multiplied by before rounding, or None: element i of row r stands for
     code * scale / multiplier."""
 
-    __slots__ = ("rows", "k", "scaling", "scale_vec", "device", "multiplier", "_data", "_scales", "_buffer", "_fields")
+    __slots__ = ("scaling", "scale_vec", "device", "multiplier", "_data", "_scales", "_buffer", "_fields")
 
     def __init__(self, data, scales, k: int, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
         scaling, scale_vec = _form(scaling, scale_vec)
@@ -120,24 +138,21 @@ class BlockScaledRows:
         at, scales_at = data.data_ptr(), scales.data_ptr()
         if at % 16 or scales_at % 16:
             raise ValueError("data and scales must start on 16-byte boundaries")
-        self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
-        self.device, self.multiplier = data.device, multiplier
+        self.scaling, self.scale_vec, self.device, self.multiplier = scaling, scale_vec, data.device, multiplier
         self._data, self._scales, self._buffer = data, scales, None
         self._fields = (at, stride, scales_at, rows, k, fmt, block)  # t5e_blocks
 
     @classmethod
-    def _new(cls, device, rows, k, scaling, scale_vec, multiplier):
+    def _new(cls, device, rows, k, choice, multiplier):
         """An instance over one new allocation: the rows, then the scale tiles.
         The views are made when they are asked for."""
         self = cls.__new__(cls)
-        fmt, block = _FORMS[scaling, scale_vec]
+        self.scaling, self.scale_vec, _, fmt, block = choice
         stride = (k + 31) // 32 * 16
         size = rows * stride
         self._buffer = buffer = torch.empty(size + (rows + 127) // 128 * (-(-k // (4 * block)) * 512), dtype=torch.uint8,
                                             device=device)
-        self.rows, self.k, self.scaling, self.scale_vec = rows, k, scaling, scale_vec
-        self.device, self.multiplier = device, multiplier
-        self._data = self._scales = None
+        self.device, self.multiplier, self._data, self._scales = device, multiplier, None, None
         at = buffer.data_ptr()
         self._fields = (at, stride, at + size, rows, k, fmt, block)
         return self
@@ -160,6 +175,14 @@ class BlockScaledRows:
     def row_stride(k: int) -> int:
         """Smallest row stride in bytes: whole groups of 32 elements."""
         return (k + 31) // 32 * 16
+
+    @property
+    def rows(self) -> int:
+        return self._fields[3]
+
+    @property
+    def k(self) -> int:
+        return self._fields[4]
 
     @property
     def data(self) -> torch.Tensor:
@@ -280,51 +303,49 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
     ``multiplier``: None (1), a positive float, a one-element float32 tensor, or
     "auto", ``block_multiplier(x)`` found in the same call.  The result carries
     no gradient (see ``block_scaled_linear``)."""
-    scaling, scale_vec = _form(scaling, scale_vec)
-    rounding = _rounding(scaling, scale_rounding)
+    choice = _choice(scaling, scale_vec, scale_rounding)
     if axis not in (-1, 0, "both"):
         raise ValueError(f"axis is -1, 0 or 'both', not {axis!r}")
-    if isinstance(multiplier, str) and multiplier != "auto":
-        raise ValueError(f"multiplier is a number, a tensor, 'auto' or None, not {multiplier!r}")
-    if multiplier is not None and not isinstance(multiplier, (str, torch.Tensor)):
-        multiplier = float(multiplier)
-        if not _F32_SMALLEST <= multiplier <= _F32_LARGEST:
-            raise ValueError(f"multiplier must be positive, finite and a normal float32, not {multiplier!r}")
+    if multiplier is not None:
+        if isinstance(multiplier, str):
+            if multiplier != "auto":
+                raise ValueError(f"multiplier is a number, a tensor, 'auto' or None, not {multiplier!r}")
+        elif not isinstance(multiplier, torch.Tensor):
+            multiplier = float(multiplier)
+            if not _F32_SMALLEST <= multiplier <= _F32_LARGEST:
+                raise ValueError(f"multiplier must be positive, finite and a normal float32, not {multiplier!r}")
     _real_tensor(x, "x")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("x must have at least one dimension and a non-empty last one")
     if isinstance(multiplier, torch.Tensor) and (multiplier.dtype != torch.float32 or multiplier.numel() != 1
                                                  or multiplier.device != x.device):
         raise ValueError("multiplier must be a one-element float32 tensor on x's device")
-    k = x.shape[-1]
+    k = shape[-1]
     r = x.numel() // k
-    by_rows, by_cols = axis in (-1, "both"), axis in (0, "both")
+    by_rows, by_cols = axis != 0, axis != -1
+    if r > _MOST or k > _MOST:
+        if (by_rows and k > nat.MAX_BLOCK_K) or (by_cols and r > nat.MAX_BLOCK_K) or max(r, k) > nat.MAX_BLOCK_ROWS:
+            raise ValueError(f"x is larger than {nat.MAX_BLOCK_K} elements along a block axis or {nat.MAX_BLOCK_ROWS} rows")
     if by_cols and r == 0:
         raise ValueError("blocks along an empty axis")
-    if (by_rows and k > nat.MAX_BLOCK_K) or (by_cols and r > nat.MAX_BLOCK_K) or max(r, k) > nat.MAX_BLOCK_ROWS:
-        raise ValueError(f"x is larger than {nat.MAX_BLOCK_K} elements along a block axis or {nat.MAX_BLOCK_ROWS} rows")
-    return _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier)
-
-
-def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplier):
-    """quantize_blocks of checked arguments, x as r rows of k: the rows, the
-    columns or the pair."""
     device = x.device
     partials = count = at = 0
     if multiplier is not None:
-        if isinstance(multiplier, str):
-            multiplier = None
-            if r:
-                count = _partial_count(r * k)
-                work = torch.empty(1 + count, dtype=torch.float32, device=device)
-                at = work.data_ptr()
-                partials, multiplier = at + 4, work[:1]
-        else:
-            if not isinstance(multiplier, torch.Tensor):
-                multiplier = torch.full((1,), multiplier, dtype=torch.float32, device=device)
+        if isinstance(multiplier, torch.Tensor):
             at = multiplier.data_ptr()
-    rows = BlockScaledRows._new(device, r, k, scaling, scale_vec, multiplier) if by_rows else None
-    cols = BlockScaledRows._new(device, k, r, scaling, scale_vec, multiplier) if by_cols else None
+        elif isinstance(multiplier, float):
+            multiplier = torch.full((1,), multiplier, dtype=torch.float32, device=device)
+            at = multiplier.data_ptr()
+        elif r:
+            count = _partial_count(r * k)
+            work = torch.empty(1 + count, dtype=torch.float32, device=device)
+            at = work.data_ptr()
+            partials, multiplier = at + 4, work[:1]
+        else:
+            multiplier = None
+    rows = BlockScaledRows._new(device, r, k, choice, multiplier) if by_rows else None
+    cols = BlockScaledRows._new(device, k, r, choice, multiplier) if by_cols else None
     if r:
         m, m_rows, m_cols, stride, turned = _matrix_of(x)
         along = _NO_BLOCKS if rows is None else rows._fields
@@ -332,11 +353,11 @@ def _quantize(x, r, k, by_rows, by_cols, scaling, scale_vec, rounding, multiplie
         if turned:
             along, across = across, along
         _call(nat.load().t5e_quantize_blocks, device.index,
-              _pack_quantize(m.data_ptr(), m_rows, m_cols, stride, _REAL[m.dtype], rounding, at, partials, count, 0, *along,
+              _pack_quantize(m.data_ptr(), m_rows, m_cols, stride, _REAL[m.dtype], choice[2], at, partials, count, 0, *along,
                              *across), 1)
-    if by_rows and by_cols:
-        return rows, cols
-    return rows if by_rows else cols
+    if rows is None:
+        return cols
+    return rows if cols is None else (rows, cols)
 
 
 def _check_blocks(q, name: str):
@@ -504,13 +525,13 @@ class _Linear(torch.autograd.Function):
     its launches."""
 
     @staticmethod
-    def forward(ctx, x, w, scaling, scale_vec, rounding, need_x, need_w):
+    def forward(ctx, x, w, choice, need_x, need_w):
         (n, k), tokens, device = w.shape, x.numel() // w.shape[1], x.device
         ctx.shapes = x.shape, n, k
         if not tokens:
             ctx.form = None
             return x.new_empty((*x.shape[:-1], n))
-        fmt, block = _FORMS[scaling, scale_vec]
+        scaling, _, rounding, fmt, block = choice
         auto = scaling == "ue4m3"
         ctx.form = rounding, auto, fmt, block
         # Blocks run along the contraction: K here, the tokens and N in the
@@ -550,7 +571,7 @@ class _Linear(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         if ctx.form is None:
             return (g.new_zeros(x_shape) if need_x else None, g.new_zeros(n, k) if need_w else None,
-                    None, None, None, None, None)
+                    None, None, None)
         dx = dw = None
         if need_x or need_w:
             rounding, auto, fmt, block = ctx.form
@@ -577,7 +598,7 @@ class _Linear(torch.autograd.Function):
                     dx = dx.view(x_shape)
             if need_w:
                 dw = _product(gt, _placed(xt, base), mg, mx, n, k, dtype, device)
-        return dx, dw, None, None, None, None, None
+        return dx, dw, None, None, None
 
 
 @torch.autograd.function.once_differentiable
@@ -599,8 +620,7 @@ def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None =
     UE4M3 forms take the "auto" multiplier for x, w and g.  x and w are read
     once each; a training step keeps their 4-bit transposes for the backward
     pass, not the tensors.  Differentiable once."""
-    scaling, scale_vec = _form(scaling, scale_vec)
-    rounding = _rounding(scaling, scale_rounding)
+    choice = _choice(scaling, scale_vec, scale_rounding)
     _real_tensor(x, "x")
     _real_tensor(w, "w")
     if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
@@ -610,4 +630,4 @@ def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None =
     if x.dtype != w.dtype or x.device != w.device:
         raise ValueError("x and w must have one type and device")
     grad = torch.is_grad_enabled()
-    return _Linear.apply(x, w, scaling, scale_vec, rounding, grad and x.requires_grad, grad and w.requires_grad)
+    return _Linear.apply(x, w, choice, grad and x.requires_grad, grad and w.requires_grad)

@@ -636,6 +636,35 @@ struct TileParams {
   Depth depth;
 };
 
+// Adds the parts of N columns of a row, in rank order, and stores the results.
+// `here` is the address of the row's first column in this block's part.
+template <bool SWAP, int N>
+__device__ __forceinline__ void join_parts(const Params& P, float alpha, uint32_t split, uint32_t here, uint32_t p,
+                                           uint32_t q) {
+  float v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (uint32_t r = 0; r < split; r += 2) {  // two blocks' parts in flight
+    float x[2][N];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t there = in_block(here, r + s);
+      if constexpr (N == 2) {
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[s][0]), "=f"(x[s][1]) : "r"(there) : "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(x[s][i]), "=f"(x[s][i + 1]), "=f"(x[s][i + 2]), "=f"(x[s][i + 3]) : "r"(there + i / 4 * 2048)
+                       : "memory");
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (v[i] + x[0][i]) + x[1][i];
+  }
+  store_results<SWAP, N>(P, alpha, p, q, N, v);
+}
+
 template <int BN, int BLOCK, bool SWAP>
 __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileParams T, uint32_t split) {
   using S = typename TileShape<BN, BLOCK>::Pipe;
@@ -650,7 +679,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   uint8_t* scale_stages = stages + T.depth.stages * S::kStageBytes;
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmem));
+                 :: "r"(smem_u32(&tmem_slot)), "n"(S::kTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (t == 0) {
@@ -725,40 +754,29 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
       store_results<SWAP, 16>(P, alpha, p0 + t, q0 + q, 16, v);
     }
   } else {
-    float* part = reinterpret_cast<float*>(stages);
+    // four columns of a row side by side, so that both sides move 16 bytes a lane
+    float4* part = reinterpret_cast<float4*>(stages);
 #pragma unroll 1
     for (int q = 0; q < BN; q += 16) {
       float v[16];
       load_acc16(lanes + q, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) part[(q + i) * 128 + t] = bad ? nan : v[i];
+      for (int i = 0; i < 4; ++i)
+        part[(q / 4 + i) * 128 + t] = bad ? make_float4(nan, nan, nan, nan)
+                                          : make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
     cluster_sync();
     const int width = BN / (int)split, w0 = width * (int)rank;
+    if (width >= 8) {
 #pragma unroll 1
-    for (int q = w0; q < w0 + width; q += 8) {
-      if (q0 + q >= P.q_rows) break;
-      const int count = width < 8 ? width : 8;
-      const uint32_t here = smem_u32(part + q * 128 + t);
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      for (uint32_t r = 0; r < split; r += 2) {  // two blocks' parts in flight
-        float x[2][8];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t there = in_block(here, r + s);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[s][i] = 0.f;
-            if (i < count)
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[s][i]) : "r"(there + i * 512) : "memory");
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (v[i] + x[0][i]) + x[1][i];
+      for (int q = w0; q < w0 + width; q += 8) {
+        if (q0 + q >= P.q_rows) break;
+        join_parts<SWAP, 8>(P, alpha, split, smem_u32(part + q / 4 * 128 + t), p0 + t, q0 + q);
       }
-      store_results<SWAP, 8>(P, alpha, p0 + t, q0 + q, count, v);
+    } else if (width == 4) {
+      join_parts<SWAP, 4>(P, alpha, split, smem_u32(part + w0 / 4 * 128 + t), p0 + t, q0 + w0);
+    } else {
+      join_parts<SWAP, 2>(P, alpha, split, smem_u32(part + w0 / 4 * 128 + t) + w0 % 4 * 4, p0 + t, q0 + w0);
     }
     cluster_sync();
   }
@@ -766,7 +784,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   __syncthreads();
   if (warp == 2) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmem));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "n"(S::kTmem));
   }
 }
 
@@ -823,7 +841,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
   uint8_t* scale_stages = stages + S::STAGES * S::kStageBytes;
   if (warp == 4) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_u32(&tmem_slot)), "r"(S::kTmem));
+                 :: "r"(smem_u32(&tmem_slot)), "n"(S::kTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   if (t == 0) {
@@ -943,7 +961,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
   cluster_sync();
   if (warp == 4) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmem));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "n"(S::kTmem));
   }
 }
 
@@ -1053,6 +1071,36 @@ int blocks_launched(cudaError_t e) {
   return kernel_status("block product launch");
 }
 
+// Blocks of clusters of `split` that the device runs at once with one block an SM
+// (clusters stay within a group of SMs: 148, 148, 132 and 120 blocks on a B200),
+// looked up once per device.
+uint64_t blocks_at_once(uint32_t split) {
+  static std::atomic<int> known[64][4];
+  const int which = split == 1u ? 0 : split == 2u ? 1 : split == 4u ? 2 : 3;
+  int dev = 0;
+  const bool cached = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  int n = cached ? known[dev][which].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return (uint64_t)n;
+  using S = TileShape<128, 16>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(split);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = S::kDeepSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {split, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (raise_smem_limit<tile_kernel<128, 16, false>>(S::kDeepSmem, "block product attribute") != T5E_OK ||
+      cudaOccupancyMaxActiveClusters(&n, tile_kernel<128, 16, false>, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();  // an estimate only: the launch reports what is wrong
+    return (uint64_t)sm_count();
+  }
+  n *= (int)split;
+  if (cached) known[dev][which].store(n, std::memory_order_relaxed);
+  return (uint64_t)n;
+}
+
 template <int BN, int BLOCK, bool SWAP>
 int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, uint32_t split, cudaStream_t stream) {
   using S = TileShape<BN, BLOCK>;
@@ -1065,7 +1113,7 @@ int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, 
   cudaLaunchConfig_t cfg = {};
   const uint64_t grid = ((p.rows + 127) / 128) * ((q.rows + BN - 1) / BN) * split;
   if (grid > 0x7FFFFFFFull) return T5E_ERR_INVALID;
-  const bool deep = grid <= (uint64_t)sm_count();
+  const bool deep = grid <= blocks_at_once(split);
   P.depth = deep ? Depth{S::kDeepStages, S::kDeepScaleStages} : Depth{S::kStages, S::kScaleStages};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(128);
@@ -1116,15 +1164,15 @@ int launch_pair(const Params& params, const t5e_blocks& a, const t5e_blocks& b, 
 }
 
 uint32_t choose_form(uint64_t p_rows, uint64_t q_rows, uint32_t stages, bool swap) {
-  const uint64_t sms = (uint64_t)sm_count(), pairs = sms / 2;
+  const uint64_t pairs = (uint64_t)sm_count() / 2;
   auto tiles = [&](uint64_t rows, uint64_t cols) { return ((p_rows + rows - 1) / rows) * ((q_rows + cols - 1) / cols); };
-  // Parts of K: as many as fill the SMs with four stages or more each; up to 32
-  // rows, whose tiles cost little to join, two blocks an SM (1 x 8192 x 8192 in
-  // 4 parts 11.4 us, in 2 parts 12.0; 48 x 14336 x 4096 whole 13.3 us, in 2
-  // parts 14.2)
-  const uint64_t room = q_rows <= 32 ? 2 * sms : sms;
+  // Parts of K: as many as run at once, with two stages or more each; where Q is
+  // one tile, two blocks an SM (1 x 8192 x 8192 in 4 parts 10.9 us, in 2 parts
+  // 12.1; 100 x 8192 x 8192 16.0 and 18.7; 48 x 14336 x 4096 whole 13.2 us, in 2
+  // parts 13.5; but 512 x 512 x 8192 in 8 parts 11.3, in 4 parts 10.0)
+  const uint64_t share = q_rows <= 128 ? 2 : 1;
   uint32_t split = 1;
-  while (split < 8 && tiles(128, 128) * split * 2 <= room && stages >= split * 4) split *= 2;
+  while (split < 8 && stages >= split * 4 && tiles(128, 128) * split * 2 <= share * blocks_at_once(split * 2)) split *= 2;
   if (swap || q_rows <= 64 || split >= 4) return split;
   // Whole K in pairs: waves of tiles over the pairs, a 256-wide tile taking 1.6
   // times a 128-wide one (1536 x 1536 x 8192: 16.7 us in 36 tiles of 256, 15.8
