@@ -345,44 +345,46 @@ __device__ __forceinline__ void store_turned(const Params& P, float alpha, uint3
   }
 }
 
-// The same results, without C, through a box of 32 rows that TMA writes: rows
-// of 64 bytes (16-bit results) or 128, swizzled as the map says, so that the
-// lanes' 16-byte stores meet no bank twice.  `boxes` are the warp's 4 KB: two
-// boxes of 16-bit results that take turns, or one of F32.
+// A warp's 32 rows by 64 results, without C, through a box of 32 rows of 128 bytes
+// that TMA writes (two boxes, one after the other, for F32): whole lines, and
+// swizzled as the map says, so that the lanes' 16-byte stores meet no bank twice.
 __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* map, float alpha, uint32_t p, uint32_t q,
-                                          const float* v, uint8_t* boxes, int turn) {
+                                          const float* v, uint8_t* box) {
   const int lane = threadIdx.x & 31;
   const bool wide = P.d_type == T5E_REAL_F32;
-  uint8_t* box = wide ? boxes : boxes + (turn & 1) * 2048;
-  if (lane == 0) {  // what was in the box has been read
-    if (wide) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-  }
-  __syncwarp();
-  if (wide) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) =
-          make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
-  } else {
+  for (int half = 0; half < 2; ++half) {
+    if (half == 1 && !wide) break;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // what was in the box has been read
+    __syncwarp();
+    uint8_t* row = box + lane * 128;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];
+    for (int j = 0; j < 8; ++j) {
+      uint4 w;
+      if (wide) {
+        const float* x = v + half * 32 + 4 * j;
+        w = make_uint4(__float_as_uint(x[0] * alpha), __float_as_uint(x[1] * alpha), __float_as_uint(x[2] * alpha),
+                       __float_as_uint(x[3] * alpha));
+      } else {
+        const float* x = v + 8 * j;
+        uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float lo = v[8 * j + 2 * i] * alpha, hi = v[8 * j + 2 * i + 1] * alpha;
-        w[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(lo, hi) : pack2<T5E_REAL_F16>(lo, hi);
+        for (int i = 0; i < 4; ++i)
+          h[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(x[2 * i] * alpha, x[2 * i + 1] * alpha)
+                                           : pack2<T5E_REAL_F16>(x[2 * i] * alpha, x[2 * i + 1] * alpha);
+        w = make_uint4(h[0], h[1], h[2], h[3]);
       }
-      *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) * 16)) = w;
     }
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-  if (lane == 0) {
-    if (q < P.q_rows && p < P.p_rows)
-      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
-                   :: "l"(map), "r"((int32_t)q), "r"((int32_t)p), "r"(smem_u32(box)) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      const uint32_t col = q + half * 32;
+      if (col < P.q_rows && p < P.p_rows)
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                     :: "l"(map), "r"((int32_t)col), "r"((int32_t)p), "r"(smem_u32(box)) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
   }
 }
 
@@ -805,14 +807,14 @@ template <int BN, int BLOCK>
 struct PairShape {
   static constexpr int kScaleStages = 4;
   static constexpr int kScaleBytes = kStageK / (4 * BLOCK) * 512 * (1 + BN / 128);
-  static constexpr int kBoxBytes = 5120;  // a results warp's shared memory: its boxes, or the 32 x 33 buffer
+  static constexpr int kBoxBytes = 5120;  // a results warp's shared memory: its box, or the 32 x 33 buffer
   static constexpr int kStages =
       (226 * 1024 - 1024 - 8 * kBoxBytes - kScaleStages * kScaleBytes) / (128 * kRowBytes + BN / 2 * kRowBytes);
   using Pipe = blockmm::Pipe<true, BN, BLOCK, kStages, kScaleStages, 512>;
   static constexpr int kSmem = kStages * Pipe::kStageBytes + kScaleStages * Pipe::kScaleBytes + 8 * kBoxBytes + 1024;
-  static constexpr int kSecond = BN <= 128 ? BN : (Pipe::kScaleCol - BN) / 32 * 32;  // column of the second accumulator
-  static constexpr int kShared = BN - kSecond;  // columns both use (0: none)
-  static_assert(kSecond + BN <= Pipe::kScaleCol && kShared % 32 == 0 && kShared >= 0, "tensor memory");
+  static constexpr int kSecond = 128;           // column of the second accumulator
+  static constexpr int kShared = BN - kSecond;  // columns both use: 0 or 128
+  static_assert((BN == 128 || BN == 256) && kSecond + BN <= Pipe::kScaleCol, "tensor memory");
 };
 
 struct PairParams {
@@ -911,45 +913,37 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
       fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (count & 1u) * L::kSecond;
       const uint32_t free_bar = in_block(smem_u32(&acc_free[count & 1u]), 0);
-      // chunks of 32 columns.  The shared ones (the last of the first accumulator,
-      // the first of the second) are all read at once, and let the next tile
-      // start before anything is done with them
-      constexpr int kChunks = BN / 32, kFirst = L::kShared / 32;
-      auto finish = [&](int chunk, int turn, float* v) {
+      // 64 columns at a time.  The shared ones (the last of the first accumulator,
+      // the first of the second) go first, and let the next tile start before
+      // anything is done with them
+      auto take = [&](int chunk, bool release) {
+        float v[64];
+        load_acc32(acc + chunk * 64, v);
+        load_acc32(acc + chunk * 64 + 32, v + 32);
+        acc_loaded();
+        if (release) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_in(free_bar);
+        }
         if (!ok) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
+          for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
-        const uint32_t q = q0 + chunk * 32;
-        if (P.boxed) store_box(P.r, &P.d_map, alpha, p, q, v, box, turn);
-        else store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
+        const uint32_t q = q0 + chunk * 64;
+        if (P.boxed) {
+          store_box(P.r, &P.d_map, alpha, p, q, v, box);
+        } else {
+          store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
+          store_turned(P.r, alpha, p, q + 32, v + 32, reinterpret_cast<float*>(box));
+        }
       };
-      auto release = [&] {
-        fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_in(free_bar);
-      };
-      const int first_shared = (count & 1u) == 0u ? kChunks - kFirst : 0, first_own = (count & 1u) == 0u ? 0 : kFirst;
-      int turn = 0;
-      if constexpr (kFirst > 0) {
-        constexpr int kHead = (kFirst + 1) / 2;  // of one warp at most
-        float head[kHead * 32];
-#pragma unroll
-        for (int i = 0; i < kHead; ++i)
-          if (2 * i + side < kFirst) load_acc32(acc + (first_shared + 2 * i + side) * 32, head + i * 32);
-        acc_loaded();
-        release();
-#pragma unroll
-        for (int i = 0; i < kHead; ++i)
-          if (2 * i + side < kFirst) finish(first_shared + 2 * i + side, turn++, head + i * 32);
-      }
-#pragma unroll 1
-      for (int i = side; i < kChunks - kFirst; i += 2) {
-        float v[32];
-        load_acc32(acc + (first_own + i) * 32, v);
-        acc_loaded();
-        if (kFirst == 0 && i + 2 >= kChunks) release();
-        finish(first_own + i, turn++, v);
+      if constexpr (L::kShared > 0) {
+        const int shared = (count & 1u) == 0u ? 2 : 0;
+        take(shared + side, true);
+        take(2 - shared + side, false);
+      } else {
+        take(side, true);
       }
     }
     if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1024,7 +1018,7 @@ int encode_scales(CUtensorMap* map, const t5e_blocks& b, uint32_t box_groups, ui
   return T5E_OK;
 }
 
-// Map of the results, boxes of 32 columns by 32 rows; *boxed = 0 where the rows
+// Map of the results, boxes of 128 bytes by 32 rows; *boxed = 0 where the rows
 // do not lie on 16-byte boundaries.
 int encode_results(CUtensorMap* map, const Params& P, int32_t* boxed) {
   const int bytes = P.d_type == T5E_REAL_F32 ? 4 : 2;
@@ -1033,12 +1027,12 @@ int encode_results(CUtensorMap* map, const Params& P, int32_t* boxed) {
   const EncodeTiled f = encoder();
   if (!f) return T5E_ERR_CUDA;
   const cuuint64_t dims[2] = {P.q_rows, P.p_rows}, strides[1] = {(cuuint64_t)(P.d_stride * bytes)};
-  const cuuint32_t box[2] = {32, 32}, unit[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), 32}, unit[2] = {1, 1};
   const CUtensorMapDataType type = P.d_type == T5E_REAL_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : P.d_type == T5E_REAL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult r = f(map, type, 2, P.d, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                       CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_cuda_error("cuTensorMapEncodeTiled", cudaErrorInvalidValue);
