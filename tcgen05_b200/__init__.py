@@ -15,15 +15,6 @@ on the tensor cores) and ``block_scaled_linear`` (a linear layer with its
 gradients).
 """
 
-from .blocks import (
-    BlockScaledRows,
-    block_multiplier,
-    block_scaled_linear,
-    block_scaled_mm,
-    block_scaled_mm_expired,
-    dequantize_blocks,
-    quantize_blocks,
-)
 from .formats import bits_to_f32, f32_to_bits
 from .model import (
     DotProduct,
@@ -36,6 +27,27 @@ from .model import (
     normalize_format,
 )
 from .simulator import PackedRows, PendingBatch, mma, mma_batch, mma_dot, mma_dot_batch, sparse_active_indices
+
+# in .blocks, which imports PyTorch; the other modules do so when they compute
+_BLOCK_SCALED = frozenset((
+    "BlockScaledRows",
+    "block_multiplier",
+    "block_scaled_linear",
+    "block_scaled_mm",
+    "block_scaled_mm_expired",
+    "dequantize_blocks",
+    "quantize_blocks",
+))
+
+
+def __getattr__(name: str):
+    if name in _BLOCK_SCALED:
+        from . import blocks
+
+        globals().update({n: getattr(blocks, n) for n in _BLOCK_SCALED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
 
 __all__ = [
     "BlockScaledRows",

@@ -8,9 +8,11 @@ is missing every emulator entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libt5e.so"
+TORCH_LIB_PATH = LIB_PATH.with_name("t5e_torch.so")
 
 ABI_VERSION = 1
 
@@ -166,12 +168,6 @@ class BlockMm(ctypes.Structure):
     ]
 
 
-# The same structs for struct.pack, which fills one in a fraction of the time a
-# ctypes.Structure takes: a small call's time is the host's.
-BLOCKS_FORMAT = "PqPQqii"
-QUANTIZE_FORMAT = "PQQqiiPPii" + 2 * BLOCKS_FORMAT
-BLOCK_MM_FORMAT = 2 * BLOCKS_FORMAT + "PPfiPiiqqPq"
-
 # every symbol include/t5e.h declares
 EXPORTED = (
     "t5e_abi_version",
@@ -266,6 +262,29 @@ def load() -> ctypes.CDLL:
         raise NativeLibraryError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")
     _lib = lib
     return lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """Load (once) and return the PyTorch side of the block-scaled calls
+    (csrc/t5e_torch.cpp); raises when it is missing."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        if not TORCH_LIB_PATH.exists():
+            raise NativeLibraryError(f"{TORCH_LIB_PATH} is not built; run `python -m tcgen05_b200.build`")
+        import torch  # noqa: F401  (its libraries have to be in the process first)
+
+        spec = importlib.util.spec_from_file_location("t5e_torch", TORCH_LIB_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.abi_version != ABI_VERSION:
+            raise NativeLibraryError(f"{TORCH_LIB_PATH} has ABI version {module.abi_version}, expected {ABI_VERSION}; "
+                                     "rebuild it")
+        _torch_ops = module
+    return _torch_ops
 
 
 def check(rc: int, what: str) -> None:

@@ -4,6 +4,8 @@
 ``tcgen05_b200/_lib/libt5e.so`` with nvcc, for the B200 architecture only
 (``-gencode arch=compute_100a,code=sm_100a``).  The library links the CUDA
 runtime statically, so loading it needs no GPU and no CUDA library path.
+``csrc/t5e_torch.cpp`` becomes ``_lib/t5e_torch.so``, the PyTorch side of the
+block-scaled calls, against the installed PyTorch and that library.
 """
 
 from __future__ import annotations
@@ -19,6 +21,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libt5e.so"
+TORCH_SRC = CSRC / "t5e_torch.cpp"
+TORCH_LIB = LIB_DIR / "t5e_torch.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -36,8 +40,40 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
+def build_torch(verbose: bool = False, force: bool = False) -> Path:
+    """Compile the PyTorch side if its sources are newer; return its path."""
+    import sysconfig
+
+    import torch
+
+    deps = [TORCH_SRC, INCLUDE / "t5e.h"]
+    if not force and TORCH_LIB.exists() and all(TORCH_LIB.stat().st_mtime >= p.stat().st_mtime for p in deps):
+        return TORCH_LIB
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    home = Path(torch.__file__).resolve().parent
+    includes = [INCLUDE, sysconfig.get_paths()["include"], cuda, home / "include", home / "include/torch/csrc/api/include"]
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=t5e_torch",
+           *[arg for i in includes for arg in ("-isystem", str(i))], str(TORCH_SRC), "-o", str(tmp),
+           "-L", str(LIB_DIR), "-l:libt5e.so", "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+           "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 def build(verbose: bool = False, ptxas_info: bool = False, force: bool = False) -> Path:
-    """Compile the library if any source is newer than it; return its path."""
+    """Compile the libraries whose sources are newer than they are; return the
+    CUDA library's path."""
+    path = _build_cuda(verbose, ptxas_info, force)
+    build_torch(verbose, force)
+    return path
+
+
+def _build_cuda(verbose: bool, ptxas_info: bool, force: bool) -> Path:
     LIB_DIR.mkdir(exist_ok=True)
     srcs = sources()
     deps = srcs + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "t5e.h"]
