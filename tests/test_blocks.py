@@ -271,7 +271,7 @@ def test_empty_calls_launch_nothing():
 @pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
 @pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
 @pytest.mark.parametrize("rows,k", [(1, 1), (1, 15), (1, 16), (2, 17), (3, 32), (5, 33), (7, 100), (130, 64), (33, 257),
-                                    (257, 520), (1, 4096), (300, 1000)])
+                                    (257, 520), (1, 4096), (300, 1000), (300, 1001), (385, 393)])
 def test_rows_and_columns_round_as_defined(form, dtype, rows, k):
     x = make(rows * 7919 + k, rows, k, dtype=dtype, wide=True)
     for ceil in ((False, True) if form[0] == "ue8m0" else (False,)):
