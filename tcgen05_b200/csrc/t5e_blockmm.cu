@@ -124,6 +124,15 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, in
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
+// Into L2 only.
+__device__ __forceinline__ void fetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" :: "l"(map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void fetch_3d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];"
+               :: "l"(map), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 template <bool PAIR>
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
                                         uint32_t bar) {
@@ -238,6 +247,14 @@ __device__ __forceinline__ void write_real(void* p, int64_t i, int32_t type, flo
   else static_cast<__half*>(p)[i] = from_f32<T5E_REAL_F16>(v);
 }
 
+// The value of an element of C from its bits.
+template <int BYTES>
+__device__ __forceinline__ float c_value(const Params& P, uint32_t bits) {
+  if constexpr (BYTES == 4) return __uint_as_float(bits);
+  return P.c_type == T5E_REAL_BF16 ? __uint_as_float(bits << 16)
+                                   : __half2float(__ushort_as_half((unsigned short)bits));
+}
+
 // N neighbouring finished results of row p, columns q .. q + N - 1: vectors where
 // the row is aligned.
 template <int N>
@@ -299,29 +316,43 @@ __device__ __forceinline__ void store_results(const Params& P, float alpha, uint
 // A warp's 32 x 32 results by way of shared memory (a 32 x 33 buffer of its
 // own): lane r brings row p + r, columns q .. q + 31; the stores, and the loads
 // of C, then run along the rows, 32 neighbouring elements at a time, whatever
-// the alignment.
-template <int TYPE, bool ADD>
+// the alignment.  ADD: bytes of an element of C, 0 for none.
+template <int TYPE, int ADD>
 __device__ __forceinline__ void turned_rows(const Params& P, float alpha, uint32_t p, uint32_t col, int rows,
                                             const float* column) {
   using T = typename blocks::Real<TYPE>::type;
   T* dst = static_cast<T*>(P.d) + (int64_t)p * P.d_stride + col;
-  int64_t from = ADD ? (int64_t)p * P.c_p_stride + (int64_t)col * P.c_q_stride : 0;
-#pragma unroll 1
-  for (int r = 0; r < rows; r += 8) {  // eight rows' loads, then their stores
+  // C of all rows is on its way before the first is used
+  uint32_t add[ADD ? 32 : 1];
+  if constexpr (ADD > 0) {
+    const char* from = static_cast<const char*>(P.c) + ((int64_t)p * P.c_p_stride + (int64_t)col * P.c_q_stride) * ADD;
+#pragma unroll
+    for (int r = 0; r < 32; ++r, from += P.c_p_stride * ADD)
+      add[r] = r >= rows ? 0u : ADD == 4 ? *reinterpret_cast<const uint32_t*>(from)
+                                         : (uint32_t)*reinterpret_cast<const uint16_t*>(from);
+  }
+#pragma unroll
+  for (int r = 0; r < 32; r += 8) {
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = column[(r + j) * 33];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float add = 0.f;
-      if (ADD && r + j < rows) add = read_real(P.c, from + j * P.c_p_stride, P.c_type);
-      x[j] = ADD ? __fmaf_rn(x[j], alpha, add) : x[j] * alpha;
+      if constexpr (ADD > 0) x[j] = __fmaf_rn(x[j], alpha, c_value<ADD>(P, add[r + j]));
+      else x[j] *= alpha;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j, dst += P.d_stride)
       if (r + j < rows) *dst = from_f32<TYPE>(x[j]);
-    from += 8 * P.c_p_stride;
   }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void turned_type(const Params& P, float alpha, uint32_t p, uint32_t col, int rows,
+                                            const float* column) {
+  if (P.c == nullptr) turned_rows<TYPE, 0>(P, alpha, p, col, rows, column);
+  else if (P.c_type == T5E_REAL_F32) turned_rows<TYPE, 4>(P, alpha, p, col, rows, column);
+  else turned_rows<TYPE, 2>(P, alpha, p, col, rows, column);
 }
 
 __device__ __forceinline__ void store_turned(const Params& P, float alpha, uint32_t p, uint32_t q, const float* v,
@@ -334,22 +365,52 @@ __device__ __forceinline__ void store_turned(const Params& P, float alpha, uint3
   const uint32_t col = q + lane;
   if (col >= P.q_rows || p >= P.p_rows) return;
   const int rows = P.p_rows - p < 32u ? (int)(P.p_rows - p) : 32;
-  if (P.c != nullptr) {
-    if (P.d_type == T5E_REAL_F32) turned_rows<T5E_REAL_F32, true>(P, alpha, p, col, rows, buffer + lane);
-    else if (P.d_type == T5E_REAL_BF16) turned_rows<T5E_REAL_BF16, true>(P, alpha, p, col, rows, buffer + lane);
-    else turned_rows<T5E_REAL_F16, true>(P, alpha, p, col, rows, buffer + lane);
-  } else {
-    if (P.d_type == T5E_REAL_F32) turned_rows<T5E_REAL_F32, false>(P, alpha, p, col, rows, buffer + lane);
-    else if (P.d_type == T5E_REAL_BF16) turned_rows<T5E_REAL_BF16, false>(P, alpha, p, col, rows, buffer + lane);
-    else turned_rows<T5E_REAL_F16, false>(P, alpha, p, col, rows, buffer + lane);
+  if (P.d_type == T5E_REAL_F32) turned_type<T5E_REAL_F32>(P, alpha, p, col, rows, buffer + lane);
+  else if (P.d_type == T5E_REAL_BF16) turned_type<T5E_REAL_BF16>(P, alpha, p, col, rows, buffer + lane);
+  else turned_type<T5E_REAL_F16>(P, alpha, p, col, rows, buffer + lane);
+}
+
+// v = v * alpha + C for 64 columns of row p, C's rows being contiguous and on
+// 16-byte boundaries (or one row for all).
+template <int BYTES>
+__device__ __forceinline__ void add_row(const Params& P, float alpha, uint32_t p, uint32_t q, float* v) {
+  constexpr int kPer = 16 / BYTES;
+  const char* row = static_cast<const char*>(P.c) + ((int64_t)p * P.c_p_stride + q) * BYTES;
+  const bool there = p < P.p_rows;
+  uint4 w[64 / kPer];
+#pragma unroll
+  for (int j = 0; j < 64 / kPer; ++j) {
+    w[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (there && q + (j + 1) * kPer <= P.q_rows) {
+      w[j] = *(reinterpret_cast<const uint4*>(row) + j);
+    } else if (there && q + j * kPer < P.q_rows) {
+      uint32_t words[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (q + j * kPer + i < P.q_rows) {
+          if constexpr (BYTES == 4) words[i] = reinterpret_cast<const uint32_t*>(row)[j * kPer + i];
+          else words[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[j * kPer + i] << (16 * (i & 1));
+        }
+      }
+      w[j] = make_uint4(words[0], words[1], words[2], words[3]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 64 / kPer; ++j) {
+    const uint32_t words[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t raw = BYTES == 4 ? words[i] : (words[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+      v[j * kPer + i] = __fmaf_rn(v[j * kPer + i], alpha, c_value<BYTES>(P, raw));
+    }
   }
 }
 
-// A warp's 32 rows by 64 results, without C, through a box of 32 rows of 128 bytes
+// A warp's 32 rows by 64 finished results through a box of 32 rows of 128 bytes
 // that TMA writes (two boxes, one after the other, for F32): whole lines, and
 // swizzled as the map says, so that the lanes' 16-byte stores meet no bank twice.
-__device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* map, float alpha, uint32_t p, uint32_t q,
-                                          const float* v, uint8_t* box) {
+__device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* map, uint32_t p, uint32_t q, const float* v,
+                                          uint8_t* box) {
   const int lane = threadIdx.x & 31;
   const bool wide = P.d_type == T5E_REAL_F32;
 #pragma unroll
@@ -363,15 +424,14 @@ __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* ma
       uint4 w;
       if (wide) {
         const float* x = v + half * 32 + 4 * j;
-        w = make_uint4(__float_as_uint(x[0] * alpha), __float_as_uint(x[1] * alpha), __float_as_uint(x[2] * alpha),
-                       __float_as_uint(x[3] * alpha));
+        w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
       } else {
         const float* x = v + 8 * j;
         uint32_t h[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          h[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(x[2 * i] * alpha, x[2 * i + 1] * alpha)
-                                           : pack2<T5E_REAL_F16>(x[2 * i] * alpha, x[2 * i + 1] * alpha);
+          h[i] = P.d_type == T5E_REAL_BF16 ? pack2<T5E_REAL_BF16>(x[2 * i], x[2 * i + 1])
+                                           : pack2<T5E_REAL_F16>(x[2 * i], x[2 * i + 1]);
         w = make_uint4(h[0], h[1], h[2], h[3]);
       }
       *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) * 16)) = w;
@@ -400,13 +460,16 @@ __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* ma
 //              unit's two tcgen05.mma
 //
 // The scales have a ring and a thread of their own because a tcgen05.cp of 512
-// bytes takes about 32 cycles, and in one thread with the products it runs
-// between them: a 256 x 256 pair stage (512 cycles of products) spent 384 more on
-// its 12 copies.  From another thread they run beside the products, and run
-// ahead of the codes, so that a stage of codes is held no longer than its
-// load and its products take; what bounds the rate is the number of bytes in
-// flight (8192^3 in blocks of 16: 384 us with the copies between the
-// products, 328 with their own thread, measured before the separate ring).
+// bytes takes about 32 cycles, and issued by the products' thread it runs
+// between them: a 256 x 256 pair stage (512 cycles of products) spent 384 more
+// on its 12 copies.  From another thread the copies run beside the products, and
+// ahead of the codes, so that a stage of codes is held no longer than its load
+// and its products take.
+//
+// What is left of 8192^3 in blocks of 16, 202 us (5.4 PFLOP/s): the products
+// alone take 140 at the clock that the power limit leaves, the loads alone 145
+// (38 KB a stage of 512 cycles; an SM takes in 64 bytes a cycle); without the
+// scales' loads and copies it was 174 us, without storing results 9 us less.
 //
 // In a pair (PAIR) both blocks load their own parts, and the first block
 // spreads and issues for both; its barriers count the bytes of both, and its
@@ -691,17 +754,28 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_maps(T.maps);
   }
+  const uint32_t rank = blockIdx.x % split;
+  const uint32_t tile = blockIdx.x / split, p_tiles = (P.p_rows + 127u) >> 7;
+  const uint32_t p0 = tile % p_tiles * 128u, q0 = tile / p_tiles * (uint32_t)BN;
+  const uint32_t first = (uint32_t)((uint64_t)P.stages * rank / split);
+  const uint32_t last = (uint32_t)((uint64_t)P.stages * (rank + 1) / split);
+  if (SWAP && warp == 3 && elected()) {
+    // The first stages of the many-row operand (the weights) into L2 while the
+    // kernel before (the rounding of the few rows) still runs: L2 sees that
+    // kernel's writes, so this may come before the wait for it.  One token
+    // rounded and multiplied, 8192 x 8192: 13.0 -> 12.5 us; 8 or 32 stages gain
+    // no more.
+    for (uint32_t st = first; st < last && st < first + 4; ++st) {
+      fetch_2d(&T.maps.p, (int32_t)(st * kRowBytes), (int32_t)p0);
+      fetch_3d(&T.maps.ps, 0, (int32_t)(st * S::kGroups), (int32_t)(p0 >> 7));
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
   blocks::let_next_grid_start();
   blocks::wait_for_previous_grid();
   const uint32_t tmem = tmem_slot;
-  const uint32_t rank = blockIdx.x % split;
-  const uint32_t tile = blockIdx.x / split, p_tiles = (P.p_rows + 127u) >> 7;
-  const uint32_t p0 = tile % p_tiles * 128u, q0 = tile / p_tiles * (uint32_t)BN;
-  const uint32_t first = (uint32_t)((uint64_t)P.stages * rank / split);
-  const uint32_t last = (uint32_t)((uint64_t)P.stages * (rank + 1) / split);
   bool ok = true;
   if (elected()) {
     Use u, unit;
@@ -822,7 +896,7 @@ struct PairParams {
   CUtensorMap d_map;
   Params r;
   uint32_t p_tiles, q_tiles;
-  int32_t boxed;  // results leave through d_map: rows on 16-byte boundaries, no C
+  int32_t boxed;  // results leave through d_map: rows of D, and of C, on 16-byte boundaries
 };
 
 constexpr int kPairThreads = 384;  // warps 0-3 the roles, 4-11 the results: two warps for each 32 rows
@@ -932,7 +1006,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
         }
         const uint32_t q = q0 + chunk * 64;
         if (P.boxed) {
-          store_box(P.r, &P.d_map, alpha, p, q, v, box);
+          if (P.r.c == nullptr) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] *= alpha;
+          } else if (P.r.c_type == T5E_REAL_F32) {
+            add_row<4>(P.r, alpha, p + lane, q, v);
+          } else {
+            add_row<2>(P.r, alpha, p + lane, q, v);
+          }
+          store_box(P.r, &P.d_map, p, q, v, box);
         } else {
           store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
           store_turned(P.r, alpha, p, q + 32, v + 32, reinterpret_cast<float*>(box));
@@ -1143,7 +1225,9 @@ int launch_pair(const Params& params, const t5e_blocks& a, const t5e_blocks& b, 
   if (rc == T5E_OK) rc = raise_smem_limit<pair_kernel<BN, BLOCK>>(S::kSmem, "block product attribute");
   if (rc != T5E_OK) return rc;
   P.boxed = 0;
-  if (params.c == nullptr) {
+  const int c_bytes = params.c_type == T5E_REAL_F32 ? 4 : 2;
+  if (params.c == nullptr || (params.c_q_stride == 1 && (params.c_p_stride * c_bytes) % 16 == 0 &&
+                              (reinterpret_cast<uintptr_t>(params.c) & 15u) == 0)) {
     rc = encode_results(&P.d_map, params, &P.boxed);
     if (rc != T5E_OK) return rc;
   }
