@@ -466,10 +466,11 @@ __device__ __forceinline__ void store_box(const Params& P, const CUtensorMap* ma
 // ahead of the codes, so that a stage of codes is held no longer than its load
 // and its products take.
 //
-// What is left of 8192^3 in blocks of 16, 202 us (5.4 PFLOP/s): the products
-// alone take 140 at the clock that the power limit leaves, the loads alone 145
-// (38 KB a stage of 512 cycles; an SM takes in 64 bytes a cycle); without the
-// scales' loads and copies it was 174 us, without storing results 9 us less.
+// 8192^3 in blocks of 16 takes 202 to 206 us (5.3 to 5.4 PFLOP/s).  Repeating
+// each product 8 times puts the products alone at 140 at the clock that the
+// power limit leaves.  Of an earlier state that took 219: without the products
+// 179, without the scales' loads and copies 174, without both 130.  Results:
+// 8192 x 4096 x 4096, then 58.7 us, took 52.9 without storing them.
 //
 // In a pair (PAIR) both blocks load their own parts, and the first block
 // spreads and issues for both; its barriers count the bytes of both, and its
