@@ -948,3 +948,68 @@ def test_the_set_as_a_model_uses_it():
         # K = 256 and 384 are too short to be split, so one token sums in the order of a batch
         one = torch.cat([serve(x[i:i + 1]) for i in range(x.shape[0])])
         assert torch.equal(one, serve(x)) and torch.equal(one, whole)
+
+
+@pytest.mark.gpu
+def test_one_tensor_as_both_operands():
+    kw = dict(scaling="ue8m0")
+    for rows, k in ((1, 64), (130, 333), (700, 520)):
+        x = make(rows, rows, k, dtype=torch.bfloat16)
+        q, same = t5.quantize_blocks(x, **kw), t5.quantize_blocks(x.clone(), **kw)
+        assert torch.equal(t5.block_scaled_mm(q, q), t5.block_scaled_mm(q, same))
+    # one leaf as both: its gradient is the sum of the two
+    x = make(5, 96, 200, dtype=torch.float32)
+    g = make(6, 96, 96)
+    both, a, b = (x.clone().requires_grad_() for _ in range(3))
+    t5.block_scaled_linear(both, both).backward(g)
+    t5.block_scaled_linear(a, b).backward(g)
+    assert torch.equal(both.grad, a.grad + b.grad)
+
+
+@pytest.mark.gpu
+def test_inference_mode():
+    x, w = make(1, 70, 96, dtype=torch.bfloat16), make(2, 50, 96, dtype=torch.bfloat16)
+    want = t5.block_scaled_linear(x, w)
+    product = t5.block_scaled_mm(t5.quantize_blocks(x), t5.quantize_blocks(w))
+    with torch.inference_mode():
+        assert torch.equal(t5.block_scaled_linear(x, w), want)
+        held = t5.quantize_blocks(w)
+        assert torch.equal(t5.block_scaled_mm(t5.quantize_blocks(x.clone()), held), product)
+    # what was rounded there serves outside
+    assert torch.equal(t5.block_scaled_mm(t5.quantize_blocks(x), held), product)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["grad", "backward"])
+def test_captured_backward_beside_a_living_graph(how):
+    """An eager graph of the same leaves, made on a stream of its own, lives
+    while a training step is captured."""
+    x = make(1, 64, 256, dtype=torch.bfloat16).requires_grad_()
+    w = make(2, 128, 256, dtype=torch.bfloat16).requires_grad_()
+    g = make(3, 64, 128, dtype=torch.bfloat16)
+
+    def step():
+        y = t5.block_scaled_linear(x, w)
+        if how == "grad":
+            return torch.autograd.grad(y, (x, w), g)
+        x.grad = w.grad = None
+        y.backward(g)
+        return x.grad, w.grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in step()]
+        living = t5.block_scaled_linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in got:
+        t.fill_(7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    again = torch.autograd.grad(living, (x, w), g)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
