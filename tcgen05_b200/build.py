@@ -57,7 +57,10 @@ def build_torch(verbose: bool = False, force: bool = False) -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=t5e_torch",
            *[arg for i in includes for arg in ("-isystem", str(i))], str(TORCH_SRC), "-o", str(tmp),
            "-L", str(LIB_DIR), "-l:libt5e.so", "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-           "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_python",
+           # PyTorch's C++ library, whatever $CXX links by itself: a static copy has locale facets of its own, and the
+           # first message that a refused call prints through libc10 ends the process
+           "-nostdlib++", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
