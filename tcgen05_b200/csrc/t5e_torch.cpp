@@ -351,7 +351,9 @@ Tensor mm(const Rows& a, const Rows& b, const optional<Tensor>& addend, double a
 // ---- the linear layer ------------------------------------------------------------
 
 // Gradients that were computed from raw memory: differentiating them again is
-// refused (they would be constants to autograd).
+// refused (they would be constants to autograd, although dx depends on w and dw
+// on x).  `tie` is any tensor that requires a gradient, so that the node exists
+// whether the incoming gradient requires one or not.
 struct Once : torch::autograd::Function<Once> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, Tensor grad, const Tensor&) {
     return {grad};
@@ -432,8 +434,10 @@ struct Linear : torch::autograd::Function<Linear> {
       }
       // grad mode is on here only under create_graph=True
       if (at::GradMode::is_enabled()) {
-        if (dx.defined()) dx = Once::apply(dx, g)[0];
-        if (dw.defined()) dw = Once::apply(dw, g)[0];
+        Tensor tie = at::empty({0});
+        tie.set_requires_grad(true);
+        if (dx.defined()) dx = Once::apply(dx, tie)[0];
+        if (dw.defined()) dw = Once::apply(dw, tie)[0];
       }
     }
     return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
