@@ -267,6 +267,12 @@ void check_apart(const Tensor& out, const Rows& r, const char* name) {
                     "out overlaps ", name);
 }
 
+// Tells autograd, as PyTorch's own `out` arguments do, that `out` is written: a
+// graph that saved it refuses its backward pass.  Refuses an inference tensor
+// outside inference mode.  Called last before the launch, so that a refused call
+// leaves no trace.
+void note_written(const Tensor& out) { out.unsafeGetTensorImpl()->bump_version(); }
+
 void check_on_device(const Rows& r, const char* name) {
   TORCH_CHECK_VALUE(r.device.is_cuda(), name, " must be on a CUDA device (there is no CPU fallback)");
 }
@@ -277,7 +283,10 @@ Tensor dequantize(const Rows& r, at::ScalarType dtype, const optional<Tensor>& g
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(r.device);
   Tensor out = result(given, (int64_t)r.b.rows, r.b.k, dtype, r.device);
-  if (given) check_apart(out, r, "blocks");
+  if (given) {
+    check_apart(out, r, "blocks");
+    note_written(out);
+  }
   check(t5e_dequantize_blocks(&r.b, r.multiplier_ptr(), real_type(dtype), out.mutable_data_ptr(),
                               r.b.rows > 1 ? out.stride(0) : r.b.k, stream_of(r.device)),
         "t5e_dequantize_blocks");
@@ -342,6 +351,7 @@ Tensor mm(const Rows& a, const Rows& b, const optional<Tensor>& addend, double a
                         (m == 1 || c.stride(0) == out.stride(0)) && (n == 1 || c.stride(1) == out.stride(1));
       TORCH_CHECK_VALUE(!(cs.first < ds.second && ds.first < cs.second) || same, "c overlaps out without being out");
     }
+    note_written(out);
   }
   launch_product(a.b, b.b, a.multiplier_ptr(), b.multiplier_ptr(), (float)alpha, form, c.defined() ? &c : nullptr, out,
                  a.device);
