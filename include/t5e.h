@@ -30,7 +30,8 @@
 extern "C" {
 #endif
 
-#define T5E_ABI_VERSION 1
+/* 1: the emulator; 2: block-scaled E2M1 tensors */
+#define T5E_ABI_VERSION 2
 
 /* operand formats (tcgen05_model.normalize_format names) */
 enum {

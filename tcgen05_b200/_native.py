@@ -14,7 +14,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libt5e.so"
 TORCH_LIB_PATH = LIB_PATH.with_name("t5e_torch.so")
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 # operand formats
 FMT_TF32, FMT_BF16, FMT_F16, FMT_E4M3, FMT_E5M2, FMT_E2M3, FMT_E3M2, FMT_E2M1, FMT_U8, FMT_S8 = range(10)
@@ -208,8 +208,14 @@ def load() -> ctypes.CDLL:
             "(this package has no CPU fallback)"
         )
     lib = ctypes.CDLL(str(LIB_PATH))
+    # the version first: a library of another one may lack the functions below
+    if not hasattr(lib, "t5e_abi_version"):
+        raise NativeLibraryError(f"{LIB_PATH} is not the emulator library")
     lib.t5e_abi_version.restype = ctypes.c_int
     lib.t5e_abi_version.argtypes = []
+    version = lib.t5e_abi_version()
+    if version != ABI_VERSION:
+        raise NativeLibraryError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")
     lib.t5e_last_error.restype = ctypes.c_char_p
     lib.t5e_last_error.argtypes = []
     for name in ("t5e_mma_dot_batch", "t5e_mma_dot_batch_generic"):
@@ -257,9 +263,6 @@ def load() -> ctypes.CDLL:
     lib.t5e_block_scaled_mm.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     lib.t5e_block_scaled_mm_expired.restype = ctypes.c_int
     lib.t5e_block_scaled_mm_expired.argtypes = [ctypes.POINTER(ctypes.c_int32)]
-    version = lib.t5e_abi_version()
-    if version != ABI_VERSION:
-        raise NativeLibraryError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")
     _lib = lib
     return lib
 
