@@ -378,7 +378,9 @@ int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t co
  * A block with a NaN or an infinity gets the NaN scale and codes 0; a zero
  * scale gets codes that are zeros.  With partials != NULL (a workspace of
  * `count` words) the multiplier is first computed as by t5e_block_multiplier
- * and stored to *multiplier. */
+ * and stored to *multiplier.  With kept != NULL the multiplier that was used is
+ * also stored to *kept, for a caller whose *multiplier changes later.  Where
+ * there is no element nothing is stored. */
 typedef struct t5e_quantize {
     const void* x;
     uint64_t rows;
@@ -392,6 +394,7 @@ typedef struct t5e_quantize {
     int32_t reserved;            /* 0 */
     t5e_blocks by_rows;
     t5e_blocks by_cols;
+    float* kept;                 /* device scalar or NULL */
 } t5e_quantize;
 
 /* One tensor, or two of one type and one block form in the launches of one

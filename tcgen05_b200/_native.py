@@ -145,6 +145,7 @@ class Quantize(ctypes.Structure):
         ("reserved", ctypes.c_int32),
         ("by_rows", Blocks),
         ("by_cols", Blocks),
+        ("kept", ctypes.c_void_p),
     ]
 
 

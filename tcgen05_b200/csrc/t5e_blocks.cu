@@ -77,6 +77,7 @@ struct Job {
   uint64_t rows, cols;
   int64_t stride;
   float* multiplier;
+  float* kept;         // NULL, or where the multiplier is stored as well
   uint32_t* partials;  // NULL: the multiplier is given
   int32_t count;
   uint32_t first_block;
@@ -154,16 +155,20 @@ __global__ void __launch_bounds__(kThreads) multiplier_kernel(const uint32_t* __
 
 // The multiplier a quantising block works with: none, given, or taken from the
 // partial maxima (every block joins them for itself, which saves a launch; the
-// job's first block stores the result).
+// job's first block stores the result, and what is to be kept).
 __device__ __forceinline__ float load_multiplier(const Job& J, uint32_t* shared) {
+  const bool first = blockIdx.x == J.first_block && threadIdx.x == 0;
+  float m;
   if (J.partials != nullptr) {
     uint32_t best = 0u;
     for (int i = threadIdx.x; i < J.count; i += kThreads) best = max(best, J.partials[i]);
-    const float m = multiplier_of(block_max(best, shared));
-    if (blockIdx.x == J.first_block && threadIdx.x == 0) *J.multiplier = m;
-    return m;
+    m = multiplier_of(block_max(best, shared));
+    if (first) *J.multiplier = m;
+  } else {
+    m = J.multiplier != nullptr ? *J.multiplier : 1.f;
   }
-  return J.multiplier != nullptr ? *J.multiplier : 1.f;
+  if (first && J.kept != nullptr) *J.kept = m;
+  return m;
 }
 
 // n / d for n < 2^31: mul = floor(2^(31 + shift) / d) + 1 with 2^(shift-1) < d <=
@@ -949,6 +954,7 @@ int t5e_quantize_blocks(const t5e_quantize* q, int32_t n, void* stream) {
     J.cols = Q.cols;
     J.stride = Q.stride;
     J.multiplier = Q.multiplier;
+    J.kept = Q.kept;
     J.partials = Q.partials;
     J.count = Q.count;
     J.vec = rows_aligned(Q.type, Q.x, Q.rows, Q.stride);

@@ -151,7 +151,7 @@ int32_t partial_count(int64_t n) {
 }
 
 t5e_quantize job_of(const Matrix& m, int32_t rounding, float* multiplier, uint32_t* partials, int32_t count,
-                    const t5e_blocks* rows, const t5e_blocks* cols) {
+                    const t5e_blocks* rows, const t5e_blocks* cols, float* kept = nullptr) {
   if (m.turned) std::swap(rows, cols);
   t5e_quantize q{};
   q.x = m.x.const_data_ptr();
@@ -165,6 +165,7 @@ t5e_quantize job_of(const Matrix& m, int32_t rounding, float* multiplier, uint32
   q.count = count;
   if (rows) q.by_rows = *rows;
   if (cols) q.by_cols = *cols;
+  q.kept = kept;
   return q;
 }
 
@@ -187,6 +188,9 @@ Tensor multiplier_of(const Tensor& x0) {
 enum { kByRows = 1, kByCols = 2 };
 
 // The rows and the columns of x that `axes` asks for (the other stays empty).
+// The blocks keep the value that `given` has now, not the caller's tensor: a
+// program may update it in place, and what was rounded before stands as it was.
+// The rounding kernel copies it (a copy of its own would be another launch).
 std::pair<Rows, Rows> quantize(const Tensor& x, int axes, int32_t fmt, int32_t block, int32_t rounding,
                                const optional<Tensor>& given, bool automatic) {
   check_real(x, "x");
@@ -201,13 +205,14 @@ std::pair<Rows, Rows> quantize(const Tensor& x, int axes, int32_t fmt, int32_t b
   TORCH_CHECK_VALUE(!(by_cols && r == 0), "blocks along an empty axis");
   const c10::Device device = x.device();
   const c10::cuda::CUDAGuard guard(device);
-  Tensor multiplier;
+  Tensor source, multiplier;  // `source`: the given one
   uint32_t* partials = nullptr;
   int32_t count = 0;
   if (given) {
-    multiplier = *given;
-    TORCH_CHECK_VALUE(multiplier.scalar_type() == at::kFloat && multiplier.numel() == 1 && multiplier.device() == device,
+    TORCH_CHECK_VALUE(given->scalar_type() == at::kFloat && given->numel() == 1 && given->device() == device,
                       "multiplier must be a one-element float32 tensor on x's device");
+    source = given->resolve_neg();
+    multiplier = r > 0 ? at::empty({1}, x.options().dtype(at::kFloat)) : source.reshape({1}).clone();
   } else if (automatic && r > 0) {
     count = partial_count(r * k);
     const Tensor work = at::empty({1 + count}, x.options().dtype(at::kFloat));
@@ -219,8 +224,9 @@ std::pair<Rows, Rows> quantize(const Tensor& x, int axes, int32_t fmt, int32_t b
   if (by_cols) out.second = new_rows(device, k, r, fmt, block, multiplier);
   if (r > 0) {
     const Matrix m = matrix_of(x);
-    const t5e_quantize q = job_of(m, rounding, multiplier.defined() ? multiplier.mutable_data_ptr<float>() : nullptr, partials,
-                                  count, by_rows ? &out.first.b : nullptr, by_cols ? &out.second.b : nullptr);
+    float* const at = multiplier.defined() ? multiplier.mutable_data_ptr<float>() : nullptr;
+    const t5e_quantize q = job_of(m, rounding, given ? const_cast<float*>(source.const_data_ptr<float>()) : at, partials, count,
+                                  by_rows ? &out.first.b : nullptr, by_cols ? &out.second.b : nullptr, given ? at : nullptr);
     check(t5e_quantize_blocks(&q, 1, stream_of(device)), "t5e_quantize_blocks");
   }
   return out;
