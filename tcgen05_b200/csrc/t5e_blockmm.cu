@@ -289,20 +289,60 @@ __device__ __forceinline__ void store_plain(const Params& P, uint32_t p, uint32_
     if (i < count) write_real(P.d, at + i, P.d_type, v[i]);
 }
 
+// What sums are multiplied by, alpha * (1 / ma) * (1 / mb): one F32 number,
+// except where that product, or its first step, leaves the normal F32 range
+// although the results need not (both tensors near 2^76: the product is infinite
+// and turned rows of zeros into NaN; near 2^-65: it is zero, and so were results
+// of 2^-118).  There the factor keeps its digits in `alpha`, at the end of the F32
+// range, and sums are first multiplied by the powers of two `by` and `by2`, which
+// is exact wherever the result is not beyond F32 anyway.
+struct Factor {
+  float alpha, by, by2;  // by = 1: alpha alone
+};
+
+__device__ __forceinline__ Factor factor_of(const Params& P) {
+  const float ra = P.multiplier_a != nullptr ? 1.f / *P.multiplier_a : 1.f;
+  const float rb = P.multiplier_b != nullptr ? 1.f / *P.multiplier_b : 1.f;
+  const float first = P.alpha * ra, joint = first * rb;
+  const auto normal = [](float v) { return ((__float_as_uint(v) >> 23) & 0xFFu) - 1u < 254u; };
+  Factor f = {joint, 1.f, 1.f};
+  if (normal(first) && normal(joint)) return f;
+  const double whole = (double)P.alpha * ra * rb;  // three F32 numbers: within F64's range
+  const int e = (int)((__double_as_longlong(whole) >> 52) & 0x7FF) - 1023;
+  if (whole == 0. || e == 1024) {
+    f.alpha = (float)whole;
+    return f;
+  }
+  const int s = e < -126 ? e + 126 : e > 126 ? e - 126 : 0, part = s < -126 ? -126 : s > 127 ? 127 : s;
+  const int rest = s - part < -126 ? -126 : s - part > 127 ? 127 : s - part;  // beyond: zero or infinite without it
+  f.alpha = (float)(whole * __longlong_as_double((long long)(1023 - s) << 52));
+  f.by = __uint_as_float((uint32_t)(part + 127) << 23);
+  f.by2 = __uint_as_float((uint32_t)(rest + 127) << 23);
+  return f;
+}
+
+template <int N>
+__device__ __forceinline__ void rescale(const Factor& f, float* v) {
+  if (f.by == 1.f) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = v[i] * f.by * f.by2;
+}
+
 // N neighbouring results of row p of the tile grid, columns q .. q + count - 1:
 // scales them, adds C and stores them.  SWAP: D is contiguous along p (lanes
 // store neighbouring elements), otherwise along q (a lane stores vectors).
 template <bool SWAP, int N>
-__device__ __forceinline__ void store_results(const Params& P, float alpha, uint32_t p, uint32_t q, int count,
+__device__ __forceinline__ void store_results(const Params& P, const Factor& f, uint32_t p, uint32_t q, int count,
                                               float (&v)[N]) {
   if (p >= P.p_rows) return;
+  rescale<N>(f, v);
   if (q + count > P.q_rows) count = q >= P.q_rows ? 0 : (int)(P.q_rows - q);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float add = 0.f;
     if (P.c != nullptr && i < count)
       add = read_real(P.c, (int64_t)p * P.c_p_stride + (int64_t)(q + i) * P.c_q_stride, P.c_type);
-    v[i] = P.c != nullptr ? __fmaf_rn(v[i], alpha, add) : v[i] * alpha;
+    v[i] = P.c != nullptr ? __fmaf_rn(v[i], f.alpha, add) : v[i] * f.alpha;
   }
   if constexpr (SWAP) {
 #pragma unroll
@@ -705,7 +745,7 @@ struct TileParams {
 // Adds the parts of N columns of a row, in rank order, and stores the results.
 // `here` is the address of the row's first column in this block's part.
 template <bool SWAP, int N>
-__device__ __forceinline__ void join_parts(const Params& P, float alpha, uint32_t split, uint32_t here, uint32_t p,
+__device__ __forceinline__ void join_parts(const Params& P, const Factor& f, uint32_t split, uint32_t here, uint32_t p,
                                            uint32_t q) {
   float v[N];
 #pragma unroll
@@ -728,7 +768,7 @@ __device__ __forceinline__ void join_parts(const Params& P, float alpha, uint32_
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (v[i] + x[0][i]) + x[1][i];
   }
-  store_results<SWAP, N>(P, alpha, p, q, N, v);
+  store_results<SWAP, N>(P, f, p, q, N, v);
 }
 
 template <int BN, int BLOCK, bool SWAP>
@@ -800,8 +840,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   const bool bad = __syncthreads_or(!ok);
   if (bad && t == 0) atomicExch(&g_expired, 1);
   const float nan = __uint_as_float(0x7FC00000u);
-  const float alpha = P.alpha * (P.multiplier_a != nullptr ? 1.f / *P.multiplier_a : 1.f) *
-                      (P.multiplier_b != nullptr ? 1.f / *P.multiplier_b : 1.f);
+  const Factor f = factor_of(P);
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   if (split == 1u && !SWAP && BN >= 32) {
     // the stages are free: 32 x 33 floats of them for each warp
@@ -816,7 +855,8 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = nan;
       }
-      store_turned(P, alpha, p0 + warp * 32u, q0 + q, v, buffer);
+      rescale<32>(f, v);
+      store_turned(P, f.alpha, p0 + warp * 32u, q0 + q, v, buffer);
     }
   } else if (split == 1u) {
 #pragma unroll 1
@@ -828,7 +868,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = nan;
       }
-      store_results<SWAP, 16>(P, alpha, p0 + t, q0 + q, 16, v);
+      store_results<SWAP, 16>(P, f, p0 + t, q0 + q, 16, v);
     }
   } else {
     // four columns of a row side by side, so that both sides move 16 bytes a lane
@@ -848,12 +888,12 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
 #pragma unroll 1
       for (int q = w0; q < w0 + width; q += 8) {
         if (q0 + q >= P.q_rows) break;
-        join_parts<SWAP, 8>(P, alpha, split, smem_u32(part + q / 4 * 128 + t), p0 + t, q0 + q);
+        join_parts<SWAP, 8>(P, f, split, smem_u32(part + q / 4 * 128 + t), p0 + t, q0 + q);
       }
     } else if (width == 4) {
-      join_parts<SWAP, 4>(P, alpha, split, smem_u32(part + w0 / 4 * 128 + t), p0 + t, q0 + w0);
+      join_parts<SWAP, 4>(P, f, split, smem_u32(part + w0 / 4 * 128 + t), p0 + t, q0 + w0);
     } else {
-      join_parts<SWAP, 2>(P, alpha, split, smem_u32(part + w0 / 4 * 128 + t) + w0 % 4 * 4, p0 + t, q0 + w0);
+      join_parts<SWAP, 2>(P, f, split, smem_u32(part + w0 / 4 * 128 + t) + w0 % 4 * 4, p0 + t, q0 + w0);
     }
     cluster_sync();
   }
@@ -975,8 +1015,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
     }
   } else {
     const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
-    const float alpha = P.r.alpha * (P.r.multiplier_a != nullptr ? 1.f / *P.r.multiplier_a : 1.f) *
-                        (P.r.multiplier_b != nullptr ? 1.f / *P.r.multiplier_b : 1.f);
+    const Factor f = factor_of(P.r);
     const int side = warp >= 8;     // of the two warps of these lanes: every other chunk
     uint8_t* box = boxes + (quarter * 2 + side) * L::kBoxBytes;
     uint32_t count = 0;
@@ -1005,20 +1044,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
+        rescale<64>(f, v);
         const uint32_t q = q0 + chunk * 64;
         if (P.boxed) {
           if (P.r.c == nullptr) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] *= alpha;
+            for (int j = 0; j < 64; ++j) v[j] *= f.alpha;
           } else if (P.r.c_type == T5E_REAL_F32) {
-            add_row<4>(P.r, alpha, p + lane, q, v);
+            add_row<4>(P.r, f.alpha, p + lane, q, v);
           } else {
-            add_row<2>(P.r, alpha, p + lane, q, v);
+            add_row<2>(P.r, f.alpha, p + lane, q, v);
           }
           store_box(P.r, &P.d_map, p, q, v, box);
         } else {
-          store_turned(P.r, alpha, p, q, v, reinterpret_cast<float*>(box));
-          store_turned(P.r, alpha, p, q + 32, v + 32, reinterpret_cast<float*>(box));
+          store_turned(P.r, f.alpha, p, q, v, reinterpret_cast<float*>(box));
+          store_turned(P.r, f.alpha, p, q + 32, v + 32, reinterpret_cast<float*>(box));
         }
       };
       if constexpr (L::kShared > 0) {

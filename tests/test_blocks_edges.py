@@ -3,11 +3,15 @@ value in the tensors' own types."""
 
 from __future__ import annotations
 
+import math
+
+import numpy as np
 import pytest
 import torch
 
 import tcgen05_b200 as t5
-from test_blocks import make
+from tcgen05_b200 import blocks as bk
+from test_blocks import make, product_bound
 
 # ------------------------------------------------------------ what is kept
 
@@ -52,3 +56,84 @@ def test_a_captured_call_keeps_the_multiplier_of_its_replay():
         scale.fill_(77.0)
         assert float(q.multiplier) == m
         assert torch.equal(t5.dequantize_blocks(q), t5.dequantize_blocks(t5.quantize_blocks(x, multiplier=m)))
+
+
+# ------------------------------------------------------------ extreme factors
+
+
+def extremes(seed, rows, k, power, dtype=torch.float32):
+    """Normal values times 2^power, every third row zeros."""
+    x = make(seed, rows, k, dtype=torch.float32).clamp(-3, 3)
+    x[::3] = 0
+    return (x.double() * 2.0 ** power).to(dtype)
+
+
+def check_factors(qa, qb, alpha, dtype, c, form):
+    """A product against its definition in 64 bits, the multipliers powers of two."""
+    bare = [t5.BlockScaledRows(q.data, q.scales, q.k, scaling=q.scaling, scale_vec=q.scale_vec) for q in (qa, qb)]
+    a, b = (t5.dequantize_blocks(q).double() for q in bare)
+    factor = float(np.float32(alpha))
+    for q in (qa, qb):
+        factor /= 1.0 if q.multiplier is None else float(q.multiplier)
+    want = factor * (a @ b.t()) + (0 if c is None else c.double())
+    got = bk._mm(qa, qb, c, alpha, dtype, None, form).double()
+    info = torch.finfo(dtype)
+    err = abs(factor) * product_bound(a, b, qa.k, 0) + 2.0 ** -24 * (0 if c is None else c.double().abs())
+    room = err + 1.01 * info.eps / 2 * (want.abs() + err) + info.smallest_normal * info.eps
+    inside = want.abs() + room < info.max
+    beyond = want.abs() - room > 2 * info.max
+    assert bool(((got - want).abs() <= room)[inside].all())
+    assert torch.equal(got[beyond], torch.sign(want[beyond]) * math.inf)
+    assert not bool(got.isnan().any())
+    return inside, beyond
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [0, 1, 2, 4, 8, 128, 256])
+@pytest.mark.parametrize("m,n", [(300, 264), (260, 130), (5, 300)])
+def test_factors_whose_product_leaves_f32(form, m, n):
+    """alpha and the two reciprocals are no single F32 number: zero rows stay zero beside ones that overflow, and
+    results within F32 keep their digits."""
+    if m == 5 and form >= 128:
+        pytest.skip("few rows take no such tile")
+    k = 2100
+    cases = [(76, 76, 1.0), (100, 100, 1.0), (115, 20, 1.0), (-65, -65, 1.0), (-66, -60, 1.0), (-60, -60, 1.37e-5),
+             (66, -66, 2.0 ** 100), (-66, 66, 2.0 ** 100), (-40, 66, 1.37 * 2.0 ** -100), (50, 50, -1.37 * 2.0 ** -120),
+             (-50, -50, 1.37 * 2.0 ** 120), (60, 60, 0.0)]
+    for pa, pb, alpha in cases:
+        qa = t5.quantize_blocks(extremes(1, m, k, pa), multiplier="auto")
+        qb = t5.quantize_blocks(extremes(2, n, k, pb), multiplier="auto")
+        for dtype in (torch.float32, torch.bfloat16):
+            for c in (None, make(3, m, n), make(4, n, dtype=torch.bfloat16), make(5, n, m).t()):
+                check_factors(qa, qb, alpha, dtype, c, form)
+
+
+@pytest.mark.gpu
+def test_a_sum_with_c_that_only_the_sum_brings_into_range():
+    """alpha * sum beyond F32 and C of the other sign: one rounding, of the sum."""
+    a = t5.quantize_blocks(torch.full((200, 64), 6.0, device="cuda"), scaling="ue8m0")
+    b = t5.quantize_blocks(torch.full((200, 64), 6.0, device="cuda"), scaling="ue8m0")
+    c = torch.full((200, 200), -1.5 * 2.0 ** 127, device="cuda")
+    alpha = 2.0 ** 127 / 1152  # 64 * 36 = 2304: the product is 2^128
+    for form in (1, 128, 256):
+        got = bk._mm(a, b, c, alpha, torch.float32, None, form)
+        assert bool((got.double() - 2.0 ** 126).abs().max() <= 2.0 ** 126 * 2.0 ** -20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_of_large_and_small_tensors(dtype):
+    """Zero rows beside values whose products overflow; small values whose products do not vanish."""
+    for power in (80, -64):
+        x, w, g = (extremes(i, 66, 128, power, dtype).requires_grad_(i < 2) for i in range(3))
+        g = g[:, :66].contiguous()
+        y = t5.block_scaled_linear(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        assert not bool(y[::3].any()) and not bool(y[:, ::3].any())
+        for t in (y, dx, dw):
+            assert not bool(t.isnan().any())
+        if power < 0:
+            r = [t5.dequantize_blocks(t5.quantize_blocks(t.detach(), multiplier="auto")).double() for t in (x, w)]
+            want = r[0] @ r[1].t()
+            room = product_bound(*r, 128, 0) + 1.01 * torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -133
+            assert bool(want.any()) and bool(((y.double() - want).abs() <= room).all())
