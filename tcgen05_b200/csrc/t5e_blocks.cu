@@ -682,9 +682,22 @@ __device__ __forceinline__ void open_rows(const uint8_t* __restrict__ data, int6
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         const float s = scale_value<E8M0>((bytes[i] >> (8 * b)) & 0xFFu);
-        const float f = FOLD ? s * back : s;
+        if constexpr (FOLD) {
+          const float f = s * back;
 #pragma unroll
-        for (int j = 0; j < BLOCK; ++j) v[b * BLOCK + j] = FOLD ? v[b * BLOCK + j] * f : v[b * BLOCK + j] * f * back;
+          for (int j = 0; j < BLOCK; ++j) v[b * BLOCK + j] *= f;
+        } else if constexpr (E8M0) {
+          // a code times a scale of 2^126 or more may be beyond F32 where the
+          // value is not: what the scale has above 2^64 comes last (a product
+          // up to there is at least 2^-65 in front of it, so nothing is lost)
+          const bool far = s > 0x1p64f;
+          const float f = far ? 0x1p64f : s, rest = far ? s * 0x1p-64f : 1.f;
+#pragma unroll
+          for (int j = 0; j < BLOCK; ++j) v[b * BLOCK + j] = v[b * BLOCK + j] * f * back * rest;
+        } else {
+#pragma unroll
+          for (int j = 0; j < BLOCK; ++j) v[b * BLOCK + j] = v[b * BLOCK + j] * s * back;
+        }
       }
       const int64_t at = (int64_t)(row0 + row[i]) * out_stride + e0[i];
       if constexpr (VEC) {

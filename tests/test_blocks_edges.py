@@ -11,7 +11,7 @@ import torch
 
 import tcgen05_b200 as t5
 from tcgen05_b200 import blocks as bk
-from test_blocks import make, product_bound
+from test_blocks import E2M1, make, product_bound
 
 # ------------------------------------------------------------ what is kept
 
@@ -137,3 +137,24 @@ def test_linear_of_large_and_small_tensors(dtype):
             want = r[0] @ r[1].t()
             room = product_bound(*r, 128, 0) + 1.01 * torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -133
             assert bool(want.any()) and bool(((y.double() - want).abs() <= room).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vec", [2, 4])
+def test_values_whose_scale_alone_leaves_f32(vec):
+    """code * scale / multiplier where code * scale is beyond F32 and the value is not."""
+    k = 96
+    words = torch.arange(16, dtype=torch.int32, device="cuda").repeat(255, k // 16)
+    scales = torch.arange(255, dtype=torch.uint8, device="cuda")[:, None].repeat(1, k // (32 if vec == 2 else 16))
+    value = torch.tensor(E2M1 + [-v for v in E2M1], dtype=torch.float64, device="cuda")[words.long()]
+    exact = value * torch.exp2(torch.arange(255, dtype=torch.float64, device="cuda") - 127)[:, None]
+    for m in (None, 1.0, 4.0, 2.0 ** 100, 2.0 ** -100, 2.0 ** 126, 2.0 ** -126, 3.0, 1e-30, 7e37):
+        mult = None if m is None else torch.full((1,), m, device="cuda")
+        q = t5.BlockScaledRows.from_words(words, scales, scaling="ue8m0", scale_vec=vec, multiplier=mult)
+        back = 1.0 if m is None else float(np.float32(1) / np.float32(m))
+        want = exact * back
+        for dtype in (torch.float32, torch.bfloat16):
+            out = torch.zeros(255, k + 3, dtype=dtype, device="cuda")[:, 1:k + 1]
+            for got in (t5.dequantize_blocks(q, dtype=dtype), t5.dequantize_blocks(q, dtype=dtype, out=out)):
+                # F32 first, then the type, by the definition
+                np.testing.assert_array_equal(got.double().cpu().numpy(), want.float().to(dtype).double().cpu().numpy())
