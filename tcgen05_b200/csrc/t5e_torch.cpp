@@ -49,19 +49,38 @@ struct Rows {
   Tensor buffer;        // the rows, then the scale tiles; or undefined, and
   Tensor data, scales;  // two tensors of a caller's
   Tensor multiplier;    // undefined: 1
+  const float* factor = nullptr;  // where the multiplier lies
   c10::Device device{c10::kCPU};
 
+  // Refuses rows whose memory is no longer where the calls take it: a storage can
+  // be freed, grown or exchanged under a tensor that somebody still holds.
+  void check_there(const char* name) const {
+    const auto holds = [](const Tensor& t, const void* p, int64_t bytes) {
+      return bytes == 0 || (t.const_data_ptr() == p &&
+                            (int64_t)t.storage().nbytes() >= t.storage_offset() * (int64_t)t.itemsize() + bytes);
+    };
+    const int64_t codes = (int64_t)b.rows * b.stride, steps = scale_bytes((int64_t)b.rows, b.k, b.scale_block);
+    const bool there = buffer.defined() ? holds(buffer, b.data, codes + steps)
+                                        : holds(data, b.data, codes) && holds(scales, b.scales, steps);
+    TORCH_CHECK_VALUE(there && (!multiplier.defined() || holds(multiplier, factor, 4)), "the memory of ", name,
+                      " was freed or moved since they were made");
+  }
   Tensor get_data() const {
+    check_there("the rows");
     if (data.defined()) return data;
     return buffer.narrow(0, 0, (int64_t)b.rows * b.stride).view({(int64_t)b.rows, b.stride});
   }
   Tensor get_scales() const {
+    check_there("the rows");
     if (scales.defined()) return scales;
     const int64_t at = (int64_t)b.rows * b.stride;
     return buffer.narrow(0, at, buffer.size(0) - at)
         .view({((int64_t)b.rows + 127) / 128, (b.k + 4 * b.scale_block - 1) / (4 * b.scale_block), 512});
   }
-  const float* multiplier_ptr() const { return multiplier.defined() ? multiplier.const_data_ptr<float>() : nullptr; }
+  void keep_multiplier(const Tensor& m) {
+    multiplier = m;
+    factor = m.defined() ? m.const_data_ptr<float>() : nullptr;
+  }
 };
 
 t5e_blocks blocks_at(char* at, int64_t rows, int64_t k, int32_t fmt, int32_t block) {
@@ -84,7 +103,7 @@ Rows new_rows(const c10::Device& device, int64_t rows, int64_t k, int32_t fmt, i
   Rows r;
   r.buffer = bytes_on(device, blocks_size(rows, k, block));
   r.b = blocks_at(static_cast<char*>(r.buffer.data_ptr()), rows, k, fmt, block);
-  r.multiplier = multiplier;
+  r.keep_multiplier(multiplier);
   r.device = device;
   return r;
 }
@@ -112,7 +131,7 @@ Rows given_rows(const Tensor& data, const Tensor& scales, int64_t k, int32_t fmt
   Rows r;
   r.data = data;
   r.scales = scales;
-  if (multiplier) r.multiplier = *multiplier;
+  if (multiplier) r.keep_multiplier(multiplier->resolve_neg());
   r.device = data.device();
   r.b.data = data.data_ptr();
   r.b.stride = stride;
@@ -284,6 +303,7 @@ void check_on_device(const Rows& r, const char* name) {
 }
 
 Tensor dequantize(const Rows& r, at::ScalarType dtype, const optional<Tensor>& given) {
+  r.check_there("blocks");
   check_on_device(r, "blocks");
   TORCH_CHECK_VALUE(real_type(dtype) >= 0, "dtype must be float32, bfloat16 or float16, not ", dtype);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -293,7 +313,7 @@ Tensor dequantize(const Rows& r, at::ScalarType dtype, const optional<Tensor>& g
     check_apart(out, r, "blocks");
     note_written(out);
   }
-  check(t5e_dequantize_blocks(&r.b, r.multiplier_ptr(), real_type(dtype), out.mutable_data_ptr(),
+  check(t5e_dequantize_blocks(&r.b, r.factor, real_type(dtype), out.mutable_data_ptr(),
                               r.b.rows > 1 ? out.stride(0) : r.b.k, stream_of(r.device)),
         "t5e_dequantize_blocks");
   return out;
@@ -322,6 +342,8 @@ void launch_product(const t5e_blocks& a, const t5e_blocks& b, const float* ma, c
 
 Tensor mm(const Rows& a, const Rows& b, const optional<Tensor>& addend, double alpha, at::ScalarType dtype,
           const optional<Tensor>& given, int32_t form) {
+  a.check_there("a");
+  b.check_there("b");
   check_on_device(a, "a");
   check_on_device(b, "b");
   TORCH_CHECK_VALUE(a.b.scale_format == b.b.scale_format && a.b.scale_block == b.b.scale_block,
@@ -359,7 +381,7 @@ Tensor mm(const Rows& a, const Rows& b, const optional<Tensor>& addend, double a
     }
     note_written(out);
   }
-  launch_product(a.b, b.b, a.multiplier_ptr(), b.multiplier_ptr(), (float)alpha, form, c.defined() ? &c : nullptr, out,
+  launch_product(a.b, b.b, a.factor, b.factor, (float)alpha, form, c.defined() ? &c : nullptr, out,
                  a.device);
   return out;
 }

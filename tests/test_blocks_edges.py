@@ -158,3 +158,42 @@ def test_values_whose_scale_alone_leaves_f32(vec):
             for got in (t5.dequantize_blocks(q, dtype=dtype), t5.dequantize_blocks(q, dtype=dtype, out=out)):
                 # F32 first, then the type, by the definition
                 np.testing.assert_array_equal(got.double().cpu().numpy(), want.float().to(dtype).double().cpu().numpy())
+
+
+# ------------------------------------------------------------ aliases and moved memory
+
+
+def held_parts(device):
+    data = torch.zeros(130, 48, dtype=torch.uint8, device=device)
+    scales = torch.zeros(2, 2, 512, dtype=torch.uint8, device=device)
+    return data, scales, torch.ones(1, device=device)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("part", [0, 1, 2])
+@pytest.mark.parametrize("how", ["free", "grow", "set"])
+def test_rows_whose_memory_was_moved_are_refused(device, part, how):
+    """The parts' storage freed (as sharded training does between uses), grown, or exchanged: no call may use the
+    addresses of before."""
+    parts = held_parts(device)
+    q = t5.BlockScaledRows(parts[0], parts[1], 96, multiplier=parts[2])
+    t = parts[part]
+    if how == "free":
+        t.untyped_storage().resize_(0)
+    elif how == "grow":
+        t.resize_(1 << 20)
+    else:
+        t.set_(torch.zeros_like(t))
+    for call in (lambda: t5.dequantize_blocks(q), lambda: t5.block_scaled_mm(q, q)):
+        with pytest.raises(ValueError, match="moved"):
+            call()
+
+
+@pytest.mark.gpu
+def test_rounded_rows_whose_memory_was_freed_are_refused():
+    q = t5.quantize_blocks(make(1, 40, 64))
+    t5.block_scaled_mm(q, q)
+    q.data.untyped_storage().resize_(0)
+    for call in (lambda: t5.dequantize_blocks(q), lambda: t5.block_scaled_mm(q, q), lambda: q.scales, lambda: q.data):
+        with pytest.raises(ValueError, match="moved"):
+            call()
