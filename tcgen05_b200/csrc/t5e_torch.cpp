@@ -279,7 +279,8 @@ Tensor result(const optional<Tensor>& out, int64_t rows, int64_t cols, at::Scala
   return *out;
 }
 
-// Refuses an `out` that shares memory with the blocks it is computed from.
+// Refuses an `out` that shares memory with the blocks it is computed from, or
+// with their multiplier, which every block of a kernel reads for itself.
 void check_apart(const Tensor& out, const Rows& r, const char* name) {
   if (out.numel() == 0) return;
   const auto d = span_of(out);
@@ -288,7 +289,8 @@ void check_apart(const Tensor& out, const Rows& r, const char* name) {
     return at < d.second && d.first < at + (uintptr_t)n;
   };
   TORCH_CHECK_VALUE(!overlaps(r.b.data, (int64_t)r.b.rows * r.b.stride) &&
-                        !overlaps(r.b.scales, scale_bytes((int64_t)r.b.rows, r.b.k, r.b.scale_block)),
+                        !overlaps(r.b.scales, scale_bytes((int64_t)r.b.rows, r.b.k, r.b.scale_block)) &&
+                        !(r.factor != nullptr && overlaps(r.factor, sizeof(float))),
                     "out overlaps ", name);
 }
 

@@ -163,6 +163,21 @@ def test_values_whose_scale_alone_leaves_f32(vec):
 # ------------------------------------------------------------ aliases and moved memory
 
 
+@pytest.mark.gpu
+def test_out_may_not_hold_a_multiplier():
+    x = make(1, 40, 64)
+    q = t5.quantize_blocks(x)
+    big = torch.ones(40, 64, device="cuda")
+    held = t5.BlockScaledRows(q.data, q.scales, 64, multiplier=big[3, 5:6])
+    other = t5.quantize_blocks(make(2, 64, 64))
+    for call in (lambda: t5.dequantize_blocks(held, out=big),
+                 lambda: t5.block_scaled_mm(held, other, dtype=torch.float32, out=big),
+                 lambda: t5.block_scaled_mm(other, held, dtype=torch.float32, out=torch.as_strided(big, (64, 40), (40, 1)))):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+    assert bool((big == 1).all())
+
+
 def held_parts(device):
     data = torch.zeros(130, 48, dtype=torch.uint8, device=device)
     scales = torch.zeros(2, 2, 512, dtype=torch.uint8, device=device)
