@@ -35,6 +35,12 @@ void check_real(const Tensor& x, const char* name) {
                     " must be a dense tensor on a CUDA device (there is no CPU fallback)");
 }
 
+// Forward-mode derivatives are not computed: an input's would be lost, an
+// output's would no longer fit its value.
+void check_no_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), name, " must not carry a forward-mode tangent");
+}
+
 void* stream_of(const c10::Device& d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
 
 int64_t row_stride(int64_t k) { return (k + 31) / 32 * 16; }
@@ -275,6 +281,7 @@ Tensor result(const optional<Tensor>& out, int64_t rows, int64_t cols, at::Scala
   TORCH_CHECK_VALUE(out->numel() == 0 || ((cols == 1 || out->stride(1) == 1) && (rows == 1 || out->stride(0) >= cols)),
                     "out must have unit column stride and rows that do not overlap");
   TORCH_CHECK_VALUE(!(out->requires_grad() && at::GradMode::is_enabled()), "out must not require a gradient");
+  check_no_tangent(*out, "out");
   TORCH_CHECK_VALUE(!out->is_neg(), "out must not be a negated view");
   return *out;
 }
@@ -361,6 +368,7 @@ Tensor mm(const Rows& a, const Rows& b, const optional<Tensor>& addend, double a
     TORCH_CHECK_VALUE(addend->device() == a.device, "c is on another device");
     TORCH_CHECK_VALUE(!(addend->requires_grad() && at::GradMode::is_enabled()),
                       "block_scaled_mm gives c no gradient; detach it or use block_scaled_linear");
+    check_no_tangent(*addend, "c");
     TORCH_CHECK_VALUE(addend->dim() <= 2, "c must broadcast to [", m, ", ", n, "]");
   }
   at::AutoDispatchBelowADInplaceOrView below;
@@ -533,6 +541,8 @@ struct Linear : torch::autograd::Function<Linear> {
 Tensor linear(const Tensor& x, const Tensor& w, int64_t fmt, int64_t block, int64_t rounding) {
   check_real(x, "x");
   check_real(w, "w");
+  check_no_tangent(x, "x");
+  check_no_tangent(w, "w");
   TORCH_CHECK_VALUE(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1), "x [..., K] and w [N, K] do not fit: ", x.sizes(),
                     ", ", w.sizes());
   TORCH_CHECK_VALUE(w.numel() > 0, "w must not be empty");

@@ -13,6 +13,33 @@ import tcgen05_b200 as t5
 from tcgen05_b200 import blocks as bk
 from test_blocks import E2M1, make, product_bound
 
+# ------------------------------------------------------------ autograd
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    a, b = t5.quantize_blocks(make(1, 40, 64)), t5.quantize_blocks(make(2, 48, 64))
+    x, w = make(3, 40, 64), make(4, 48, 64)
+    with forward_ad.dual_level():
+        c = forward_ad.make_dual(make(5, 40, 48), make(6, 40, 48))
+        with pytest.raises(ValueError, match="tangent"):
+            t5.block_scaled_mm(a, b, c)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+            t5.block_scaled_mm(a, b, c[0])
+        with pytest.raises(ValueError, match="tangent"):
+            t5.block_scaled_mm(a, b, dtype=torch.float32, out=c)
+        values = forward_ad.make_dual(torch.zeros(40, 64, device="cuda"), x)
+        with pytest.raises(ValueError, match="tangent"):
+            t5.dequantize_blocks(a, out=values)
+        for p, q in ((forward_ad.make_dual(x, x), w), (x, forward_ad.make_dual(w, w))):
+            with pytest.raises(ValueError, match="tangent"):
+                t5.block_scaled_linear(p, q)
+        assert torch.equal(t5.block_scaled_mm(a, b, forward_ad.unpack_dual(c).primal),
+                           t5.block_scaled_mm(a, b, make(5, 40, 48)))
+
+
 # ------------------------------------------------------------ what is kept
 
 
