@@ -7,6 +7,7 @@
 
 #include "t5e.h"
 #include "t5e_blocks.cuh"
+#include "t5e_blocktiles.h"
 #include "t5e_dispatch.h"
 
 namespace t5e {
@@ -1018,29 +1019,32 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
     const Factor f = factor_of(P.r);
     const int side = warp >= 8;     // of the two warps of these lanes: every other chunk
     uint8_t* box = boxes + (quarter * 2 + side) * L::kBoxBytes;
-    uint32_t count = 0;
-    for (uint32_t tile = blockIdx.x / 2; ok && tile < tiles; tile += clusters, ++count) {
+    const auto wait = [&](uint32_t count) {
+      const bool there = barrier_wait(smem_u32(&acc_full[count & 1u]), (count >> 1) & 1u, &failed);
+      return (bool)__all_sync(0xFFFFFFFFu, there);
+    };
+    const auto take_tile = [&](uint32_t tile, uint32_t count, bool good) {
       const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
       const uint32_t p = pt * 256u + rank * 128u + quarter * 32u, q0 = qt * BN;
-      ok = barrier_wait(smem_u32(&acc_full[count & 1u]), (count >> 1) & 1u, &failed);
-      ok = __all_sync(0xFFFFFFFFu, ok);
       fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (count & 1u) * L::kSecond;
       const uint32_t free_bar = in_block(smem_u32(&acc_free[count & 1u]), 0);
       // 64 columns at a time.  The shared ones (the last of the first accumulator,
       // the first of the second) go first, and let the next tile start before
-      // anything is done with them
+      // anything is done with them.  Without good accumulators nothing is released:
+      // the other block may still have its own to take
       auto take = [&](int chunk, bool release) {
         float v[64];
-        load_acc32(acc + chunk * 64, v);
-        load_acc32(acc + chunk * 64 + 32, v + 32);
-        acc_loaded();
-        if (release) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_in(free_bar);
-        }
-        if (!ok) {
+        if (good) {
+          load_acc32(acc + chunk * 64, v);
+          load_acc32(acc + chunk * 64 + 32, v + 32);
+          acc_loaded();
+          if (release) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_in(free_bar);
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
@@ -1068,7 +1072,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
       } else {
         take(side, true);
       }
-    }
+    };
+    ok = take_tiles(blockIdx.x / 2, tiles, clusters, wait, take_tile);
     if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
