@@ -1019,32 +1019,29 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
     const Factor f = factor_of(P.r);
     const int side = warp >= 8;     // of the two warps of these lanes: every other chunk
     uint8_t* box = boxes + (quarter * 2 + side) * L::kBoxBytes;
-    const auto wait = [&](uint32_t count) {
-      const bool there = barrier_wait(smem_u32(&acc_full[count & 1u]), (count >> 1) & 1u, &failed);
-      return (bool)__all_sync(0xFFFFFFFFu, there);
-    };
-    const auto take_tile = [&](uint32_t tile, uint32_t count, bool good) {
+    uint32_t count = 0, tile = blockIdx.x / 2;
+    for (; ok && tile < tiles; tile += clusters, ++count) {
       const uint32_t pt = tile % P.p_tiles, qt = tile / P.p_tiles;
       const uint32_t p = pt * 256u + rank * 128u + quarter * 32u, q0 = qt * BN;
+      ok = barrier_wait(smem_u32(&acc_full[count & 1u]), (count >> 1) & 1u, &failed);
+      ok = __all_sync(0xFFFFFFFFu, ok);
       fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (count & 1u) * L::kSecond;
       const uint32_t free_bar = in_block(smem_u32(&acc_free[count & 1u]), 0);
       // 64 columns at a time.  The shared ones (the last of the first accumulator,
       // the first of the second) go first, and let the next tile start before
-      // anything is done with them.  Without good accumulators nothing is released:
-      // the other block may still have its own to take
+      // anything is done with them
       auto take = [&](int chunk, bool release) {
         float v[64];
-        if (good) {
-          load_acc32(acc + chunk * 64, v);
-          load_acc32(acc + chunk * 64 + 32, v + 32);
-          acc_loaded();
-          if (release) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_in(free_bar);
-          }
-        } else {
+        load_acc32(acc + chunk * 64, v);
+        load_acc32(acc + chunk * 64 + 32, v + 32);
+        acc_loaded();
+        if (release) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_in(free_bar);
+        }
+        if (!ok) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
@@ -1072,8 +1069,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
       } else {
         take(side, true);
       }
-    };
-    ok = take_tiles(blockIdx.x / 2, tiles, clusters, wait, take_tile);
+    }
+    // a wait ran out: the tiles behind that one become NaN as well.  No waits, and
+    // no accumulators released: the other block's may be good and not yet taken
+    spoil_tiles<BN>(tile, tiles, clusters, P.p_tiles, rank * 128u + quarter * 32u, side * 64u, lane, P.r.p_rows, P.r.q_rows,
+                    [&](uint32_t row, uint32_t col) {
+                      write_real(P.r.d, (int64_t)row * P.r.d_stride + col, P.r.d_type, __uint_as_float(0x7FC00000u));
+                    });
     if (P.boxed && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();

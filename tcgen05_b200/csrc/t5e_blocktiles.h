@@ -1,6 +1,5 @@
-// t5e_blocktiles.h -- the order in which a results warp of the pair kernel takes
-// its tiles, apart from what it does with them: plain C++, so that what happens
-// once a wait ran out can be run without a GPU.
+// t5e_blocktiles.h -- what a results warp of the pair kernel does with the tiles
+// behind one whose wait ran out: plain C++, so that it can be run without a GPU.
 #pragma once
 
 #include <cstdint>
@@ -14,19 +13,20 @@
 namespace t5e {
 namespace blockmm {
 
-// Tiles first, first + step, ... below `tiles`, the count-th of them by
-// take(tile, count, ok) after wait(count).  Once a wait returned false no other
-// is made, and every tile from there on is taken with ok = false: its results
-// are still written (as NaN), so that none keeps what memory held before.
-template <typename Wait, typename Take>
-T5E_ANYWHERE bool take_tiles(uint32_t first, uint32_t tiles, uint32_t step, Wait wait, Take take) {
-  bool ok = true;
-  uint32_t count = 0;
-  for (uint32_t tile = first; tile < tiles; tile += step, ++count) {
-    ok = ok && wait(count);
-    take(tile, count, ok);
+// write(row, col) for one lane's share of the tiles first, first + step, ... below
+// `tiles`: of the warp's 32 rows from row0 of a tile of 256 rows by BN columns,
+// the warp's 64 columns from col0 and, in a tile of 256, those 128 further on;
+// a lane takes every 32nd column.
+template <int BN, typename Write>
+T5E_ANYWHERE void spoil_tiles(uint32_t first, uint32_t tiles, uint32_t step, uint32_t p_tiles, uint32_t row0, uint32_t col0,
+                              uint32_t lane, uint32_t p_rows, uint32_t q_rows, Write write) {
+  for (uint32_t tile = first; tile < tiles; tile += step) {
+    const uint32_t p = tile % p_tiles * 256u + row0, q = tile / p_tiles * BN + col0 + lane;
+    for (uint32_t i = 0; i < BN / 64 * 32u; ++i) {
+      const uint32_t row = p + (i & 31u), col = q + (i >> 6) * 128u + (i >> 5 & 1u) * 32u;
+      if (row < p_rows && col < q_rows) write(row, col);
+    }
   }
-  return ok;
 }
 
 }  // namespace blockmm

@@ -32,36 +32,47 @@ def test_a_library_of_another_version_is_named(tmp_path, monkeypatch, source, wo
         nat.load()
 
 
-def test_every_tile_is_written_once_a_wait_ran_out(tmp_path):
-    """The pair kernel's results warps, with waits that run out at any of their tiles: each tile is taken once, from
-    the failing one on with `ok` false (its results become NaN), and no further wait is made."""
+def test_every_result_is_written_once_a_wait_ran_out(tmp_path):
+    """The pair kernel's results warps, each with a wait that runs out at another of its tiles: what it had taken by
+    then (the failing tile included) and what it spoils behind it are every result once."""
     src, exe = tmp_path / "tiles.cpp", tmp_path / "tiles"
     src.write_text("""
 #include "t5e_blocktiles.h"
 #include <cstdio>
-int main() {
-  int wrong = 0;
-  for (uint32_t tiles = 0; tiles < 12; ++tiles)
-    for (uint32_t step = 1; step < 5; ++step)
-      for (uint32_t first = 0; first < step; ++first)
-        for (int fail = -1; fail < 12; ++fail) {  // the count-th wait runs out
-          int waits = 0, taken[12] = {0}, good[12] = {0};
-          uint32_t counts = 0;
-          const bool ok = t5e::blockmm::take_tiles(
-              first, tiles, step, [&](uint32_t count) { ++waits; return (int)count != fail; },
-              [&](uint32_t tile, uint32_t count, bool ok) { ++taken[tile]; good[tile] = ok; wrong += count != counts++; });
-          const int mine = tiles > first ? (int)((tiles - first + step - 1) / step) : 0;
-          const bool fails = fail >= 0 && fail < mine;
-          wrong += ok == fails || waits != (fails ? fail + 1 : mine);
-          for (uint32_t t = 0; t < tiles; ++t) {
-            const bool my = t >= first && (t - first) % step == 0;
-            wrong += taken[t] != (my ? 1 : 0) || good[t] != (my && (!fails || (int)((t - first) / step) < fail));
+#include <vector>
+template <int BN>
+int wrong(uint32_t rows, uint32_t cols, uint32_t clusters, uint32_t seed) {
+  const uint32_t p_tiles = (rows + 255) / 256, tiles = p_tiles * ((cols + BN - 1) / BN);
+  std::vector<int> seen(rows * cols);
+  const auto write = [&](uint32_t row, uint32_t col) { ++seen[row * cols + col]; };
+  for (uint32_t cluster = 0; cluster < clusters; ++cluster)
+    for (uint32_t warp = 0; warp < 16; ++warp) {  // two blocks of four quarters by two sides
+      const uint32_t rank = warp / 8, quarter = warp % 4, side = warp / 4 % 2;
+      uint32_t taken = 1 + (seed + warp * 5 + cluster * 3) % 4, tile = cluster;
+      for (; taken > 0 && tile < tiles; tile += clusters, --taken)
+        for (uint32_t r = 0; r < 32; ++r)
+          for (uint32_t c = side * 64; c < BN; c += c % 64 == 63 ? 65 : 1) {
+            const uint32_t row = tile % p_tiles * 256 + rank * 128 + quarter * 32 + r, col = tile / p_tiles * BN + c;
+            if (row < rows && col < cols) write(row, col);
           }
-        }
-  std::printf("%d\\n", wrong);
-  return wrong != 0;
+      for (uint32_t lane = 0; lane < 32; ++lane)
+        t5e::blockmm::spoil_tiles<BN>(tile, tiles, clusters, p_tiles, rank * 128 + quarter * 32, side * 64, lane, rows, cols,
+                                      write);
+    }
+  int bad = 0;
+  for (int n : seen) bad += n != 1;
+  return bad;
+}
+int main() {
+  int bad = 0;
+  for (uint32_t seed = 0; seed < 4; ++seed)
+    for (uint32_t rows : {1u, 129u, 256u, 700u, 1100u})
+      for (uint32_t cols : {1u, 63u, 128u, 300u, 515u, 777u})
+        for (uint32_t clusters : {1u, 2u, 5u}) bad += wrong<128>(rows, cols, clusters, seed) + wrong<256>(rows, cols, clusters, seed);
+  std::printf("%d\\n", bad);
+  return bad != 0;
 }
 """)
     csrc = nat.LIB_PATH.parents[1] / "csrc"
-    subprocess.run(["g++", "-std=c++17", "-I", str(csrc), str(src), "-o", str(exe)], check=True)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(csrc), str(src), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.strip() == "0"
