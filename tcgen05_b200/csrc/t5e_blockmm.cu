@@ -301,14 +301,16 @@ struct Factor {
   float alpha, by, by2;  // by = 1: alpha alone
 };
 
-__device__ __forceinline__ Factor factor_of(const Params& P) {
-  const float ra = P.multiplier_a != nullptr ? 1.f / *P.multiplier_a : 1.f;
-  const float rb = P.multiplier_b != nullptr ? 1.f / *P.multiplier_b : 1.f;
-  const float first = P.alpha * ra, joint = first * rb;
-  const auto normal = [](float v) { return ((__float_as_uint(v) >> 23) & 0xFFu) - 1u < 254u; };
+__host__ __device__ __forceinline__ bool is_normal(float v) {
+  const float size = v < 0.f ? -v : v;
+  return size >= 0x1p-126f && size <= 0x1.fffffep127f;
+}
+
+__device__ __forceinline__ Factor factor_of(float alpha, float ma, float mb) {
+  const float ra = 1.f / ma, rb = 1.f / mb, first = alpha * ra, joint = first * rb;
   Factor f = {joint, 1.f, 1.f};
-  if (normal(first) && normal(joint)) return f;
-  const double whole = (double)P.alpha * ra * rb;  // three F32 numbers: within F64's range
+  if (is_normal(first) && is_normal(joint)) return f;
+  const double whole = (double)alpha * ra * rb;  // three F32 numbers: within F64's range
   const int e = (int)((__double_as_longlong(whole) >> 52) & 0x7FF) - 1023;
   if (whole == 0. || e == 1024) {
     f.alpha = (float)whole;
@@ -321,6 +323,8 @@ __device__ __forceinline__ Factor factor_of(const Params& P) {
   f.by2 = __uint_as_float((uint32_t)(rest + 127) << 23);
   return f;
 }
+
+__device__ __forceinline__ float multiplier_at(const float* p) { return p != nullptr ? *p : 1.f; }
 
 template <int N>
 __device__ __forceinline__ void rescale(const Factor& f, float* v) {
@@ -720,6 +724,11 @@ __device__ __forceinline__ bool drain_ring(uint64_t* empty, const Use& u, uint32
 // memory and each block finishes BN / split columns, adding the parts in rank
 // order.
 //
+// FACTORS: whether there are multipliers, or an alpha that is not a normal number;
+// without them the code of factor_of stays out (48 x 14336 x 4096: 12.84 us, with
+// it 13.20).  Multipliers are on their way while the pipeline runs (the same
+// with two of them: 13.70, read behind it 14.05).
+//
 // Depth of the rings: half of the shared memory where two blocks share an SM,
 // all of it where there are no more blocks than SMs; a row of tiles that streams
 // a weight matrix past a few rows is bound by the bytes in flight.
@@ -772,7 +781,7 @@ __device__ __forceinline__ void join_parts(const Params& P, const Factor& f, uin
   store_results<SWAP, N>(P, f, p, q, N, v);
 }
 
-template <int BN, int BLOCK, bool SWAP>
+template <int BN, int BLOCK, bool SWAP, bool FACTORS>
 __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileParams T, uint32_t split) {
   using S = typename TileShape<BN, BLOCK>::Pipe;
   const Params& P = T.r;
@@ -817,6 +826,8 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   fence_after();
   blocks::let_next_grid_start();
   blocks::wait_for_previous_grid();
+  // under way while the pipeline runs
+  const float ma = FACTORS ? multiplier_at(P.multiplier_a) : 1.f, mb = FACTORS ? multiplier_at(P.multiplier_b) : 1.f;
   const uint32_t tmem = tmem_slot;
   bool ok = true;
   if (elected()) {
@@ -841,7 +852,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   const bool bad = __syncthreads_or(!ok);
   if (bad && t == 0) atomicExch(&g_expired, 1);
   const float nan = __uint_as_float(0x7FC00000u);
-  const Factor f = factor_of(P);
+  const Factor f = FACTORS ? factor_of(P.alpha, ma, mb) : Factor{P.alpha, 1.f, 1.f};
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   if (split == 1u && !SWAP && BN >= 32) {
     // the stages are free: 32 x 33 floats of them for each warp
@@ -1016,7 +1027,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1) pai
     }
   } else {
     const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
-    const Factor f = factor_of(P.r);
+    const Factor f = factor_of(P.r.alpha, multiplier_at(P.r.multiplier_a), multiplier_at(P.r.multiplier_b));
     const int side = warp >= 8;     // of the two warps of these lanes: every other chunk
     uint8_t* box = boxes + (quarter * 2 + side) * L::kBoxBytes;
     uint32_t count = 0, tile = blockIdx.x / 2;
@@ -1215,8 +1226,8 @@ uint64_t blocks_at_once(uint32_t split) {
   attr[0].val.clusterDim = {split, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (raise_smem_limit<tile_kernel<128, 16, false>>(S::kDeepSmem, "block product attribute") != T5E_OK ||
-      cudaOccupancyMaxActiveClusters(&n, tile_kernel<128, 16, false>, &cfg) != cudaSuccess || n < 1) {
+  if (raise_smem_limit<tile_kernel<128, 16, false, true>>(S::kDeepSmem, "block product attribute") != T5E_OK ||
+      cudaOccupancyMaxActiveClusters(&n, tile_kernel<128, 16, false, true>, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();  // an estimate only: the launch reports what is wrong
     return (uint64_t)sm_count();
   }
@@ -1231,7 +1242,12 @@ int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, 
   TileParams P;
   P.r = params;
   int rc = encode_maps<typename S::Pipe>(&P.maps, p, q);
-  if (rc == T5E_OK) rc = raise_smem_limit<tile_kernel<BN, BLOCK, SWAP>>(S::kDeepSmem, "block product attribute");
+  // no multipliers and an ordinary alpha need none of factor_of's code
+  const bool plain = params.multiplier_a == nullptr && params.multiplier_b == nullptr && is_normal(params.alpha);
+  const auto kernel = plain ? tile_kernel<BN, BLOCK, SWAP, false> : tile_kernel<BN, BLOCK, SWAP, true>;
+  if (rc == T5E_OK)
+    rc = plain ? raise_smem_limit<tile_kernel<BN, BLOCK, SWAP, false>>(S::kDeepSmem, "block product attribute")
+               : raise_smem_limit<tile_kernel<BN, BLOCK, SWAP, true>>(S::kDeepSmem, "block product attribute");
   if (rc != T5E_OK) return rc;
   P.r.idesc = instruction(p, BN);
   cudaLaunchConfig_t cfg = {};
@@ -1250,7 +1266,7 @@ int launch_tile(const Params& params, const t5e_blocks& p, const t5e_blocks& q, 
   attr[1].val.clusterDim = {split, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return blocks_launched(cudaLaunchKernelEx(&cfg, tile_kernel<BN, BLOCK, SWAP>, P, split));
+  return blocks_launched(cudaLaunchKernelEx(&cfg, kernel, P, split));
 }
 
 template <int BLOCK>
