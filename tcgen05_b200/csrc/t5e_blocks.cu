@@ -125,13 +125,13 @@ __global__ void __launch_bounds__(kThreads) partials_kernel(const __grid_constan
       for (; i + 3 * step < vecs; i += 4 * step) {
         uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __ldg(p + i + j * step);
+        for (int j = 0; j < 4; ++j) v[j] = load16(p + i + j * step);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           best = join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(best, v[j].x), v[j].y), v[j].z), v[j].w);
       }
       for (; i < vecs; i += step) {
-        const uint4 v = __ldg(p + i);
+        const uint4 v = load16(p + i);
         best = join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(join_max<TYPE>(best, v.x), v.y), v.z), v.w);
       }
       done = vecs * kPer;
@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(kThreads) partials_kernel(const __grid_constan
   if (threadIdx.x == 0) J.partials[block] = m;
 }
 
-__global__ void __launch_bounds__(kThreads) multiplier_kernel(const uint32_t* __restrict__ partials, int count,
-                                                              float* __restrict__ multiplier) {
+__global__ void __launch_bounds__(kThreads) multiplier_kernel(const uint32_t* partials, int count,
+                                                              float* multiplier) {
   __shared__ uint32_t shared[kThreads / 32];
   let_next_grid_start();
   wait_for_previous_grid();
@@ -262,7 +262,7 @@ __device__ __forceinline__ void load_chunk(const Job& J, uint64_t row0, const Wa
       if (within<TYPE>(J, first, kVecs * 16)) {
         c.shift = shift;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) c.w[j] = __ldg(first + j);
+        for (int j = 0; j < kVecs; ++j) c.w[j] = load16(first + j);
         return;
       }
     }
@@ -596,9 +596,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == T5E_REAL_BF16 ? 4 : TYPE == 
       for (int j = 0; j < kBatch; ++j, row += (int64_t)kRows * J.stride * Real<TYPE>::kBytes) {
         shift[j] = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
         const uint4* p = reinterpret_cast<const uint4*>(row - shift[j]) + v;
-        a[j] = __ldg(p);
+        a[j] = load16(p);
         b[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (v == kVecs - 1) b[j] = __ldg(p + 1);
+        if (v == kVecs - 1) b[j] = load16(p + 1);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j, to += kRows * B::kPitch) {
@@ -638,9 +638,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == T5E_REAL_BF16 ? 4 : TYPE == 
 // neighbours.  FOLD: 1 / m is a power of two near 1, so its product with the
 // scale is exact and one product per element is enough.
 template <int TYPE, bool E8M0, int BLOCK, bool VEC, bool FOLD>
-__device__ __forceinline__ void open_rows(const uint8_t* __restrict__ data, int64_t data_stride,
-                                          const uint8_t* __restrict__ scales, uint32_t groups, uint32_t rows, uint64_t row0,
-                                          uint32_t k, const Divider& chunks, float back, void* __restrict__ out,
+__device__ __forceinline__ void open_rows(const uint8_t* data, int64_t data_stride,
+                                          const uint8_t* scales, uint32_t groups, uint32_t rows, uint64_t row0,
+                                          uint32_t k, const Divider& chunks, float back, void* out,
                                           int64_t out_stride, bool wide, float* turn) {
   constexpr int kAtOnce = 2, kBlocks = kChunk / BLOCK;
   const uint32_t total = rows * chunks.d, step = gridDim.x * kThreads;
@@ -662,12 +662,12 @@ __device__ __forceinline__ void open_rows(const uint8_t* __restrict__ data, int6
       w[i] = make_uint4(0u, 0u, 0u, 0u);
       bytes[i] = 0u;
       if (in) {
-        w[i] = __ldg(reinterpret_cast<const uint4*>(data + (int64_t)(row0 + row[i]) * data_stride + e0[i] / 2u));
+        w[i] = load16(data + (int64_t)(row0 + row[i]) * data_stride + e0[i] / 2u);
         const uint32_t b = e0[i] / BLOCK;
         const uint8_t* at = scales + ((row[i] >> 7) * groups + (b >> 2)) * 512u + (row[i] & 31u) * 16u +
                             ((row[i] >> 5) & 3u) * 4u + (b & 3u);
-        if constexpr (BLOCK == 16) bytes[i] = __ldg(reinterpret_cast<const uint16_t*>(at));
-        else bytes[i] = __ldg(at);
+        if constexpr (BLOCK == 16) bytes[i] = *reinterpret_cast<const uint16_t*>(at);
+        else bytes[i] = *at;
       }
       walk.advance(rows_on, chunks_on, chunks.d);
     }
@@ -738,10 +738,10 @@ __device__ __forceinline__ void open_rows(const uint8_t* __restrict__ data, int6
 }
 
 template <int TYPE, bool E8M0, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_stride,
-                                                              const uint8_t* __restrict__ scales, uint32_t groups,
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* data, int64_t data_stride,
+                                                              const uint8_t* scales, uint32_t groups,
                                                               uint32_t rows, uint64_t row0, uint32_t k, Divider chunks,
-                                                              const float* multiplier, void* __restrict__ out,
+                                                              const float* multiplier, void* out,
                                                               int64_t out_stride, bool wide) {
   __shared__ __align__(16) float turn[VEC ? 4 : kThreads * 36];
   let_next_grid_start();

@@ -67,15 +67,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// Loads of memory that the kernel before on the stream wrote.  Ordinary loads
+// that stay behind the wait for that kernel: with programmatic launches it may
+// still be writing while this one has begun, so the memory is not read-only for
+// this kernel's whole time as non-coherent loads (__ldg, ld.global.nc) ask, and a
+// compiler may move those ahead of the wait.  They take the same time (8192 x
+// 8192 BF16 to UE4M3 blocks 31 to 32 us either way, back 29.3 and 29.4).
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // 32 bytes of a lane in one access (32-byte aligned) or two (16-byte aligned): a
 // warp whose lanes take neighbouring 32 bytes then touches whole lines.
 __device__ __forceinline__ void load32(const void* p, bool wide, uint4& a, uint4& b) {
   if (wide) {
-    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
   } else {
-    a = __ldg(static_cast<const uint4*>(p));
-    b = __ldg(static_cast<const uint4*>(p) + 1);
+    a = load16(p);
+    b = load16(static_cast<const uint4*>(p) + 1);
   }
 }
 __device__ __forceinline__ void store32(void* p, bool wide, const uint4& a, const uint4& b) {

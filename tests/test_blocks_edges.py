@@ -191,6 +191,33 @@ def test_values_whose_scale_alone_leaves_f32(vec):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(40, 131), (300, 267), (700, 1027)])
+def test_chains_without_a_pause(m, n):
+    """Each call reads what the one before has just written, in rows that share lines of memory; the same as with the
+    device idle between them."""
+    a, b = t5.quantize_blocks(make(1, m, 96)), t5.quantize_blocks(make(2, n, 96))
+    x = make(3, m, n)
+
+    def chain(pause):
+        c, back, out = x.clone(), torch.empty(m, n, device="cuda"), []
+        for i in range(40):
+            for call in (lambda: t5.block_scaled_mm(a, b, c, alpha=0.25, dtype=torch.float32, out=c),
+                         lambda: out.append(t5.quantize_blocks(c, axis="both", multiplier="auto")),
+                         lambda: t5.dequantize_blocks(out[-1][0], out=back),
+                         lambda: out.append(t5.quantize_blocks(back, scaling="ue8m0")),
+                         lambda: t5.dequantize_blocks(out[-1], out=c)):
+                call()
+                if pause:
+                    torch.cuda.synchronize()
+        return c, back, out[-2][0].data, out[-2][1].data, out[-1].data
+
+    want = chain(True)
+    for _ in range(3):
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(chain(False), want))
+
+
+@pytest.mark.gpu
 def test_out_may_not_hold_a_multiplier():
     x = make(1, 40, 64)
     q = t5.quantize_blocks(x)

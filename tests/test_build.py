@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import re
 import subprocess
 
 import pytest
@@ -76,3 +77,15 @@ int main() {
     csrc = nat.LIB_PATH.parents[1] / "csrc"
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(csrc), str(src), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.strip() == "0"
+
+
+def test_block_kernels_read_through_ordinary_loads():
+    """With programmatic launches a kernel begins while the one before still writes what it will read: no load may be
+    of the kind that asks for memory that is read-only all the while, or that a compiler may move ahead of the wait."""
+    csrc = nat.LIB_PATH.parents[1] / "csrc"
+    for name in ("t5e_blocks.cuh", "t5e_blocks.cu", "t5e_blockmm.cu"):
+        code = "\n".join(line.split("//")[0] for line in (csrc / name).read_text().splitlines())
+        assert "griddepcontrol.wait" in code or "wait_for_previous_grid" in code
+        for word in ("__ldg(", ".nc", "__restrict__", "__ldcg(", "__ldlu("):
+            assert word not in code, (name, word)
+        assert not re.findall(r"asm\s*\(\s*\"[^;]*\bld\.", code), name
