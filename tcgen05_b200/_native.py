@@ -282,8 +282,11 @@ def torch_ops():
         import torch  # noqa: F401  (its libraries have to be in the process first)
 
         spec = importlib.util.spec_from_file_location("t5e_torch", TORCH_LIB_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise NativeLibraryError(f"{TORCH_LIB_PATH} does not load with this PyTorch ({e}); rebuild it") from e
         if module.abi_version != ABI_VERSION:
             raise NativeLibraryError(f"{TORCH_LIB_PATH} has ABI version {module.abi_version}, expected {ABI_VERSION}; "
                                      "rebuild it")

@@ -40,21 +40,34 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def build_torch(verbose: bool = False, force: bool = False) -> Path:
-    """Compile the PyTorch side if its sources are newer; return its path."""
+def build_torch(verbose: bool = False, force: bool = False) -> Path | None:
+    """Compile the PyTorch side if its sources are newer or it was built for
+    another PyTorch or Python; return its path.  Without PyTorch or a C++
+    compiler it is left out, with a message: the C ABI needs neither."""
     import sysconfig
 
-    import torch
-
+    try:
+        import torch
+    except ImportError as e:
+        print(f"{TORCH_LIB.name} is left out: {e}", file=sys.stderr, flush=True)
+        return None
+    cxx = os.environ.get("CXX", "g++")
+    if shutil.which(cxx) is None:
+        print(f"{TORCH_LIB.name} is left out: no C++ compiler {cxx}", file=sys.stderr, flush=True)
+        return None
+    built_for = f"torch {torch.__version__} python {sys.version_info[0]}.{sys.version_info[1]}"
     deps = [TORCH_SRC, INCLUDE / "t5e.h"]
-    if not force and TORCH_LIB.exists() and all(TORCH_LIB.stat().st_mtime >= p.stat().st_mtime for p in deps):
+    # the library holds the words it was built with
+    if not force and TORCH_LIB.exists() and all(TORCH_LIB.stat().st_mtime >= p.stat().st_mtime for p in deps) \
+            and f"t5e_torch for {built_for}\0".encode() in TORCH_LIB.read_bytes():
         return TORCH_LIB
     cuda = Path(nvcc()).resolve().parents[1] / "include"
     home = Path(torch.__file__).resolve().parent
     includes = [INCLUDE, sysconfig.get_paths()["include"], cuda, home / "include", home / "include/torch/csrc/api/include"]
     tmp = TORCH_LIB.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=t5e_torch",
+           f'-DT5E_BUILT_FOR="t5e_torch for {built_for}"',
            *[arg for i in includes for arg in ("-isystem", str(i))], str(TORCH_SRC), "-o", str(tmp),
            "-L", str(LIB_DIR), "-l:libt5e.so", "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
            "-ltorch_python",

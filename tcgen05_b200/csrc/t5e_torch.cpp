@@ -573,4 +573,5 @@ PYBIND11_MODULE(t5e_torch, m) {
   m.def("mm", &mm);
   m.def("linear", &linear);
   m.attr("abi_version") = (int)T5E_ABI_VERSION;
+  m.attr("built_for") = T5E_BUILT_FOR;  // what the build command looks for in the file
 }

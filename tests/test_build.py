@@ -4,10 +4,12 @@ from __future__ import annotations
 
 import re
 import subprocess
+import sys
 
 import pytest
 
 from tcgen05_b200 import _native as nat
+from tcgen05_b200 import build
 
 
 def test_extension_shares_the_cxx_library_of_pytorch():
@@ -89,3 +91,37 @@ def test_block_kernels_read_through_ordinary_loads():
         for word in ("__ldg(", ".nc", "__restrict__", "__ldcg(", "__ldlu("):
             assert word not in code, (name, word)
         assert not re.findall(r"asm\s*\(\s*\"[^;]*\bld\.", code), name
+
+
+def test_the_c_library_builds_without_pytorch_or_a_cxx_compiler(monkeypatch, capfd):
+    monkeypatch.setattr(build, "_build_cuda", lambda *a: build.LIB)
+    monkeypatch.setattr(build.subprocess, "run", lambda *a, **k: pytest.fail("a compiler was called"))
+    monkeypatch.setenv("CXX", "/nowhere/g++")
+    assert build.build(force=True) == build.LIB
+    assert "left out: no C++ compiler /nowhere/g++" in capfd.readouterr().err
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build(force=True) == build.LIB
+    assert "t5e_torch.so is left out" in capfd.readouterr().err
+
+
+def test_the_extension_is_rebuilt_for_another_pytorch(monkeypatch):
+    import torch
+
+    calls = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **k: calls.append(cmd))
+    monkeypatch.setattr(build.os, "replace", lambda a, b: None)
+    monkeypatch.setattr(build, "TORCH_SRC", build.INCLUDE / "t5e.h")  # newer sources are not what this is about
+    words = f"t5e_torch for torch {torch.__version__} python".encode()
+    assert words in build.TORCH_LIB.read_bytes()
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build_torch()
+    assert len(calls) == 1 and any("t5e_torch for torch 0.0.1 python" in str(arg) for arg in calls[0])
+
+
+def test_an_extension_that_does_not_load_is_named(tmp_path, monkeypatch):
+    bad = tmp_path / "t5e_torch.so"
+    bad.write_bytes(b"not a library")
+    monkeypatch.setattr(nat, "TORCH_LIB_PATH", bad)
+    monkeypatch.setattr(nat, "_torch_ops", None)
+    with pytest.raises(nat.NativeLibraryError, match="rebuild it"):
+        nat.torch_ops()
