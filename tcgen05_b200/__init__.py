@@ -15,6 +15,8 @@ on the tensor cores) and ``block_scaled_linear`` (a linear layer with its
 gradients).
 """
 
+import importlib.util as _util
+
 from .formats import bits_to_f32, f32_to_bits
 from .model import (
     DotProduct,
@@ -50,7 +52,6 @@ def __getattr__(name: str):
 
 
 __all__ = [
-    "BlockScaledRows",
     "DotProduct",
     "PackedRows",
     "PendingBatch",
@@ -60,11 +61,6 @@ __all__ = [
     "Tcgen05MixedRawWindowMmaModel",
     "Tcgen05RawWindowNvfp4MmaModel",
     "bits_to_f32",
-    "block_multiplier",
-    "block_scaled_linear",
-    "block_scaled_mm",
-    "block_scaled_mm_expired",
-    "dequantize_blocks",
     "f32_to_bits",
     "make_model",
     "mma",
@@ -72,6 +68,9 @@ __all__ = [
     "mma_dot",
     "mma_dot_batch",
     "normalize_format",
-    "quantize_blocks",
     "sparse_active_indices",
 ]
+
+# `from tcgen05_b200 import *` works without PyTorch, as it did before these
+if _util.find_spec("torch") is not None:
+    __all__ += sorted(_BLOCK_SCALED)

@@ -125,3 +125,14 @@ def test_an_extension_that_does_not_load_is_named(tmp_path, monkeypatch):
     monkeypatch.setattr(nat, "_torch_ops", None)
     with pytest.raises(nat.NativeLibraryError, match="rebuild it"):
         nat.torch_ops()
+
+
+def test_star_import_without_pytorch():
+    """What needs no PyTorch is imported without it; where it is there, the block-scaled calls come along."""
+    code = "import sys\n{}\nfrom tcgen05_b200 import *\nprint(make_model('tf32') is not None, 'quantize_blocks' in globals())\n"
+    hide = ("import importlib.util as u\nfind = u.find_spec\nu.find_spec = lambda n, *a: None if n == 'torch' else find(n, *a)\n"
+            "sys.modules['torch'] = None")
+    for first, words in ((hide, "True False"), ("", "True True")):
+        r = subprocess.run([sys.executable, "-c", code.format(first)], capture_output=True, text=True,
+                           cwd=nat.LIB_PATH.parents[2])
+        assert r.stdout.strip() == words, r.stderr[-800:]
