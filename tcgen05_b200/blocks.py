@@ -131,15 +131,22 @@ class BlockScaledRows:
     @classmethod
     def from_words(cls, words, scales, *, scaling: str = "ue4m3", scale_vec: int | None = None, multiplier=None):
         """From a [rows, K] CUDA tensor of raw E2M1 container words and
-        [rows, blocks] scale bytes, as ``mma_dot_batch`` takes them."""
+        [rows, blocks] scale bytes, as ``mma_dot_batch`` takes them (K up to
+        its 65536)."""
         scaling, scale_vec = _form(scaling, scale_vec)
-        if words.dim() != 2:
-            raise ValueError("words must be a [rows, K] tensor of words")
+        _tensor(words, "words"), _tensor(scales, "scales")
+        if words.dim() != 2 or words.dtype.is_floating_point or words.dtype.is_complex:
+            raise ValueError("words must be a [rows, K] tensor of integers")
         rows, k = words.shape
+        if not 1 <= k <= nat.MAX_K:
+            raise ValueError(f"K must be between 1 and {nat.MAX_K}, not {k}")
         blocks = -(-k // _FORMS[scaling, scale_vec][1])
         if tuple(scales.shape) != (rows, blocks):
             raise ValueError(f"scales must be [{rows}, {blocks}] bytes")
-        data = packing.pack_rows_device(words, nat.FMT_E2M1, cls.row_stride(k))
+        if not words.is_cuda or scales.device != words.device:
+            raise ValueError("words and scales must be on one CUDA device (there is no CPU fallback)")
+        with torch.cuda.device(words.device):
+            data = packing.pack_rows_device(words, nat.FMT_E2M1, cls.row_stride(k))
         return cls(data, tile_scales(scales), k, scaling=scaling, scale_vec=scale_vec, multiplier=multiplier)
 
     @staticmethod

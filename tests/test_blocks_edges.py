@@ -266,3 +266,18 @@ def test_rounded_rows_whose_memory_was_freed_are_refused():
     for call in (lambda: t5.dequantize_blocks(q), lambda: t5.block_scaled_mm(q, q), lambda: q.scales, lambda: q.data):
         with pytest.raises(ValueError, match="moved"):
             call()
+
+
+# ------------------------------------------------------------ refusals, each by its own words (CPU)
+
+
+def test_each_bad_word_tensor_is_named():
+    words, scales = torch.zeros(4, 70, dtype=torch.int32), torch.zeros(4, 5, dtype=torch.uint8)
+    make_rows = t5.BlockScaledRows.from_words
+    for w, s, message in ((words, scales, "on one CUDA device"), (words.float(), scales, "tensor of integers"),
+                          (words[0], scales, "tensor of integers"), (words, scales[:, :4], r"scales must be \[4, 5\]"),
+                          (words[:, :0], scales[:, :0], "K must be between"), ([[1]], scales, "words must be a torch tensor"),
+                          (words, [[1]], "scales must be a torch tensor"),
+                          (words[:1].expand(1, 70).repeat(1, 1000), scales, "K must be between 1 and 65536, not 70000")):
+        with pytest.raises(ValueError, match=message):
+            make_rows(w, s)
