@@ -11,9 +11,73 @@ import torch
 
 import tcgen05_b200 as t5
 from tcgen05_b200 import blocks as bk
-from test_blocks import E2M1, make, product_bound
+from test_blocks import BLOCK, E2M1, FORMS, TYPES, check_rows, define, make, product_bound
 
 # ------------------------------------------------------------ autograd
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "w", "both"])
+def test_second_derivative_is_refused_whatever_the_incoming_gradient(which):
+    """dx depends on w and dw on x even where the incoming gradient is a constant: a loss of them has to refuse its
+    backward pass, not to leave the terms out."""
+    x, w = make(1, 20, 64), make(2, 30, 64)
+    want = torch.autograd.grad(t5.block_scaled_linear(*(p := [t.clone().requires_grad_() for t in (x, w)])).sum(), p)
+    x.requires_grad_(which != "w")
+    w.requires_grad_(which != "x")
+    leaves = [t for t in (x, w) if t.requires_grad]
+    for weight in (None, torch.ones(20, 30, device="cuda")):
+        y = t5.block_scaled_linear(x, w)
+        out = y.sum() if weight is None else y
+        got = torch.autograd.grad(out, leaves, weight, create_graph=True)
+        for t, g in zip(leaves, got):
+            assert g.requires_grad and torch.equal(g, want[0] if t is x else want[1])
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                (y.square().sum() + g.square().sum()).backward(retain_graph=True)
+        # what does not use them is differentiated as ever
+        first = torch.autograd.grad(y.square().sum(), leaves)
+        assert all(bool(t.isfinite().all()) and not t.requires_grad for t in first)
+
+
+@pytest.mark.gpu
+def test_out_is_seen_as_written():
+    """A tensor that autograd saved may not be overwritten behind its back."""
+    a, b = t5.quantize_blocks(make(1, 40, 64)), t5.quantize_blocks(make(2, 64, 64))
+
+    def product(out):
+        t5.block_scaled_mm(a, b, dtype=torch.float32, out=out)
+
+    def values(out):
+        t5.dequantize_blocks(a, out=out)
+
+    for write in (product, values):
+        buffer = make(3, 40, 64)
+        w = torch.ones(40, 64, device="cuda", requires_grad=True)
+        z = w * buffer
+        version = buffer._version
+        write(buffer)
+        assert buffer._version == version + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        # a part of a larger tensor counts for the whole
+        big = make(4, 50, 80)
+        z = w * big[5:45, 8:72]
+        write(big[5:45, 8:72])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        # a refused call writes nothing and counts nothing
+        version = big._version
+        with pytest.raises(ValueError):
+            write(big[5:45, 8:71])
+        assert big._version == version
+        with torch.inference_mode():
+            held = torch.zeros(40, 64, device="cuda")
+            write(held)
+            assert bool(held.any())
+            held.zero_()
+        with pytest.raises(RuntimeError, match="[Ii]nference tensor"):
+            write(held)
+        assert not bool(held.any())
 
 
 @pytest.mark.gpu
@@ -268,7 +332,105 @@ def test_rounded_rows_whose_memory_was_freed_are_refused():
             call()
 
 
+# ------------------------------------------------------------ roundings, value by value
+
+
+def steps_of(form):
+    return [m / 8 * 2.0 ** e for m in range(8, 16) for e in (-6, 0, 5)] if form[0] == "ue4m3" else \
+        [2.0 ** e for e in (-6, 0, 5)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_ties_and_the_types_own_neighbours(form, dtype):
+    """Elements at every border of E2M1 times a scale and the type's next values on either side, which are other
+    values than the border."""
+    blocks = []
+    for step in steps_of(form):
+        ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64) * step
+        tie = ties.to(dtype)
+        assert torch.equal(tie.double(), ties)
+        for side in (None, math.inf, 0.0):
+            t = tie if side is None else torch.nextafter(tie, torch.full_like(tie, side))
+            assert side is None or not bool((t == tie).any())
+            for sign in (1, -1):
+                blocks.append(torch.cat([torch.tensor([6 * step]).to(dtype), sign * t,
+                                         torch.zeros(BLOCK[form] - 8, dtype=dtype)]))
+    x = torch.stack(blocks).cuda()
+    for m in (1.0, 0.25, 2.0 ** 60, 2.0 ** -60, 2.0 ** 70, 1.5):
+        codes, scale, _ = define(x, form, m)
+        kw = dict(scaling=form[0], scale_vec=form[1], multiplier=None if m == 1 else m)
+        check_rows(t5.quantize_blocks(x, **kw), codes, scale)
+        check_rows(t5.quantize_blocks(x.t().contiguous(), axis=0, **kw), codes, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=lambda t: str(t)[6:])
+def test_every_16_bit_element_against_every_significand_of_a_scale(form, dtype):
+    block = BLOCK[form]
+    every = torch.arange(1, 0x7F80 if dtype == torch.bfloat16 else 0x7C00, dtype=torch.int16).view(dtype)
+    rows = []
+    for step in steps_of(form)[1::3]:  # every significand, the middle exponent
+        v = every[(every.double() >= 0.05 * step) & (every.double() <= 6 * step)]
+        v = torch.nn.functional.pad(v, (0, -v.numel() % (block - 1))).view(-1, block - 1)
+        rows.append(torch.cat([torch.full((v.shape[0], 1), 6 * step, dtype=dtype), v], 1))
+    x = torch.cat(rows).cuda()
+    for m in (1.0, 2.0 ** 7, 2.0 ** 60, 2.0 ** -60):
+        # the elements' quotients are those of m = 1 with a scale that is m times larger
+        kw = dict(scaling=form[0], scale_vec=form[1], multiplier=None if m == 1 else m)
+        codes, scale, _ = define(x, form, m)
+        check_rows(t5.quantize_blocks(x, **kw), codes, scale)
+    codes, scale, _ = define(-x, form)
+    check_rows(t5.quantize_blocks(-x.t(), axis=0, scaling=form[0], scale_vec=form[1]), codes, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}")
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=lambda t: str(t)[6:])
+def test_every_16_bit_value_as_a_blocks_largest(form, dtype):
+    every = torch.arange(0, 0x8000, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.zeros(every.numel(), BLOCK[form], dtype=dtype)
+    x[:, 3] = every
+    x[:, 5] = -(every.double() / 3).to(dtype)
+    x = x.cuda()
+    for ceil in ((False, True) if form[0] == "ue8m0" else (False,)):
+        for m in (1.0, 2.0 ** 11, 2.0 ** -20):
+            codes, scale, _ = define(x, form, m, ceil)
+            kw = dict(scaling=form[0], scale_vec=form[1], multiplier=None if m == 1 else m)
+            if form[0] == "ue8m0":
+                kw["scale_rounding"] = "ceil" if ceil else "floor"
+            check_rows(t5.quantize_blocks(x, **kw), codes, scale)
+
+
 # ------------------------------------------------------------ refusals, each by its own words (CPU)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(scaling="ue4m3", scale_vec=2), "takes scaling"), (dict(scaling="ue5m3"), "takes scaling"),
+    (dict(scaling="ue8m0", scale_vec=1), "takes scaling"), (dict(scaling="ue4m3", scale_rounding="floor"), "scale_rounding is"),
+    (dict(scaling="ue8m0", scale_rounding="nearest"), "scale_rounding is"),
+    (dict(scaling="ue8m0", scale_rounding="up"), "scale_rounding is"), (dict(axis=1), "axis is"),
+    (dict(axis="rows"), "axis is"), (dict(multiplier="max"), "multiplier is a number"),
+    *[(dict(multiplier=m), "multiplier must be positive") for m in (0.0, -2.0, math.nan, math.inf, 1e300, 1e-300, 1e-45)],
+    (dict(), "must be a dense tensor on a CUDA device"),
+])
+def test_each_bad_argument_is_named(kw, words):
+    with pytest.raises(ValueError, match=words):
+        t5.quantize_blocks(torch.zeros(4, 64), **kw)
+
+
+def test_each_bad_tensor_is_named():
+    calls = (t5.quantize_blocks, t5.block_multiplier, lambda v: t5.block_scaled_linear(v, v))
+    for call in calls:
+        for dtype in (torch.float64, torch.int32, torch.float8_e4m3fn):
+            with pytest.raises(ValueError, match="must be float32, bfloat16 or float16"):
+                call(torch.zeros(4, 64, dtype=dtype))
+        with pytest.raises(ValueError, match="on a CUDA device"):
+            call(torch.zeros(4, 64))
+        with pytest.raises(ValueError, match="must be a torch tensor"):
+            call([[1.0]])
 
 
 def test_each_bad_word_tensor_is_named():
