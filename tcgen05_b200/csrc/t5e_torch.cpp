@@ -468,7 +468,7 @@ struct Linear : torch::autograd::Function<Linear> {
     Tensor y = at::empty({tokens, n}, x.options());
     launch_product(xb, wb, m, automatic ? m + 1 : nullptr, 1.f, 0, nullptr, y, device);
     ctx->save_for_backward({keep});
-    saved["parts"] = std::vector<int64_t>{xt, wt};
+    saved["parts"] = std::vector<int64_t>{xt, wt, kept.size};
     return x.dim() == 2 ? y : y.view(shape);
   }
 
@@ -506,6 +506,11 @@ struct Linear : torch::autograd::Function<Linear> {
     const std::vector<int64_t> parts = saved["parts"].toIntVector();
     const Tensor keep = ctx->get_saved_variables()[0];
     const c10::Device device = g.device();
+    // hooks on saved tensors may have put another one in its place
+    TORCH_CHECK_VALUE(keep.device() == device && keep.scalar_type() == at::kByte && keep.dim() == 1 &&
+                          keep.size(0) == parts[2] && keep.is_contiguous() &&
+                          reinterpret_cast<uintptr_t>(keep.const_data_ptr()) % 16 == 0,
+                      "what block_scaled_linear saved came back on another device or in another form");
     const c10::cuda::CUDAGuard guard(device);
     Space space;
     const int64_t gr = need_x ? space.take(blocks_size(tokens, n, block)) : -1;

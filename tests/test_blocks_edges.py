@@ -104,6 +104,25 @@ def test_forward_mode_tangents_are_refused():
                            t5.block_scaled_mm(a, b, make(5, 40, 48)))
 
 
+@pytest.mark.gpu
+def test_saved_tensors_pass_through_hooks():
+    """What the layer keeps may be moved to the host between the passes; what does not come back as it was is
+    refused, not read."""
+    x, w = make(1, 33, 96).requires_grad_(), make(2, 50, 96).requires_grad_()
+    want = torch.autograd.grad(t5.block_scaled_linear(x, w).square().sum(), (x, w))
+    with torch.autograd.graph.save_on_cpu():
+        y = t5.block_scaled_linear(x, w).square().sum()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w)), want))
+    for unpack in (lambda t: t.cpu() if t.dtype == torch.uint8 else t, lambda t: t[:-1] if t.dtype == torch.uint8 else t,
+                   lambda t: t.float() if t.dtype == torch.uint8 else t,
+                   lambda t: torch.cat([t, t])[::2] if t.dtype == torch.uint8 else t,
+                   lambda t: torch.cat([t[:1], t])[1:] if t.dtype == torch.uint8 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = t5.block_scaled_linear(x, w).square().sum()
+        with pytest.raises(ValueError, match="came back"):
+            y.backward()
+
+
 # ------------------------------------------------------------ what is kept
 
 
