@@ -29,10 +29,21 @@ int32_t real_type(at::ScalarType t) {
   return t == at::kFloat ? T5E_REAL_F32 : t == at::kBFloat16 ? T5E_REAL_BF16 : t == at::kHalf ? T5E_REAL_F16 : -1;
 }
 
+// Refuses a tensor whose elements are no longer all there: its storage can be
+// freed under it, and kernels would read or write where it was.
+void check_stored(const Tensor& t, const char* name) {
+  if (t.numel() == 0) return;
+  int64_t last = t.storage_offset();
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  TORCH_CHECK_VALUE((int64_t)t.storage().nbytes() >= (last + 1) * (int64_t)t.itemsize(), "the memory of ", name,
+                    " was freed");
+}
+
 void check_real(const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(real_type(x.scalar_type()) >= 0, name, " must be float32, bfloat16 or float16, not ", x.scalar_type());
   TORCH_CHECK_VALUE(x.is_cuda() && x.layout() == at::kStrided, name,
                     " must be a dense tensor on a CUDA device (there is no CPU fallback)");
+  check_stored(x, name);
 }
 
 // Forward-mode derivatives are not computed: an input's would be lost, an
@@ -236,6 +247,7 @@ std::pair<Rows, Rows> quantize(const Tensor& x, int axes, int32_t fmt, int32_t b
   if (given) {
     TORCH_CHECK_VALUE(given->scalar_type() == at::kFloat && given->numel() == 1 && given->device() == device,
                       "multiplier must be a one-element float32 tensor on x's device");
+    check_stored(*given, "multiplier");
     source = given->resolve_neg();
     multiplier = r > 0 ? at::empty({1}, x.options().dtype(at::kFloat)) : source.reshape({1}).clone();
   } else if (automatic && r > 0) {
@@ -282,6 +294,7 @@ Tensor result(const optional<Tensor>& out, int64_t rows, int64_t cols, at::Scala
                     "out must have unit column stride and rows that do not overlap");
   TORCH_CHECK_VALUE(!(out->requires_grad() && at::GradMode::is_enabled()), "out must not require a gradient");
   check_no_tangent(*out, "out");
+  check_stored(*out, "out");
   TORCH_CHECK_VALUE(!out->is_neg(), "out must not be a negated view");
   return *out;
 }

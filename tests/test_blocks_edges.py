@@ -351,6 +351,26 @@ def test_rounded_rows_whose_memory_was_freed_are_refused():
             call()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 16])
+def test_tensors_whose_memory_was_freed_are_refused(offset):
+    def freed(*shape):
+        n = math.prod(shape)
+        t = torch.zeros(n + offset, device="cuda")[offset:].view(*shape)
+        t.untyped_storage().resize_(0)
+        return t
+
+    a, b = t5.quantize_blocks(make(1, 40, 64)), t5.quantize_blocks(make(2, 48, 64))
+    x, w = make(1, 40, 64), make(2, 48, 64)
+    for call in (lambda: t5.quantize_blocks(freed(40, 64)), lambda: t5.block_multiplier(freed(40, 64)),
+                 lambda: t5.quantize_blocks(x, multiplier=freed(1)), lambda: t5.block_scaled_mm(a, b, freed(40, 48)),
+                 lambda: t5.block_scaled_mm(a, b, dtype=torch.float32, out=freed(40, 48)),
+                 lambda: t5.dequantize_blocks(a, out=freed(40, 64)), lambda: t5.block_scaled_linear(freed(40, 64), w),
+                 lambda: t5.block_scaled_linear(x, freed(48, 64))):
+        with pytest.raises(ValueError, match="was freed"):
+            call()
+
+
 # ------------------------------------------------------------ roundings, value by value
 
 
