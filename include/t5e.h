@@ -380,7 +380,9 @@ int t5e_block_multiplier(int32_t type, const void* x, uint64_t rows, uint64_t co
  * `count` words) the multiplier is first computed as by t5e_block_multiplier
  * and stored to *multiplier.  With kept != NULL the multiplier that was used is
  * also stored to *kept, for a caller whose *multiplier changes later.  Where
- * there is no element nothing is stored. */
+ * there is no element nothing is stored.  A multiplier is a positive normal F32
+ * number; its value is not checked (others give NaN scales or values that do not
+ * come back). */
 typedef struct t5e_quantize {
     const void* x;
     uint64_t rows;
@@ -418,7 +420,10 @@ int t5e_dequantize_blocks(const t5e_blocks* blocks, const float* multiplier, int
  * or 8: tiles of 128 rows by up to 128, K in that many parts (at most
  * ceil(k/256)); 128 or 256: tiles of 256 rows of a by that many of b (not
  * where a has fewer rows than b and at most 128).
- * If a bounded wait inside the kernel runs out, the tile becomes NaN and
+ * Where alpha * F32(1/ma) * F32(1/mb) leaves the F32 range the result does so
+ * only if its own value does.
+ * If a bounded wait inside the kernel runs out, the tile becomes NaN, in forms
+ * 128 and 256 with the tiles that the same blocks had still to write, and
  * t5e_block_scaled_mm_expired reports it.
  */
 typedef struct t5e_block_mm {

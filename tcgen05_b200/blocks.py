@@ -113,7 +113,8 @@ class BlockScaledRows:
     of 32, zero), ``scales`` the tiled scale bytes (``tile_scales``),
     ``multiplier`` a one-element float32 tensor that the values were
     multiplied by before rounding, or None: element i of row r stands for
-    code * scale / multiplier."""
+    code * scale / multiplier.  The three tensors are held as they are, not
+    copied; a call refuses rows whose memory was freed or moved since."""
 
     __slots__ = ("_rows", "scaling", "scale_vec")
 
@@ -233,8 +234,11 @@ def quantize_blocks(x, *, axis=-1, scaling: str = "ue4m3", scale_vec: int | None
     gets the NaN scale, and everything computed from it is NaN.
 
     ``multiplier``: None (1), a positive float, a one-element float32 tensor, or
-    "auto", ``block_multiplier(x)`` found in the same call.  The result carries
-    no gradient (see ``block_scaled_linear``)."""
+    "auto", ``block_multiplier(x)`` found in the same call.  The result keeps a
+    given tensor's value of this call, whatever the tensor holds later; it has
+    to be a positive normal number, which is not checked (that would take a
+    synchronization).  The result carries no gradient (see
+    ``block_scaled_linear``)."""
     choice = _choice(scaling, scale_vec, scale_rounding)
     axes = _AXES.get(axis)
     if axes is None:
@@ -266,7 +270,7 @@ def _rows_of(q, name: str):
 def dequantize_blocks(blocks: BlockScaledRows, *, dtype=torch.float32, out=None) -> torch.Tensor:
     """The [rows, K] values code * scale / multiplier (times the reciprocal of
     the multiplier, rounded to float32) rounded to ``dtype``; into ``out`` (unit
-    column stride) if given."""
+    column stride) if given, which counts as a change in place."""
     return _ops().dequantize(_rows_of(blocks, "blocks"), dtype, out)
 
 
@@ -282,8 +286,14 @@ def block_scaled_mm(a: BlockScaledRows, b: BlockScaledRows, c=None, *, alpha: fl
     Sums are the instruction's own: float32 accumulators that take K in
     ascending steps of 64, each step truncated as ``mma_dot_batch`` models it
     word for word; where few tiles would leave the GPU idle, K is split into
-    parts that are joined in float32.  The result carries no gradient (see
-    ``block_scaled_linear``)."""
+    parts that are joined in float32.  So a float32 result is off, always toward
+    zero, by up to 2^-23 of the running sum per step, about 5e-6 of it in all at
+    K = 8192; the rounding of 16-bit results is larger.  alpha divided by the multipliers may
+    leave float32's range where the results do not.
+
+    ``c`` may not require a gradient or carry a forward-mode tangent, and the
+    result carries neither (see ``block_scaled_linear``); writing to ``out``
+    counts as a change in place."""
     return _mm(a, b, c, alpha, dtype, out, 0)
 
 
@@ -317,6 +327,8 @@ def block_scaled_linear(x, w, *, scaling: str = "ue4m3", scale_vec: int | None =
     and ``w`` [N, K] are CUDA tensors of one type; y, dx and dw have that type.
     UE4M3 forms take the "auto" multiplier for x, w and g.  x and w are read
     once each; a training step keeps their 4-bit transposes for the backward
-    pass, not the tensors.  Differentiable once."""
+    pass, not the tensors.  Differentiable once: under ``create_graph=True`` the
+    gradients require gradients, and a backward pass through them is refused.
+    Forward-mode tangents are refused."""
     choice = _choice(scaling, scale_vec, scale_rounding)
     return _ops().linear(_tensor(x, "x"), _tensor(w, "w"), choice[3], choice[4], choice[2])

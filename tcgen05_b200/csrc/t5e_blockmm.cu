@@ -1310,13 +1310,17 @@ uint32_t choose_form(uint64_t p_rows, uint64_t q_rows, uint32_t stages, bool swa
   auto tiles = [&](uint64_t rows, uint64_t cols) { return ((p_rows + rows - 1) / rows) * ((q_rows + cols - 1) / cols); };
   // Parts of K: as many as run at once, with two stages or more each; where Q is
   // one tile, two blocks an SM (1 x 8192 x 8192 in 4 parts 10.9 us, in 2 parts
-  // 12.1; 100 x 8192 x 8192 16.0 and 18.7; 48 x 14336 x 4096 whole 13.2 us, in 2
-  // parts 13.5; but 512 x 512 x 8192 in 8 parts 11.3, in 4 parts 10.0)
+  // 12.1; 100 x 8192 x 8192 16.0 and 18.7; but 512 x 512 x 8192 in 8 parts 11.3,
+  // in 4 parts 10.0).  Counting blocks is not best everywhere: the two parts it
+  // picks take 13.5 us for 48 x 14336 x 4096, whole 13.2, and for 48 x 18944 x
+  // 4096 (UE4M3) 16.3 and 15.0
   const uint64_t share = q_rows <= 128 ? 2 : 1;
   uint32_t split = 1;
   while (split < 8 && stages >= split * 4 && tiles(128, 128) * split * 2 <= share * blocks_at_once(split * 2)) split *= 2;
   if (swap || q_rows <= 64 || split >= 4) return split;
-  // Whole K in pairs: waves of tiles over the pairs, a 256-wide tile taking 1.6
+  // Whole K in pairs: waves of tiles over the pairs (the main loop alone: neither
+  // K nor the results' phase, the longer one at few stages, is counted), a
+  // 256-wide tile taking 1.6
   // times a 128-wide one (1536 x 1536 x 8192: 16.7 us in 36 tiles of 256, 15.8
   // in 72 of 128; 8192 x 4096 x 4096: 59 us in 7 waves, 81 in 14)
   const uint64_t wide = (tiles(256, 256) + pairs - 1) / pairs * 16, narrow = (tiles(256, 128) + pairs - 1) / pairs * 10;
