@@ -11,6 +11,7 @@ block-scaled calls, against the installed PyTorch and that library.
 from __future__ import annotations
 
 import os
+import shlex
 import shutil
 import subprocess
 import sys
@@ -51,9 +52,9 @@ def build_torch(verbose: bool = False, force: bool = False) -> Path | None:
     except ImportError as e:
         print(f"{TORCH_LIB.name} is left out: {e}", file=sys.stderr, flush=True)
         return None
-    cxx = os.environ.get("CXX", "g++")
-    if shutil.which(cxx) is None:
-        print(f"{TORCH_LIB.name} is left out: no C++ compiler {cxx}", file=sys.stderr, flush=True)
+    cxx = shlex.split(os.environ.get("CXX") or "g++")  # $CXX may hold a wrapper and options
+    if shutil.which(cxx[0]) is None:
+        print(f"{TORCH_LIB.name} is left out: no C++ compiler {cxx[0]}", file=sys.stderr, flush=True)
         return None
     built_for = f"torch {torch.__version__} python {sys.version_info[0]}.{sys.version_info[1]}"
     deps = [TORCH_SRC, INCLUDE / "t5e.h"]
@@ -65,7 +66,7 @@ def build_torch(verbose: bool = False, force: bool = False) -> Path | None:
     home = Path(torch.__file__).resolve().parent
     includes = [INCLUDE, sysconfig.get_paths()["include"], cuda, home / "include", home / "include/torch/csrc/api/include"]
     tmp = TORCH_LIB.with_suffix(".so.tmp")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
+    cmd = [*cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=t5e_torch",
            f'-DT5E_BUILT_FOR="t5e_torch for {built_for}"',
            *[arg for i in includes for arg in ("-isystem", str(i))], str(TORCH_SRC), "-o", str(tmp),

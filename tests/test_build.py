@@ -114,8 +114,9 @@ def test_the_extension_is_rebuilt_for_another_pytorch(monkeypatch):
     words = f"t5e_torch for torch {torch.__version__} python".encode()
     assert words in build.TORCH_LIB.read_bytes()
     monkeypatch.setattr(torch, "__version__", "0.0.1")
+    monkeypatch.setenv("CXX", "env g++ -g0")  # a command, not only a path
     build.build_torch()
-    assert len(calls) == 1 and any("t5e_torch for torch 0.0.1 python" in str(arg) for arg in calls[0])
+    assert len(calls) == 1 and calls[0][:3] == ["env", "g++", "-g0"] and any("t5e_torch for torch 0.0.1 python" in str(arg) for arg in calls[0])
 
 
 def test_an_extension_that_does_not_load_is_named(tmp_path, monkeypatch):
